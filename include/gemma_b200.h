@@ -212,6 +212,149 @@ const char* gg_last_error(const gg_engine* eng);
 int gg_sample_logits_noalloc(const float* logits, int vocab, const uint32_t* seen_bits, const gg_sample* sp,
                              double uniform, int32_t* out_token, void* stream);
 
+/* ---- Operators on device memory: rotary positions, block plans and a paged 8-bit KV cache.
+ * They have no counterpart in the reference (one f32 cache slot of the full context,
+ * engine.ts:440-447; half-split RoPE over the whole head, shaders.ts:420-467). All take device
+ * pointers on the calling thread's current device and a cudaStream_t of that device (NULL: the
+ * default stream), allocate nothing, are asynchronous and may be captured into a CUDA graph.
+ * Sizes and types are checked on the host (GG_E_ARG); what only the device sees (lengths, slots,
+ * block ids) is bounds-checked by the kernels. Messages come from gg_last_error(NULL). */
+
+#define GG_T_F32 0
+#define GG_T_BF16 1
+#define GG_T_F16 2
+
+/* A view of [rows][heads][head_dim] values: strides in elements, the head_dim values of a head
+ * next to each other, `data` aligned to its element. Any other alignment or order of rows and
+ * heads works; 16-byte aligned heads are the fastest. */
+typedef struct {
+  void* data;
+  int64_t row_stride, head_stride;
+  int32_t heads;
+  int32_t type; /* GG_T_* */
+} gg_rows;
+
+/* Rotary positions: the pair (a, b) of a row at position p becomes
+ *   (a c - b s, b c + a s),  c = mscale cos(p w_i), s = mscale sin(p w_i),  i < rot_dim / 2.
+ * GG_ROPE_HALF pairs values i and i + rot_dim / 2, GG_ROPE_INTERLEAVED 2i and 2i + 1; values from
+ * rot_dim on are copied. inverse != 0 turns back (s -> -s): the gradient of the forward call.
+ *   freqs      rot_dim / 2 device doubles, radians per position (gg_rope_freqs computes them on
+ *              the host). p w_i is formed in double precision: exact enough for any int32 p.
+ *   positions  [rows] device int32; a row at a negative position is copied unchanged (padding).
+ * q_out / k_out have the heads and types of q / k and may be the same views (in place); any other
+ * overlap is undefined. k and k_out may both be NULL. */
+#define GG_ROPE_HALF 0
+#define GG_ROPE_INTERLEAVED 1
+int gg_rope(const gg_rows* q, const gg_rows* k, const gg_rows* q_out, const gg_rows* k_out, int rows, int head_dim,
+            int rot_dim, int layout, const int32_t* positions, const double* freqs, double mscale, int inverse,
+            void* stream);
+
+/* The rot_dim / 2 frequencies of one of the scalings, host memory (no GPU involved). With
+ * w_i = theta^(-2i / rot_dim):
+ *   GG_ROPE_NONE    w_i
+ *   GG_ROPE_LINEAR  w_i / factor
+ *   GG_ROPE_BANDS   w_i where a turn is shorter than trained / high positions, w_i / factor where
+ *                   longer than trained / low, between them t w_i + (1 - t) w_i / factor with
+ *                   t = (trained w_i / 2 pi - low) / (high - low)
+ *   GG_ROPE_YARN    t w_i + (1 - t) w_i / factor, t = 1 up to the pair that turns `high` times in
+ *                   the trained positions, 0 from the pair that turns `low` times, linear in i
+ *                   between (the border pairs rounded outwards); *mscale = 0.1 ln(factor) + 1
+ * *mscale is 1 for the others. low < high; trained, low, high are ignored by the first two. */
+#define GG_ROPE_NONE 0
+#define GG_ROPE_LINEAR 1
+#define GG_ROPE_BANDS 2
+#define GG_ROPE_YARN 3
+int gg_rope_freqs(int scaling, int rot_dim, double theta, double factor, double trained, double low, double high,
+                  double* freqs, double* mscale);
+
+/* One scheduler step over `seqs` requests whose cached length goes from old_len[i] to new_len[i]:
+ * the block table, the stack of free blocks and, for every new token, its request, position and
+ * cache slot, all on the device. Request i holds blocks table[i][0 .. ceil(len / block_tokens)).
+ *   shrinking requests give their blocks back first (request order, then block order), pushed on
+ *   free_list[0 .. *free_count); then growing requests take theirs from its top, in request and
+ *   block order. Tokens old_len[i] .. new_len[i] - 1 become rows cu_rows[i] .. cu_rows[i + 1] - 1.
+ *   Outputs: cu_rows [seqs + 1], lens [seqs] (= new_len), row_seq / positions / slots [rows]
+ *   (slot = block * block_tokens + position % block_tokens; all three -1 behind the last row),
+ *   *free_count_out (may be free_count itself) and *status, a sum of GG_PLAN_* bits.
+ * All or nothing: with a status other than 0 the table, the list and the count stay as they were,
+ * lens = old_len, cu_rows is all 0 and every row is padding, so later operators do nothing. */
+#define GG_PLAN_OK 0
+#define GG_PLAN_NO_BLOCKS 1  /* the free list is too short */
+#define GG_PLAN_TOO_LONG 2   /* a new length needs more than max_blocks blocks */
+#define GG_PLAN_NO_ROWS 4    /* more new tokens than `rows` */
+#define GG_PLAN_BAD_LENGTH 8 /* a negative length, or an old one beyond max_blocks */
+#define GG_PLAN_BAD_STACK 16 /* *free_count outside 0 .. free_capacity, or no room to push */
+typedef struct {
+  const int32_t* old_len;
+  const int32_t* new_len;
+  int32_t* table; /* [seqs][table_stride], max_blocks of each row used */
+  int64_t table_stride;
+  int32_t* free_list; /* [free_capacity] */
+  const int32_t* free_count;
+  int32_t* cu_rows;
+  int32_t* lens;
+  int32_t* row_seq;
+  int32_t* positions;
+  int32_t* slots;
+  int32_t* free_count_out;
+  int32_t* status;
+  int32_t seqs, max_blocks, block_tokens, free_capacity, rows;
+} gg_block_plan;
+int gg_plan_blocks(const gg_block_plan* plan, void* stream);
+
+/* A paged KV cache in 8 bits: codes [num_blocks][kv_heads][block_tokens][head_dim], one f32 scale
+ * for each (block, head) of K and of V, [num_blocks][kv_heads]; a value is code * scale. Codes are
+ * int8 (-127..127) or e4m3 (finite). block_tokens is 16, 32, 64 or 128, head_dim a multiple of 16
+ * up to 256, num_blocks * block_tokens below 2^31, all four arrays 16-byte aligned. */
+#define GG_KV8_INT8 0
+#define GG_KV8_E4M3 1
+typedef struct {
+  void* k_codes;
+  void* v_codes;
+  float* k_scale;
+  float* v_scale;
+  int32_t num_blocks, block_tokens, kv_heads, head_dim;
+  int32_t code; /* GG_KV8_* */
+} gg_kv8_cache;
+
+/* Quantises k and v [rows][kv_heads][head_dim] into the cache at slots[row] (device int32; a slot
+ * outside 0 .. num_blocks * block_tokens - 1 skips the row). The rows of one block stand next to
+ * each other, as gg_plan_blocks lists them, and a block belongs to one request; of rows with the
+ * same slot the last one counts. For each (block, head): the scale is the smallest power of two
+ * 2^e, e >= -60, whose largest code reaches every new value (127 2^e, 448 2^e). If the first new
+ * slot is not the block's first one, the slots below it hold earlier tokens: the scale is at
+ * least the block's old one, and where it grows their codes are re-rounded to it. Slots above the
+ * new ones keep their codes. Division by a power of two is exact, so every code is off by at most
+ * half a step of the final scale per growth. A NaN or infinity makes the scale of its
+ * (block, head) NaN until the block is started anew. */
+int gg_kv8_append(const gg_kv8_cache* cache, const gg_rows* k, const gg_rows* v, const int32_t* slots, int rows,
+                  void* stream);
+
+/* The query rows of a ragged batch: rows cu_rows[i] .. cu_rows[i + 1] - 1 are the last tokens of
+ * request i, whose cache holds lens[i] tokens in blocks table[i][...]. max_rows and max_len are at
+ * least every request's number of rows and length (longer ones: rows from max_rows on are not
+ * computed, keys from max_len on not read). A table entry outside 0 .. num_blocks - 1 hides its
+ * keys. Rows outside cu_rows[0] .. cu_rows[seqs] - 1 are left as they were. */
+typedef struct {
+  const int32_t* cu_rows; /* [seqs + 1], ascending */
+  const int32_t* lens;    /* [seqs] */
+  const int32_t* table;   /* [seqs][table_stride] */
+  int64_t table_stride;
+  int32_t seqs, rows, max_rows, max_len;
+} gg_kv8_batch;
+
+/* Attention over the cache: the row at position p = lens[i] - (rows of i) + r sees the keys at
+ * max(0, p - window + 1) .. p (window 0: from 0), o = sum softmax(scale q k) v; query head h reads
+ * key head h / (q heads / kv_heads). A row that sees no key gives zeros. lse (f32, [rows][q heads],
+ * or NULL) receives ln sum exp(scale q k), -inf for such a row. out has q's type. Scores, softmax
+ * and sums are held in f32. `workspace`: gg_kv8_attention_workspace bytes, 16-byte aligned, for
+ * this call alone until it has run (calls that may run at the same time need one each). */
+int gg_kv8_attention(const gg_kv8_cache* cache, const gg_rows* q, const gg_rows* out, float* lse,
+                     const gg_kv8_batch* batch, double scale, int window, void* workspace, size_t workspace_bytes,
+                     void* stream);
+int gg_kv8_attention_workspace(const gg_kv8_cache* cache, const gg_rows* q, const gg_kv8_batch* batch, int window,
+                               size_t* bytes);
+
 /* ---- Tokenizer (host only; no GPU involved). Replaces src/tokenizer.ts: the greedy
  * longest-match encoder the reference runs in JavaScript, with its UTF-16 code-unit semantics
  * (lengths, prefix search and the skip over unknown input count UTF-16 units). Strings cross

@@ -50,6 +50,12 @@ SIGNATURES = {
     "gg_selftest_wait": (_I, [_P, ctypes.c_uint64]),
     "gg_set_gemm_kernel": (_I, [_I]),
     "gg_sample_logits_noalloc": (_I, [_P, _I, _P, _P, _D, _P, _P]),
+    "gg_rope": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _D, _I, _P]),
+    "gg_rope_freqs": (_I, [_I, _I, _D, _D, _D, _D, _D, _P, ctypes.POINTER(_D)]),
+    "gg_plan_blocks": (_I, [_P, _P]),
+    "gg_kv8_append": (_I, [_P, _P, _P, _P, _I, _P]),
+    "gg_kv8_attention": (_I, [_P, _P, _P, _P, _P, _D, _I, _P, ctypes.c_size_t, _P]),
+    "gg_kv8_attention_workspace": (_I, [_P, _P, _P, _I, ctypes.POINTER(ctypes.c_size_t)]),
     "gg_set_timeout": (_I, [_P, ctypes.c_uint64]),
     "gg_last_device_ms": (_I, [_P, ctypes.POINTER(ctypes.c_float)]),
     "gg_destroy": (_I, [_P]),
@@ -68,6 +74,37 @@ GG_FLAG_SERIAL_PREFILL = 1  # prefill one token per launch (the reference's orde
 
 class GGSample(ctypes.Structure):
     _fields_ = [("temperature", ctypes.c_double), ("top_p", ctypes.c_double), ("rep_penalty", ctypes.c_double)]
+
+
+# Views and batches of the operators on device memory (include/gemma_b200.h)
+GG_T_F32, GG_T_BF16, GG_T_F16 = 0, 1, 2
+GG_ROPE_HALF, GG_ROPE_INTERLEAVED = 0, 1
+GG_ROPE_NONE, GG_ROPE_LINEAR, GG_ROPE_BANDS, GG_ROPE_YARN = 0, 1, 2, 3
+GG_KV8_INT8, GG_KV8_E4M3 = 0, 1
+GG_PLAN_OK, GG_PLAN_NO_BLOCKS, GG_PLAN_TOO_LONG, GG_PLAN_NO_ROWS, GG_PLAN_BAD_LENGTH, GG_PLAN_BAD_STACK = 0, 1, 2, 4, 8, 16
+
+
+class GGRows(ctypes.Structure):
+    _fields_ = [("data", _P), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("heads", ctypes.c_int32), ("type", ctypes.c_int32)]
+
+
+class GGBlockPlan(ctypes.Structure):
+    _fields_ = ([("old_len", _P), ("new_len", _P), ("table", _P), ("table_stride", ctypes.c_int64)]
+                + [(n, _P) for n in ("free_list", "free_count", "cu_rows", "lens", "row_seq", "positions", "slots",
+                                     "free_count_out", "status")]
+                + [(n, ctypes.c_int32) for n in ("seqs", "max_blocks", "block_tokens", "free_capacity", "rows")])
+
+
+class GGKv8Cache(ctypes.Structure):
+    _fields_ = ([(n, _P) for n in ("k_codes", "v_codes", "k_scale", "v_scale")]
+                + [(n, ctypes.c_int32) for n in ("num_blocks", "block_tokens", "kv_heads", "head_dim", "code")])
+
+
+class GGKv8Batch(ctypes.Structure):
+    _fields_ = [("cu_rows", _P), ("lens", _P), ("table", _P), ("table_stride", ctypes.c_int64),
+                ("seqs", ctypes.c_int32), ("rows", ctypes.c_int32), ("max_rows", ctypes.c_int32),
+                ("max_len", ctypes.c_int32)]
 
 
 class GemmaB200Error(RuntimeError):
