@@ -242,12 +242,17 @@ typedef struct {
  *              the host). p w_i is formed in double precision: exact enough for any int32 p.
  *   positions  [rows] device int32; a row at a negative position is copied unchanged (padding).
  * q_out / k_out have the heads and types of q / k and may be the same views (in place); any other
- * overlap is undefined. k and k_out may both be NULL. */
+ * overlap is undefined. k.data and k_out.data may both be NULL: no keys. */
 #define GG_ROPE_HALF 0
 #define GG_ROPE_INTERLEAVED 1
-int gg_rope(const gg_rows* q, const gg_rows* k, const gg_rows* q_out, const gg_rows* k_out, int rows, int head_dim,
-            int rot_dim, int layout, const int32_t* positions, const double* freqs, double mscale, int inverse,
-            void* stream);
+typedef struct {
+  gg_rows q, k, q_out, k_out;
+  const int32_t* positions;
+  const double* freqs;
+  double mscale;
+  int32_t rows, head_dim, rot_dim, layout, inverse;
+} gg_rope_call;
+int gg_rope(const gg_rope_call* call, void* stream);
 
 /* The rot_dim / 2 frequencies of one of the scalings, host memory (no GPU involved). With
  * w_i = theta^(-2i / rot_dim):
@@ -327,33 +332,40 @@ typedef struct {
  * new ones keep their codes. Division by a power of two is exact, so every code is off by at most
  * half a step of the final scale per growth. A NaN or infinity makes the scale of its
  * (block, head) NaN until the block is started anew. */
-int gg_kv8_append(const gg_kv8_cache* cache, const gg_rows* k, const gg_rows* v, const int32_t* slots, int rows,
-                  void* stream);
-
-/* The query rows of a ragged batch: rows cu_rows[i] .. cu_rows[i + 1] - 1 are the last tokens of
- * request i, whose cache holds lens[i] tokens in blocks table[i][...]. max_rows and max_len are at
- * least every request's number of rows and length (longer ones: rows from max_rows on are not
- * computed, keys from max_len on not read). A table entry outside 0 .. num_blocks - 1 hides its
- * keys. Rows outside cu_rows[0] .. cu_rows[seqs] - 1 are left as they were. */
 typedef struct {
+  gg_rows k, v;
+  const int32_t* slots;
+  int32_t rows;
+} gg_kv8_append_call;
+int gg_kv8_append(const gg_kv8_cache* cache, const gg_kv8_append_call* call, void* stream);
+
+/* Attention of the query rows of a ragged batch over the cache. Rows cu_rows[i] .. cu_rows[i + 1] - 1
+ * are the last tokens of request i, whose cache holds lens[i] tokens in blocks table[i][...]; the row
+ * at position p = lens[i] - (rows of i) + r sees the keys at max(0, p - window + 1) .. p (window 0:
+ * from 0): o = sum softmax(scale q k) v; query head h reads key head h / (q heads / kv_heads). A row
+ * that sees no key gives zeros. lse (f32, [rows][q heads], or NULL) receives ln sum exp(scale q k),
+ * -inf for such a row. out has q's type. Scores, softmax and sums are held in f32.
+ *   max_rows and max_len are at least every request's number of rows and length (of longer ones,
+ *   rows from max_rows on are not computed and keys from max_len on not read); a table entry outside
+ *   0 .. num_blocks - 1 hides its keys; rows outside cu_rows[0] .. cu_rows[seqs] - 1 are left as
+ *   they were. workspace: gg_kv8_attention_workspace bytes, 16-byte aligned, for this call alone
+ *   until it has run (calls that may run at the same time need one each). */
+typedef struct {
+  gg_rows q, out;
+  float* lse;
   const int32_t* cu_rows; /* [seqs + 1], ascending */
   const int32_t* lens;    /* [seqs] */
   const int32_t* table;   /* [seqs][table_stride] */
   int64_t table_stride;
-  int32_t seqs, rows, max_rows, max_len;
-} gg_kv8_batch;
-
-/* Attention over the cache: the row at position p = lens[i] - (rows of i) + r sees the keys at
- * max(0, p - window + 1) .. p (window 0: from 0), o = sum softmax(scale q k) v; query head h reads
- * key head h / (q heads / kv_heads). A row that sees no key gives zeros. lse (f32, [rows][q heads],
- * or NULL) receives ln sum exp(scale q k), -inf for such a row. out has q's type. Scores, softmax
- * and sums are held in f32. `workspace`: gg_kv8_attention_workspace bytes, 16-byte aligned, for
- * this call alone until it has run (calls that may run at the same time need one each). */
-int gg_kv8_attention(const gg_kv8_cache* cache, const gg_rows* q, const gg_rows* out, float* lse,
-                     const gg_kv8_batch* batch, double scale, int window, void* workspace, size_t workspace_bytes,
-                     void* stream);
-int gg_kv8_attention_workspace(const gg_kv8_cache* cache, const gg_rows* q, const gg_kv8_batch* batch, int window,
-                               size_t* bytes);
+  void* workspace;
+  size_t workspace_bytes;
+  double scale;
+  int32_t seqs, rows, max_rows, max_len, window;
+} gg_kv8_attention_call;
+int gg_kv8_attention(const gg_kv8_cache* cache, const gg_kv8_attention_call* call, void* stream);
+/* Bytes of workspace that a call of these sizes needs: of `call`, q.heads, q.type, seqs, rows, max_rows,
+ * max_len and window are read. */
+int gg_kv8_attention_workspace(const gg_kv8_cache* cache, const gg_kv8_attention_call* call, size_t* bytes);
 
 /* ---- Tokenizer (host only; no GPU involved). Replaces src/tokenizer.ts: the greedy
  * longest-match encoder the reference runs in JavaScript, with its UTF-16 code-unit semantics

@@ -11,7 +11,7 @@ import pytest
 import ops_reference as ref
 from conftest import ROOT
 from gemma_b200 import native
-from gemma_b200.native import GGBlockPlan, GGKv8Batch, GGKv8Cache, GGRows
+from gemma_b200.native import GGBlockPlan, GGKv8AppendCall, GGKv8AttentionCall, GGKv8Cache, GGRopeCall, GGRows
 
 P = 4096  # stands for a device pointer: never read
 
@@ -33,8 +33,14 @@ def cache(**kw):
                                   kv_heads=4, head_dim=256, code=0), **kw))
 
 
-def batch(**kw):
-    return GGKv8Batch(**dict(dict(cu_rows=P, lens=P, table=P, table_stride=8, seqs=2, rows=2, max_rows=1, max_len=128), **kw))
+def attend(q=None, out=None, **kw):
+    return GGKv8AttentionCall(**dict(dict(q=q or rows(), out=out or rows(), cu_rows=P, lens=P, table=P, table_stride=8, workspace=P,
+                                          workspace_bytes=1 << 40, scale=0.1, seqs=2, rows=2, max_rows=1, max_len=128), **kw))
+
+
+def append(lib, c, k, v, slots=P, n=3):
+    call = GGKv8AppendCall(k, v, slots, n)
+    return lib.gg_kv8_append(ctypes.byref(c), ctypes.byref(call), None)
 
 
 def refused(lib, rc, *words):
@@ -50,11 +56,9 @@ def refused(lib, rc, *words):
     (dict(head_dim=0), "head_dim"), (dict(kv_heads=0), "kv_heads"), (dict(num_blocks=0), "num_blocks"),
     (dict(num_blocks=1 << 27, block_tokens=16), "num_blocks"), (dict(code=2), "code 2")])
 def test_cache_refused(lib, kw, word):
-    k = rows()
     c = cache(**kw)
-    refused(lib, lib.gg_kv8_append(ctypes.byref(c), ctypes.byref(k), ctypes.byref(k), P, 3, None), "gg_kv8_append", word)
-    q, b = rows(), batch()
-    refused(lib, lib.gg_kv8_attention(ctypes.byref(c), ctypes.byref(q), ctypes.byref(q), None, ctypes.byref(b), 0.1, 0, P, 1 << 30, None), word)
+    refused(lib, append(lib, c, rows(), rows()), "gg_kv8_append", word)
+    refused(lib, lib.gg_kv8_attention(ctypes.byref(c), ctypes.byref(attend()), None), word)
 
 
 @pytest.mark.parametrize("kw, word", [
@@ -62,45 +66,43 @@ def test_cache_refused(lib, kw, word):
     (dict(data=P + 2), "aligned"), (dict(row_stride=-1024), "negative"), (dict(head_stride=255), "overlap"),
     (dict(row_stride=255), "overlap"), (dict(type=1), "different types")])
 def test_append_rows_refused(lib, kw, word):
-    c, k, v = cache(), rows(**kw), rows()
-    refused(lib, lib.gg_kv8_append(ctypes.byref(c), ctypes.byref(k), ctypes.byref(v), P, 3, None), word)
-    refused(lib, lib.gg_kv8_append(ctypes.byref(c), ctypes.byref(v), ctypes.byref(v), P, -1, None), "rows")
-    refused(lib, lib.gg_kv8_append(ctypes.byref(c), None, ctypes.byref(v), P, 3, None), "null")
-    refused(lib, lib.gg_kv8_append(ctypes.byref(c), ctypes.byref(v), ctypes.byref(v), None, 3, None), "null")
+    c, v = cache(), rows()
+    refused(lib, append(lib, c, rows(**kw), v), word)
+    refused(lib, append(lib, c, v, v, n=-1), "rows")
+    refused(lib, append(lib, c, v, v, slots=None), "null")
+    refused(lib, lib.gg_kv8_append(ctypes.byref(c), None, None), "null")
 
 
-@pytest.mark.parametrize("bkw, qkw, okw, window, scale, word", [
-    (dict(table_stride=7), {}, {}, 0, 0.1, "table_stride 7"), (dict(seqs=-1), {}, {}, 0, 0.1, "seqs -1"),
-    (dict(max_len=-1), {}, {}, 0, 0.1, "max_len"), (dict(lens=None), {}, {}, 0, 0.1, "null array"),
-    ({}, dict(heads=6), dict(heads=6), 0, 0.1, "6 query heads over 4"), ({}, {}, dict(type=2), 0, 0.1, "another type"),
-    ({}, {}, {}, -1, 0.1, "window"), ({}, {}, {}, 0, math.nan, "scale"), ({}, {}, {}, 0, math.inf, "scale"),
-    (dict(seqs=1 << 20, rows=1 << 20, max_rows=1 << 20), {}, {}, 0, 0.1, "tiles")])
-def test_attention_refused(lib, bkw, qkw, okw, window, scale, word):
-    c, q, o, b = cache(), rows(**qkw), rows(**okw), batch(**bkw)
-    refused(lib, lib.gg_kv8_attention(ctypes.byref(c), ctypes.byref(q), ctypes.byref(o), None, ctypes.byref(b), scale, window,
-                                      P, 1 << 40, None), word)
+@pytest.mark.parametrize("kw, qkw, okw, word", [
+    (dict(table_stride=7), {}, {}, "table_stride 7"), (dict(seqs=-1), {}, {}, "seqs -1"), (dict(max_len=-1), {}, {}, "max_len"),
+    (dict(lens=None), {}, {}, "null array"), ({}, dict(heads=6), dict(heads=6), "6 query heads over 4"), ({}, {}, dict(type=2), "another type"),
+    ({}, dict(type=5), {}, "q.type 5"), (dict(window=-1), {}, {}, "window"), (dict(scale=math.nan), {}, {}, "scale"),
+    (dict(scale=math.inf), {}, {}, "scale"), (dict(seqs=1 << 20, rows=1 << 20, max_rows=1 << 20), {}, {}, "tiles")])
+def test_attention_refused(lib, kw, qkw, okw, word):
+    c, call = cache(), attend(rows(**qkw), rows(**okw), **kw)
+    refused(lib, lib.gg_kv8_attention(ctypes.byref(c), ctypes.byref(call), None), word)
 
 
-def test_attention_workspace_refused(lib):
-    c, q, b = cache(), rows(), batch(max_len=128 * 16, table_stride=128)
+@pytest.mark.parametrize("n, max_rows", [(2, 1), (300, 300)])
+def test_attention_workspace_refused(lib, n, max_rows):
+    c, call = cache(), attend(max_len=128 * 16, table_stride=128, rows=n, max_rows=max_rows)
     need = ctypes.c_size_t()
-    assert lib.gg_kv8_attention_workspace(ctypes.byref(c), ctypes.byref(q), ctypes.byref(b), 0, ctypes.byref(need)) == 0
+    assert lib.gg_kv8_attention_workspace(ctypes.byref(c), ctypes.byref(call), ctypes.byref(need)) == 0
     assert need.value > 0
-    call = lambda ws, n: lib.gg_kv8_attention(ctypes.byref(c), ctypes.byref(q), ctypes.byref(q), None, ctypes.byref(b), 0.1, 0, ws, n, None)  # noqa: E731
-    refused(lib, call(P, need.value - 1), "workspace")
-    refused(lib, call(None, need.value), "workspace")
-    refused(lib, call(P + 8, need.value), "workspace")
+    for ws, size in ((P, need.value - 1), (None, need.value), (P + 8, need.value)):
+        call.workspace, call.workspace_bytes = ws, size
+        refused(lib, lib.gg_kv8_attention(ctypes.byref(c), ctypes.byref(call), None), "workspace")
 
 
 @pytest.mark.parametrize("kw, word", [
-    (dict(head_dim=0), "head_dim"), (dict(rot=3), "rot_dim 3"), (dict(rot=258), "rot_dim"), (dict(rot=0), "rot_dim"),
-    (dict(layout=2), "layout"), (dict(rows=-1), "rows"), (dict(pos=None), "null"), (dict(freqs=None), "null"),
-    (dict(k_out=None), "null"), (dict(ko=dict(heads=2)), "heads"), (dict(ko=dict(type=1)), "another type")])
+    (dict(head_dim=0), "head_dim"), (dict(rot_dim=3), "rot_dim 3"), (dict(rot_dim=258), "rot_dim"), (dict(rot_dim=0), "rot_dim"),
+    (dict(layout=2), "layout"), (dict(rows=-1), "rows"), (dict(positions=None), "null"), (dict(freqs=None), "null"),
+    (dict(k_out=rows(data=None)), "null"), (dict(k_out=rows(heads=2)), "heads"), (dict(k_out=rows(type=1)), "another type"),
+    (dict(q=rows(type=9)), "q.type 9")])
 def test_rope_refused(lib, kw, word):
-    q, k, ko = rows(), rows(), rows(**kw.get("ko", {}))
-    k_out = ctypes.byref(ko) if kw.get("k_out", 1) else None
-    refused(lib, lib.gg_rope(ctypes.byref(q), ctypes.byref(k), ctypes.byref(q), k_out, kw.get("rows", 2), kw.get("head_dim", 256),
-                             kw.get("rot", 256), kw.get("layout", 0), kw.get("pos", P), kw.get("freqs", P), 1.0, 0, None), word)
+    call = GGRopeCall(**dict(dict(q=rows(), k=rows(), q_out=rows(), k_out=rows(), positions=P, freqs=P, mscale=1.0, rows=2, head_dim=256,
+                                  rot_dim=256), **kw))
+    refused(lib, lib.gg_rope(ctypes.byref(call), None), word)
 
 
 PLAN = dict(old_len=P, new_len=P, table=P, table_stride=8, free_list=P, free_count=P, cu_rows=P, lens=2 * P, row_seq=P,
@@ -118,10 +120,11 @@ def test_plan_refused(lib, kw, word):
 
 def test_rows_of_nothing_are_fine(lib):
     """Zero rows: accepted, and nothing is launched (there is no GPU here)."""
-    c, k, b = cache(), rows(), batch(rows=0)
-    assert lib.gg_kv8_append(ctypes.byref(c), ctypes.byref(k), ctypes.byref(k), P, 0, None) == 0
-    assert lib.gg_rope(ctypes.byref(k), None, ctypes.byref(k), None, 0, 256, 256, 0, P, P, 1.0, 0, None) == 0
-    assert lib.gg_kv8_attention(ctypes.byref(c), ctypes.byref(k), ctypes.byref(k), None, ctypes.byref(b), 0.1, 0, None, 0, None) == 0
+    c, k = cache(), rows()
+    assert append(lib, c, k, k, n=0) == 0
+    call = GGRopeCall(q=k, q_out=k, positions=P, freqs=P, mscale=1.0, rows=0, head_dim=256, rot_dim=256)
+    assert lib.gg_rope(ctypes.byref(call), None) == 0
+    assert lib.gg_kv8_attention(ctypes.byref(c), ctypes.byref(attend(rows=0)), None) == 0
 
 
 def freqs(lib, scaling, rot, theta=1e6, factor=8.0, trained=8192.0, low=1.0, high=4.0):
@@ -169,7 +172,8 @@ def test_frequencies_refused(lib, kw, word):
 
 
 def test_structures_match_the_header(tmp_path):
-    structs = {"gg_rows": GGRows, "gg_block_plan": GGBlockPlan, "gg_kv8_cache": GGKv8Cache, "gg_kv8_batch": GGKv8Batch}
+    structs = {"gg_rows": GGRows, "gg_block_plan": GGBlockPlan, "gg_kv8_cache": GGKv8Cache,
+               "gg_rope_call": GGRopeCall, "gg_kv8_append_call": GGKv8AppendCall, "gg_kv8_attention_call": GGKv8AttentionCall}
     consts = ["GG_T_F32", "GG_T_BF16", "GG_T_F16", "GG_ROPE_HALF", "GG_ROPE_INTERLEAVED", "GG_ROPE_NONE", "GG_ROPE_LINEAR",
               "GG_ROPE_BANDS", "GG_ROPE_YARN", "GG_KV8_INT8", "GG_KV8_E4M3", "GG_PLAN_OK", "GG_PLAN_NO_BLOCKS", "GG_PLAN_TOO_LONG",
               "GG_PLAN_NO_ROWS", "GG_PLAN_BAD_LENGTH", "GG_PLAN_BAD_STACK"]
@@ -188,6 +192,18 @@ def test_structures_match_the_header(tmp_path):
             assert int(got[f"{n}.{f}"]) == getattr(c, f).offset, (n, f)
     for c in consts:
         assert int(got[c]) == getattr(native, c), c
+    # the packed forms that gemma_b200.ops hands over
+    ops = pytest.importorskip("gemma_b200.ops")
+    n = range(1, 100)
+    for pack, c, count in ((ops._pack_plan, GGBlockPlan, 18), (ops._pack_rope, GGRopeCall, 28), (ops._pack_append, GGKv8AppendCall, 12),
+                           (ops._pack_attend, GGKv8AttentionCall, 23)):
+        raw = pack(*n[:count])
+        assert len(raw) == ctypes.sizeof(c)
+        flat = []
+        for f, t in c._fields_:
+            v = getattr(c.from_buffer_copy(raw), f)
+            flat += [getattr(v, g) for g, _ in GGRows._fields_] if t is GGRows else [v]
+        assert flat == list(n[:count]), c
 
 
 def test_reference_codes():

@@ -13,139 +13,10 @@
 // (22 bits) and so are their weights: the lo rows fill the half of the 16-row MMA tile that few
 // query rows leave empty, and the two halves are added in registers. f16 and bf16 queries are exact
 // in one f16; their weights are rounded to f16 (2^-12 relative, below the output's own 2^-9 / 2^-12).
-#include <cuda_fp8.h>
+#include "gg_kv8.h"
 
-#include "gg_launch.h"
-#include "gg_ops.h"
 
 namespace gg {
-
-constexpr float KV8_SLACK = 8.f;    // w_j <= 2^8
-constexpr float KV8_WMUL = 128.f;    // weights enter the MMA as w_j 2^7 <= 2^15
-constexpr float KV8_NEG = -1e30f;   // stands for -inf in running maxima (no inf - inf)
-
-struct Kv8Args {
-  const uint8_t *kc, *vc;
-  const float *ks, *vs;
-  const void* q;
-  void* out;
-  float* lse;
-  const int32_t *cu, *lens, *table;
-  float* part_o;    // [row][head][split][hd]
-  float2* part_ml;  // [row][head][split]: r, l
-  long long q_row, q_head, o_row, o_head, table_stride;
-  float scale_log2;
-  int seqs, rows, max_rows, max_len, num_blocks, block_shift, kv_heads, group, hd, window, q_type;
-  int row_tiles, splits, split_steps;
-  int q_vec;  // every head of q starts on a 16-byte boundary
-};
-
-GG_DEV float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-GG_DEV void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
-GG_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {  // bytes 0: fills zeros, reads nothing
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-GG_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-GG_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-GG_DEV uint32_t half2_bits(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-// f32 pair -> f16 hi pair and the f16 pair of what hi leaves.
-GG_DEV void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(a, b);
-  const float2 f = __half22float2(h);
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = half2_bits(a - f.x, b - f.y);
-}
-
-GG_DEV uint32_t hsub2_bits(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-GG_DEV uint32_t e4m3x2_f16x2(uint32_t two) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"((unsigned short)two));
-  return d;
-}
-// Four codes next to each other -> (0, 1) and (2, 3) as f16 pairs. int8: byte + 128 in the mantissa
-// of 1024 (f16 0x6400, steps of 1), minus 1152.
-template <int CODE>
-GG_DEV void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (CODE == GG_KV8_INT8) {
-    w ^= 0x80808080u;
-    lo = hsub2_bits(__byte_perm(w, 0x64646464u, 0x4140), 0x64806480u);
-    hi = hsub2_bits(__byte_perm(w, 0x64646464u, 0x4342), 0x64806480u);
-  } else {
-    lo = e4m3x2_f16x2(w);
-    hi = e4m3x2_f16x2(w >> 16);
-  }
-}
-// Words a and b of two keys (four dims each) -> for each dim the f16 pair (a, b).
-template <int CODE>
-GG_DEV void widen4_pairs(uint32_t a, uint32_t b, uint32_t (&d)[4]) {
-  if constexpr (CODE == GG_KV8_INT8) {
-    const uint32_t x = __byte_perm(a, b, 0x5140) ^ 0x80808080u, y = __byte_perm(a, b, 0x7362) ^ 0x80808080u;
-    d[0] = hsub2_bits(__byte_perm(x, 0x64646464u, 0x4140), 0x64806480u);
-    d[1] = hsub2_bits(__byte_perm(x, 0x64646464u, 0x4342), 0x64806480u);
-    d[2] = hsub2_bits(__byte_perm(y, 0x64646464u, 0x4140), 0x64806480u);
-    d[3] = hsub2_bits(__byte_perm(y, 0x64646464u, 0x4342), 0x64806480u);
-  } else {
-    const uint32_t a0 = e4m3x2_f16x2(a), a1 = e4m3x2_f16x2(a >> 16), b0 = e4m3x2_f16x2(b), b1 = e4m3x2_f16x2(b >> 16);
-    d[0] = __byte_perm(a0, b0, 0x5410);
-    d[1] = __byte_perm(a0, b0, 0x7632);
-    d[2] = __byte_perm(a1, b1, 0x5410);
-    d[3] = __byte_perm(a1, b1, 0x7632);
-  }
-}
-
-GG_DEV float load_elem(const void* p, int type, long long i) {
-  if (type == GG_T_F32) return static_cast<const float*>(p)[i];
-  if (type == GG_T_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(static_cast<const __half*>(p)[i]);
-}
-GG_DEV void store_elem(void* p, int type, long long i, float v) {
-  if (type == GG_T_F32) static_cast<float*>(p)[i] = v;
-  else if (type == GG_T_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-  else static_cast<__half*>(p)[i] = __float2half_rn(v);
-}
-// Four elements from i on (a multiple of four).
-GG_DEV float4 load_elem4(const void* p, int type, long long i, int vec) {
-  if (!vec) return make_float4(load_elem(p, type, i), load_elem(p, type, i + 1), load_elem(p, type, i + 2), load_elem(p, type, i + 3));
-  if (type == GG_T_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-  const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
-  if (type == GG_T_BF16)
-    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-  return make_float4(a.x, a.y, b.x, b.y);
-}
-
-// The rows of request s: first row, number of rows (within the batch and max_rows), length.
-struct Kv8Seq {
-  int row0, n, len;
-  long long first_pos;  // position of row row0
-};
-GG_DEV Kv8Seq kv8_seq(const Kv8Args& a, int s) {
-  Kv8Seq q;
-  const int c0 = a.cu[s], c1 = a.cu[s + 1], len = max(a.lens[s], 0);
-  q.row0 = max(c0, 0);
-  q.n = max(min(c1, a.rows) - q.row0, 0);
-  q.first_pos = (long long)len - (c1 - c0);
-  q.n = min(q.n, a.max_rows);
-  q.len = min(len, a.max_len);
-  return q;
-}
 
 // ------------------------------------------------------------------------------ few rows
 //
@@ -486,8 +357,8 @@ __global__ void __launch_bounds__(128) gg_kv8_merge_kernel(const Kv8Args a) {
   long long x = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int hq = (int)(x % heads);
   x /= heads;
-  const int tok = (int)(x % a.max_rows);
-  x /= a.max_rows;
+  const int tok = (int)(x % a.merge_tokens);
+  x /= a.merge_tokens;
   if (x >= a.seqs) return;
   const Kv8Seq sq = kv8_seq(a, (int)x);
   if (tok >= sq.n) return;
@@ -509,10 +380,8 @@ __global__ void __launch_bounds__(128) gg_kv8_merge_kernel(const Kv8Args a) {
 template <int HD, int CODE, bool HILO>
 cudaError_t launch_rows(const Kv8Args& a, cudaStream_t s) {
   auto* k = gg_kv8_rows_kernel<HD, CODE, HILO>;
-  cudaError_t r = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, RowsShape<HD>::SMEM);
-  if (r != cudaSuccess) return r;
   const long long grid = (long long)a.seqs * a.kv_heads * a.row_tiles * a.splits;
-  return launch_pdl(k, dim3((unsigned)grid), dim3(KV8_WARPS * 32), RowsShape<HD>::SMEM, s, a);
+  return launch_big_smem(k, dim3((unsigned)grid), dim3(KV8_WARPS * 32), RowsShape<HD>::SMEM, s, a);
 }
 template <int HD>
 cudaError_t launch_rows_hd(const Kv8Args& a, int code, cudaStream_t s) {
@@ -521,118 +390,148 @@ cudaError_t launch_rows_hd(const Kv8Args& a, int code, cudaStream_t s) {
   return hilo ? launch_rows<HD, GG_KV8_E4M3, true>(a, s) : launch_rows<HD, GG_KV8_E4M3, false>(a, s);
 }
 
-// How a call is cut: row tiles of a request and head, key ranges, steps of a range.
-struct Kv8Plan {
-  int row_tiles, splits, split_steps;
+// How a call is cut. Requests with few rows (rows * group up to KV8_FEW) take the kernel above, the
+// others the one of gg_kv8_prompt.cu; a call that may hold both launches both, and each skips the
+// other's requests.
+constexpr int KV8_FEW = 32;
+
+struct Kv8Cut {
+  int row_tiles = 0, splits = 0, split_steps = 1;  // row_tiles 0: not launched
+  size_t parts = 0;                                // partial results
 };
-static Kv8Plan kv8_plan(const gg_kv8_cache& c, const gg_rows& q, const gg_kv8_batch& b, int window) {
-  Kv8Plan p;
-  const int rt = q.type == GG_T_F32 ? 8 : 16;
-  const long long items = (long long)b.max_rows * (q.heads / c.kv_heads);
-  p.row_tiles = (int)((items + rt - 1) / rt);
+static Kv8Cut kv8_cut(long long items, int tile, long long slots, int least_steps, long long rows, int q_heads,
+                      const gg_kv8_cache& c, const gg_kv8_attention_call& b) {
+  Kv8Cut p;
+  p.row_tiles = (int)((items + tile - 1) / tile);
   // keys that a tile may read: all, or its window with the rows between its first and last
   long long keys = b.max_len;
-  if (window) keys = keys < (long long)window + rt + 2 * KV8_STEP ? keys : (long long)window + rt + 2 * KV8_STEP;
+  if (b.window && keys > (long long)b.window + tile + 2 * KV8_STEP) keys = (long long)b.window + tile + 2 * KV8_STEP;
   const long long steps = (keys + KV8_STEP - 1) / KV8_STEP;
   const long long units = (long long)b.seqs * c.kv_heads * p.row_tiles;
-  // two CTAs fit an SM; four waves of them even out requests of different lengths
-  long long splits = (148 * 2 * 4 + units - 1) / units;
-  const long long most = (steps + 2 * KV8_WARPS - 1) / (2 * KV8_WARPS);  // at least two steps for each warp
+  long long splits = units ? (slots + units - 1) / units : 1;
+  const long long most = (steps + least_steps - 1) / least_steps;
   if (splits > most) splits = most;
   if (splits < 1) splits = 1;
   p.split_steps = (int)((steps + splits - 1) / splits);
   if (p.split_steps < 1) p.split_steps = 1;
   p.splits = (int)((steps + p.split_steps - 1) / p.split_steps);
   if (p.splits < 1) p.splits = 1;
+  if (p.splits > 1) p.parts = (size_t)rows * q_heads * p.splits;
   return p;
 }
-static size_t kv8_bytes(const Kv8Plan& p, const gg_kv8_cache& c, const gg_rows& q, const gg_kv8_batch& b) {
-  if (p.splits == 1) return 0;
-  const size_t parts = (size_t)b.rows * q.heads * p.splits;
-  return parts * c.head_dim * 4 + parts * 8;
+struct Kv8Plan {
+  Kv8Cut few, many;
+  size_t few_bytes, bytes;
+};
+static Kv8Plan kv8_plan(const gg_kv8_cache& c, const gg_kv8_attention_call& b) {
+  Kv8Plan p;
+  const int group = b.q.heads / c.kv_heads;
+  const long long items = (long long)b.max_rows * group;
+  // few rows: two CTAs fit an SM; four waves of them even out requests of different lengths; at
+  // least two steps for each warp. Many rows: one CTA an SM, at least 512 keys.
+  p.few = kv8_cut(items < KV8_FEW ? items : KV8_FEW, b.q.type == GG_T_F32 ? 8 : 16, 148 * 2 * 4, 2 * KV8_WARPS, b.rows, b.q.heads, c, b);
+  if (items > KV8_FEW) p.many = kv8_cut(items, kv8_prompt_tile(c.head_dim), 148, 32, b.rows, b.q.heads, c, b);
+  const auto bytes = [&](const Kv8Cut& k) { return k.parts * c.head_dim * 4 + k.parts * 8; };
+  p.few_bytes = bytes(p.few);
+  p.bytes = p.few_bytes + bytes(p.many);
+  return p;
 }
 
-static int kv8_check(const char* fn, const gg_kv8_cache* c, const gg_rows* q, const gg_kv8_batch* b, int window) {
+static int kv8_check(const char* fn, const gg_kv8_cache* c, const gg_kv8_attention_call* b) {
   if (int rc = ops_check_cache(fn, c)) return rc;
-  if (int rc = ops_check_rows(fn, "q", q, b->rows, c->head_dim)) return rc;
-  if (q->heads % c->kv_heads) return ops_fail(GG_E_ARG, "%s: %d query heads over %d key heads", fn, q->heads, c->kv_heads);
-  if (!b->cu_rows || !b->lens || !b->table) return ops_fail(GG_E_ARG, "%s: null array in the batch", fn);
+  if (b->q.type < GG_T_F32 || b->q.type > GG_T_F16) return ops_fail(GG_E_ARG, "%s: q.type %d is none of GG_T_*", fn, b->q.type);
+  if (b->q.heads < 1 || b->q.heads > 65535 || b->q.heads % c->kv_heads)
+    return ops_fail(GG_E_ARG, "%s: %d query heads over %d key heads", fn, b->q.heads, c->kv_heads);
   if (b->seqs < 0 || b->rows < 0 || b->max_rows < 0 || b->max_len < 0)
     return ops_fail(GG_E_ARG, "%s: seqs %d, rows %d, max_rows %d, max_len %d out of range", fn, b->seqs, b->rows, b->max_rows, b->max_len);
-  if (b->table_stride < ((long long)b->max_len + c->block_tokens - 1) / c->block_tokens)
-    return ops_fail(GG_E_ARG, "%s: table_stride %lld holds fewer than max_len %d tokens", fn, (long long)b->table_stride, b->max_len);
-  if (window < 0) return ops_fail(GG_E_ARG, "%s: window %d", fn, window);
-  const Kv8Plan p = kv8_plan(*c, *q, *b, window);
-  if ((long long)b->seqs * c->kv_heads * p.row_tiles * p.splits >= (1ll << 31))
-    return ops_fail(GG_E_ARG, "%s: the batch needs more than 2^31 tiles", fn);
+  if (b->window < 0) return ops_fail(GG_E_ARG, "%s: window %d", fn, b->window);
+  const Kv8Plan p = kv8_plan(*c, *b);
+  for (const Kv8Cut* k : {&p.few, &p.many})
+    if ((double)b->seqs * c->kv_heads * k->row_tiles * k->splits >= 2147483647.0)
+      return ops_fail(GG_E_ARG, "%s: the batch needs more than 2^31 tiles", fn);
   return GG_OK;
 }
 
 }  // namespace gg
 
-extern "C" int gg_kv8_attention_workspace(const gg_kv8_cache* c, const gg_rows* q, const gg_kv8_batch* b, int window, size_t* bytes) {
+extern "C" int gg_kv8_attention_workspace(const gg_kv8_cache* c, const gg_kv8_attention_call* call, size_t* bytes) {
   using namespace gg;
   const char* fn = "gg_kv8_attention_workspace";
-  if (!c || !q || !b || !bytes) return ops_fail(GG_E_ARG, "%s: null argument", fn);
-  if (int rc = kv8_check(fn, c, q, b, window)) return rc;
-  *bytes = b->seqs ? kv8_bytes(kv8_plan(*c, *q, *b, window), *c, *q, *b) : 0;
+  if (!c || !call || !bytes) return ops_fail(GG_E_ARG, "%s: null argument", fn);
+  if (int rc = kv8_check(fn, c, call)) return rc;
+  *bytes = call->seqs ? kv8_plan(*c, *call).bytes : 0;
   return GG_OK;
 }
 
-extern "C" int gg_kv8_attention(const gg_kv8_cache* c, const gg_rows* q, const gg_rows* out, float* lse, const gg_kv8_batch* b,
-                                double scale, int window, void* workspace, size_t workspace_bytes, void* stream) {
+extern "C" int gg_kv8_attention(const gg_kv8_cache* c, const gg_kv8_attention_call* call, void* stream) {
   using namespace gg;
   const char* fn = "gg_kv8_attention";
-  if (!c || !q || !out || !b) return ops_fail(GG_E_ARG, "%s: null argument", fn);
-  if (int rc = kv8_check(fn, c, q, b, window)) return rc;
-  if (int rc = ops_check_rows(fn, "out", out, b->rows, c->head_dim)) return rc;
-  if (out->type != q->type || out->heads != q->heads) return ops_fail(GG_E_ARG, "%s: out has another type or number of heads than q", fn);
-  if (!(scale == scale) || scale > 1e30 || scale < -1e30) return ops_fail(GG_E_ARG, "%s: scale is not a number", fn);
+  if (!c || !call) return ops_fail(GG_E_ARG, "%s: null argument", fn);
+  const gg_kv8_attention_call& b = *call;
+  if (int rc = kv8_check(fn, c, call)) return rc;
+  if (int rc = ops_check_rows(fn, "q", &b.q, b.rows, c->head_dim)) return rc;
+  if (int rc = ops_check_rows(fn, "out", &b.out, b.rows, c->head_dim)) return rc;
+  if (b.out.type != b.q.type || b.out.heads != b.q.heads) return ops_fail(GG_E_ARG, "%s: out has another type or number of heads than q", fn);
+  if (!b.cu_rows || !b.lens || !b.table) return ops_fail(GG_E_ARG, "%s: null array in the batch", fn);
+  if (b.table_stride < ((long long)b.max_len + c->block_tokens - 1) / c->block_tokens)
+    return ops_fail(GG_E_ARG, "%s: table_stride %lld holds fewer than max_len %d tokens", fn, (long long)b.table_stride, b.max_len);
+  if (!(b.scale >= -1e30 && b.scale <= 1e30)) return ops_fail(GG_E_ARG, "%s: scale is not a number", fn);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int rc = ops_check_stream(fn, s)) return rc;
-  if (b->seqs == 0 || b->rows == 0 || b->max_rows == 0) return GG_OK;
-  const Kv8Plan p = kv8_plan(*c, *q, *b, window);
-  const size_t need = kv8_bytes(p, *c, *q, *b);
-  if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace & 15))
-    return ops_fail(GG_E_ARG, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", fn, need, workspace ? workspace_bytes : (size_t)0);
+  if (b.seqs == 0 || b.rows == 0 || b.max_rows == 0) return GG_OK;
+  const Kv8Plan p = kv8_plan(*c, b);
+  if (p.bytes && (!b.workspace || b.workspace_bytes < p.bytes || (uintptr_t)b.workspace & 15))
+    return ops_fail(GG_E_ARG, "%s: needs %zu bytes of 16-byte aligned workspace, got %zu", fn, p.bytes, b.workspace ? b.workspace_bytes : (size_t)0);
   Kv8Args a = {};
   a.kc = static_cast<const uint8_t*>(c->k_codes);
   a.vc = static_cast<const uint8_t*>(c->v_codes);
   a.ks = c->k_scale;
   a.vs = c->v_scale;
-  a.q = q->data;
-  a.out = out->data;
-  a.lse = lse;
-  a.cu = b->cu_rows;
-  a.lens = b->lens;
-  a.table = b->table;
-  a.table_stride = b->table_stride;
-  a.q_row = q->row_stride;
-  a.q_head = q->head_stride;
-  a.o_row = out->row_stride;
-  a.o_head = out->head_stride;
-  a.scale_log2 = (float)(scale * 1.4426950408889634074);
-  a.seqs = b->seqs;
-  a.rows = b->rows;
-  a.max_rows = b->max_rows;
-  a.max_len = b->max_len;
+  a.q = b.q.data;
+  a.out = b.out.data;
+  a.lse = b.lse;
+  a.cu = b.cu_rows;
+  a.lens = b.lens;
+  a.table = b.table;
+  a.table_stride = b.table_stride;
+  a.q_row = b.q.row_stride;
+  a.q_head = b.q.head_stride;
+  a.o_row = b.out.row_stride;
+  a.o_head = b.out.head_stride;
+  a.scale_log2 = (float)(b.scale * 1.4426950408889634074);
+  a.seqs = b.seqs;
+  a.rows = b.rows;
+  a.max_rows = b.max_rows;
+  a.max_len = b.max_len;
   a.num_blocks = c->num_blocks;
   a.block_shift = __builtin_ctz(c->block_tokens);
   a.kv_heads = c->kv_heads;
-  a.group = q->heads / c->kv_heads;
+  a.group = b.q.heads / c->kv_heads;
   a.hd = c->head_dim;
-  a.window = window;
-  a.q_type = q->type;
-  a.q_vec = ops_aligned16(*q);
-  a.row_tiles = p.row_tiles;
-  a.splits = p.splits;
-  a.split_steps = p.split_steps;
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + (size_t)b->rows * q->heads * p.splits * c->head_dim);
-  cudaError_t r = c->head_dim <= 64 ? launch_rows_hd<64>(a, c->code, s) : c->head_dim <= 128 ? launch_rows_hd<128>(a, c->code, s) : launch_rows_hd<256>(a, c->code, s);
-  if (r == cudaSuccess && p.splits > 1) {
-    const long long warps = (long long)b->seqs * b->max_rows * q->heads;
-    r = launch_pdl(gg_kv8_merge_kernel, dim3((unsigned)((warps + 3) / 4)), dim3(128), 0, s, a);
+  a.window = b.window;
+  a.q_type = b.q.type;
+  a.q_vec = ops_aligned16(b.q);
+  a.o_vec = ops_aligned16(b.out);
+  cudaError_t r = cudaSuccess;
+  for (int many = 0; many < 2 && r == cudaSuccess; many++) {
+    const Kv8Cut& k = many ? p.many : p.few;
+    if (!k.row_tiles) continue;
+    a.row_tiles = k.row_tiles;
+    a.splits = k.splits;
+    a.split_steps = k.split_steps;
+    a.items_lo = many ? KV8_FEW : 0;
+    a.items_hi = many ? 0x7fffffff : KV8_FEW;
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(b.workspace) + (many ? p.few_bytes : 0));
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + k.parts * c->head_dim);
+    r = many ? kv8_launch_prompt(a, c->code, s)
+        : c->head_dim <= 64 ? launch_rows_hd<64>(a, c->code, s)
+        : c->head_dim <= 128 ? launch_rows_hd<128>(a, c->code, s)
+                             : launch_rows_hd<256>(a, c->code, s);
+    if (r == cudaSuccess && k.splits > 1) {
+      const long long tokens = many ? b.max_rows : (k.row_tiles * (long long)(b.q.type == GG_T_F32 ? 8 : 16) + a.group - 1) / a.group;
+      a.merge_tokens = (int)(tokens < b.max_rows ? tokens : b.max_rows);
+      r = launch_pdl(gg_kv8_merge_kernel, dim3((unsigned)(((long long)b.seqs * a.merge_tokens * b.q.heads + 3) / 4)), dim3(128), 0, s, a);
+    }
   }
   if (r != cudaSuccess) return ops_fail(GG_E_CUDA, "%s: launch: %s", fn, cudaGetErrorString(r));
   return GG_OK;

@@ -1,0 +1,147 @@
+// gg_kv8.h -- what the kernels that read the paged 8-bit KV cache share: the arguments of a call, the
+// widening of codes and the exponent arithmetic of the softmax.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "gg_launch.h"
+#include "gg_ops.h"
+
+namespace gg {
+
+constexpr float KV8_SLACK = 8.f;    // w_j <= 2^8
+constexpr float KV8_WMUL = 128.f;    // weights enter the MMA as w_j 2^7 <= 2^15
+constexpr float KV8_NEG = -1e30f;   // stands for -inf in running maxima (no inf - inf)
+
+struct Kv8Args {
+  const uint8_t *kc, *vc;
+  const float *ks, *vs;
+  const void* q;
+  void* out;
+  float* lse;
+  const int32_t *cu, *lens, *table;
+  float* part_o;    // [row][head][split][hd]
+  float2* part_ml;  // [row][head][split]: r, l
+  long long q_row, q_head, o_row, o_head, table_stride;
+  float scale_log2;
+  int seqs, rows, max_rows, max_len, num_blocks, block_shift, kv_heads, group, hd, window, q_type;
+  int row_tiles, splits, split_steps;  // split_steps: 16-key steps of a key range
+  int merge_tokens;                    // tokens of a request that the merge looks at
+  int items_lo, items_hi;  // this launch takes requests with items_lo < rows * group <= items_hi
+  int q_vec, o_vec;  // every head of q / out starts on a 16-byte boundary
+};
+
+GG_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+GG_DEV void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+GG_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {  // bytes 0: fills zeros, reads nothing
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+GG_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+GG_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+GG_DEV uint32_t half2_bits(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// f32 pair -> f16 hi pair and the f16 pair of what hi leaves.
+GG_DEV void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = half2_bits(a - f.x, b - f.y);
+}
+
+GG_DEV uint32_t hsub2_bits(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+GG_DEV uint32_t e4m3x2_f16x2(uint32_t two) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"((unsigned short)two));
+  return d;
+}
+// Four codes next to each other -> (0, 1) and (2, 3) as f16 pairs. int8: byte + 128 in the mantissa
+// of 1024 (f16 0x6400, steps of 1), minus 1152.
+template <int CODE>
+GG_DEV void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (CODE == GG_KV8_INT8) {
+    w ^= 0x80808080u;
+    lo = hsub2_bits(__byte_perm(w, 0x64646464u, 0x4140), 0x64806480u);
+    hi = hsub2_bits(__byte_perm(w, 0x64646464u, 0x4342), 0x64806480u);
+  } else {
+    lo = e4m3x2_f16x2(w);
+    hi = e4m3x2_f16x2(w >> 16);
+  }
+}
+// Words a and b of two keys (four dims each) -> for each dim the f16 pair (a, b).
+template <int CODE>
+GG_DEV void widen4_pairs(uint32_t a, uint32_t b, uint32_t (&d)[4]) {
+  if constexpr (CODE == GG_KV8_INT8) {
+    const uint32_t x = __byte_perm(a, b, 0x5140) ^ 0x80808080u, y = __byte_perm(a, b, 0x7362) ^ 0x80808080u;
+    d[0] = hsub2_bits(__byte_perm(x, 0x64646464u, 0x4140), 0x64806480u);
+    d[1] = hsub2_bits(__byte_perm(x, 0x64646464u, 0x4342), 0x64806480u);
+    d[2] = hsub2_bits(__byte_perm(y, 0x64646464u, 0x4140), 0x64806480u);
+    d[3] = hsub2_bits(__byte_perm(y, 0x64646464u, 0x4342), 0x64806480u);
+  } else {
+    const uint32_t a0 = e4m3x2_f16x2(a), a1 = e4m3x2_f16x2(a >> 16), b0 = e4m3x2_f16x2(b), b1 = e4m3x2_f16x2(b >> 16);
+    d[0] = __byte_perm(a0, b0, 0x5410);
+    d[1] = __byte_perm(a0, b0, 0x7632);
+    d[2] = __byte_perm(a1, b1, 0x5410);
+    d[3] = __byte_perm(a1, b1, 0x7632);
+  }
+}
+
+GG_DEV float load_elem(const void* p, int type, long long i) {
+  if (type == GG_T_F32) return static_cast<const float*>(p)[i];
+  if (type == GG_T_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(static_cast<const __half*>(p)[i]);
+}
+GG_DEV void store_elem(void* p, int type, long long i, float v) {
+  if (type == GG_T_F32) static_cast<float*>(p)[i] = v;
+  else if (type == GG_T_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+// Four elements from i on (a multiple of four).
+GG_DEV float4 load_elem4(const void* p, int type, long long i, int vec) {
+  if (!vec) return make_float4(load_elem(p, type, i), load_elem(p, type, i + 1), load_elem(p, type, i + 2), load_elem(p, type, i + 3));
+  if (type == GG_T_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+  const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+  if (type == GG_T_BF16)
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
+// The rows of request s: first row, number of rows (within the batch and max_rows), length.
+struct Kv8Seq {
+  int row0, n, len;
+  long long first_pos;  // position of row row0
+};
+GG_DEV Kv8Seq kv8_seq(const Kv8Args& a, int s) {
+  Kv8Seq q;
+  const int c0 = a.cu[s], c1 = a.cu[s + 1], len = max(a.lens[s], 0);
+  q.row0 = max(c0, 0);
+  q.n = max(min(c1, a.rows) - q.row0, 0);
+  q.first_pos = (long long)len - (c1 - c0);
+  q.n = min(q.n, a.max_rows);
+  const long long items = (long long)q.n * a.group;
+  if (items <= a.items_lo || items > a.items_hi) q.n = 0;  // another launch's request
+  q.len = min(len, a.max_len);
+  return q;
+}
+
+
+// Many rows (gg_kv8_prompt.cu): query rows of a tile, and the launch.
+int kv8_prompt_tile(int head_dim);
+cudaError_t kv8_launch_prompt(const Kv8Args& a, int code, cudaStream_t s);
+
+}  // namespace gg

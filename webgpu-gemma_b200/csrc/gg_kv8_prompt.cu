@@ -1,0 +1,588 @@
+// gg_kv8_prompt.cu -- attention over the paged 8-bit KV cache for many query rows (prompts and
+// prompt chunks). The mathematics and the exponent arithmetic are those of gg_kv8.cu.
+//
+// Bound by the tensor cores: 4 hd operations for each (row, key) pair. One CTA takes NQ tiles of
+// 128 query rows (the heads that share a key head, token by token) and one range of keys, KT at a
+// time; both products run as tcgen05 kind::f16 with f32 accumulators in TMEM:
+//   converter warps  codes from global memory through registers (one tile ahead), widened to f16
+//                    (exact) and stored as SW128 tiles: K (K-major B operand of Q K^T) and V, the
+//                    same bytes read MN-major as the B operand of P V, so V is never transposed
+//   MMA warp         S = Q K^T into TMEM, then O += P V with P read from TMEM
+//   softmax warps    four per query tile, a thread per row: S from TMEM, weights in registers (no
+//                    shuffles), f16 weights back over S's columns as the A operand of P V
+// With two query tiles (hd <= 128) the tensor cores work on one while the other's softmax runs;
+// with one (hd = 256: O alone takes 256 columns) S is double-buffered instead. f32 queries make
+// both products twice, for the hi and the lo half of q and of the weights, into the same
+// accumulators. The running maximum r is kept an integer and raised only when a weight would pass
+// 2^KV8_SLACK, so the accumulator in TMEM is rarely rescaled (first tile, then now and then).
+#include "gg_kv8.h"
+#include "gg_tc.cuh"
+
+namespace gg {
+
+template <int HD, bool HILO>
+struct PromptShape {
+  static constexpr int NQ = HD == 256 ? 1 : 2;                       // query tiles of 128 rows
+  static constexpr int KT = HD == 64 || (HD == 128 && !HILO) ? 128 : 64;  // keys of a tile
+  static constexpr int ST = HD == 256 && HILO ? 1 : 2;               // ring stages of K and of V
+  static constexpr int Q_BYTES = 128 * HD * 2 * (HILO ? 2 : 1);      // per query tile
+  static constexpr int KV_BYTES = KT * HD * 2;
+  static constexpr int GROUPS = 256;                                 // 16-key groups in the scale ring
+  static constexpr int OFF_K = NQ * Q_BYTES;
+  static constexpr int OFF_V = OFF_K + ST * KV_BYTES;
+  static constexpr int OFF_META = OFF_V + ST * KV_BYTES;
+  static constexpr int OFF_MUL = OFF_META + GROUPS * 16;
+  static constexpr int OFF_BAR = OFF_MUL + NQ * 128 * 4;
+  static constexpr int SMEM = OFF_BAR + 256 + 1024;  // + alignment of the operand tiles
+  static constexpr int SOFT_WARPS = 4 * NQ, CONV_WARPS = 4;
+  static constexpr int THREADS = (SOFT_WARPS + CONV_WARPS + 1) * 32;
+  static constexpr int TMEM_S = KT;               // columns of one S buffer (two of them)
+  static constexpr int TMEM_O = 2 * KT;           // first column of O
+  static_assert(2 * KT + NQ * HD <= 512, "TMEM columns");
+};
+
+// MN-major operand, 128-byte swizzle: rows of 64 values of the N index, 8 rows (K index) to an
+// atom of 1024 B; the next 8 rows follow 1024 B on, the next 64 values of N `slab` bytes on.
+GG_DEV uint64_t umma_desc_sw128_mn(uint32_t saddr, uint32_t slab) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+  d |= (uint64_t)((slab >> 4) & 0x3FFFu) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// kind::f16 with f16 operands and f32 sums, M = 128, N = n; B MN-major if b_mn.
+GG_DEV uint32_t umma_idesc_f16_m128(int n, bool b_mn) {
+  return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+// D(tmem) (+)= A(tmem) x B(smem desc)
+GG_DEV void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+GG_DEV void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+GG_DEV void tmem_ld_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+GG_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+GG_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+GG_DEV void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Wait for an mbarrier phase; after two seconds (or when another warp gave up) sets *abort and
+// returns false: the CTA then drains its MMAs and leaves NaN in its rows.
+GG_DEV bool prompt_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+#pragma unroll 1
+  for (int it = 0; it < 64; ++it)
+    if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+#pragma unroll 1
+  for (;;) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*abort) return false;
+    if (global_timer_ns() - t0 > 2000000000ull) {
+      *abort = 1;
+      return false;
+    }
+  }
+}
+
+// The same for a whole warp: all lanes agree on the outcome.
+GG_DEV bool prompt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, prompt_wait(bar, parity, abort));
+}
+
+template <int HD, int CODE, bool HILO>
+__global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prompt_kernel(const Kv8Args a) {
+  typedef PromptShape<HD, HILO> S;
+  constexpr int NQ = S::NQ, KT = S::KT, ST = S::ST, GT = KT / 16, HALVES = KT / 64;
+  extern __shared__ unsigned char prompt_smem[];
+  unsigned char* sm = prompt_smem + ((1024 - (smem_u32(prompt_smem) & 1023)) & 1023);
+  float4* meta = reinterpret_cast<float4*>(sm + S::OFF_META);  // per 16-key group: ks, log2 vs, 1 / vs
+  float* s_mul = reinterpret_cast<float*>(sm + S::OFF_MUL);
+  uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + S::OFF_BAR);
+  uint64_t *kempty = kfull + 2, *vfull = kfull + 4, *vempty = kfull + 6, *sfull = kfull + 8, *pfull = kfull + 10,
+           *odone = kfull + 12, *drain = kfull + 14;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 15);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int MMA_WARP = S::SOFT_WARPS + S::CONV_WARPS;
+
+  pdl_wait();
+  int x = blockIdx.x;
+  const int split = x % a.splits;
+  x /= a.splits;
+  const int rt = a.row_tiles - 1 - x % a.row_tiles;  // the tiles with the most keys first
+  x /= a.row_tiles;
+  const int h = x % a.kv_heads, s = x / a.kv_heads;
+  const Kv8Seq sq = kv8_seq(a, s);
+  const int items = sq.n * a.group, base = rt * (NQ * 128);
+  const int nitems = max(min(NQ * 128, items - base), 0);
+  const int heads = a.kv_heads * a.group;
+  if (!nitems) {
+    pdl_trigger();
+    return;
+  }
+  // TMEM is taken after the wait for earlier kernels and before later ones may become resident: none
+  // that waits for this one can hold the columns this one needs
+  if (warp == MMA_WARP) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+    if (lane == 0) {
+      for (int i = 0; i < 2; i++) {
+        mbar_init(&kfull[i], S::CONV_WARPS);
+        mbar_init(&kempty[i], 1);
+        mbar_init(&vfull[i], S::CONV_WARPS);
+        mbar_init(&vempty[i], 1);
+        mbar_init(&sfull[i], 1);
+        mbar_init(&pfull[i], 4);
+        mbar_init(&odone[i], 1);
+      }
+      mbar_init(drain, 1);
+      *abort = 0;
+      mbar_fence_init();
+    }
+  }
+  const long long pos_lo = sq.first_pos + base / a.group, pos_hi = sq.first_pos + (base + nitems - 1) / a.group;
+  const int kmax = (int)min((long long)sq.len, pos_hi + 1);
+  const int kmin = a.window ? (int)max(0ll, pos_lo - a.window + 1) & ~15 : 0;
+  const int k00 = (int)min(kmin + 16ll * split * a.split_steps, (long long)kmax);  // first key of this range
+  const int kend = (int)min((long long)kmax, k00 + (long long)a.split_steps * 16);
+  const int nt = kend > k00 ? (kend - k00 + KT - 1) / KT : 0;
+
+  // ---- query rows -> f16 tiles, each row times its own power of two
+  if (nt) {
+    for (int row = warp; row < NQ * 128; row += S::THREADS / 32) {
+      const bool live = row < nitems;
+      const int it = base + row;
+      const long long qi = live ? (long long)(sq.row0 + it / a.group) * a.q_row + (long long)(h * a.group + it % a.group) * a.q_head : 0;
+      constexpr int PER = (HD / 4 + 31) / 32;
+      float4 v[PER];
+      uint32_t top = 0;
+#pragma unroll
+      for (int p = 0; p < PER; p++) {
+        const int d = 4 * (lane + 32 * p);
+        v[p] = live && d < a.hd ? load_elem4(a.q, a.q_type, qi + d, a.q_vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+        top = max(max(top, __float_as_uint(v[p].x) & 0x7fffffffu), __float_as_uint(v[p].y) & 0x7fffffffu);
+        top = max(max(top, __float_as_uint(v[p].z) & 0x7fffffffu), __float_as_uint(v[p].w) & 0x7fffffffu);
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      const int ex = min(max((int)(top >> 23) - 127, -100), 127);
+      const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
+      if (lane == 0) s_mul[row] = __uint_as_float((uint32_t)(ex - 14 + 127) << 23) * a.scale_log2;
+      unsigned char* qt = sm + (row >> 7) * S::Q_BYTES;
+      const int r = row & 127;
+#pragma unroll
+      for (int p = 0; p < PER; p++) {
+        const int d = 4 * (lane + 32 * p);
+        if (d >= HD) break;
+        uint2* dst = reinterpret_cast<uint2*>(qt + (d >> 6) * (128 * 128) + sw128_offset(r, d & 63));
+        if constexpr (HILO) {
+          uint2 hi, lo;
+          split_f16(v[p].x * up, v[p].y * up, hi.x, lo.x);
+          split_f16(v[p].z * up, v[p].w * up, hi.y, lo.y);
+          *dst = hi;
+          *reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(dst) + S::Q_BYTES / 2) = lo;
+        } else {
+          *dst = make_uint2(half2_bits(v[p].x * up, v[p].y * up), half2_bits(v[p].z * up, v[p].w * up));
+        }
+      }
+    }
+    fence_proxy_async_smem();
+  }
+
+  // ---- block ids and scales of 16-key groups, 64 groups (two to a lane) at a time
+  const int32_t* table = a.table + (long long)s * a.table_stride;
+  const auto load_id = [&](int group) {  // group of this range; -1 for a block the cache has not
+    const long long key = k00 + 16ll * group;
+    if (key >= kend) return -1;
+    const int id = table[key >> a.block_shift];
+    return id >= 0 && id < a.num_blocks ? id : -1;
+  };
+  const auto load_scales = [&](int id) {
+    return id < 0 ? make_float2(0.f, 1.f) : make_float2(a.ks[(long long)id * a.kv_heads + h], a.vs[(long long)id * a.kv_heads + h]);
+  };
+  const auto put_group = [&](int group, int id, float2 sc) {
+    // no block: scores of 0 under an exponent of -huge, rows of zeros in V, nothing added to l. A NaN
+    // scale reaches l through the weights of the rows that see it, not through 1 / vs.
+    meta[group & (S::GROUPS - 1)] = id < 0 ? make_float4(0.f, KV8_NEG, 0.f, 0.f) : make_float4(sc.x, log2f(sc.y), sc.y == sc.y ? 1.f / sc.y : 1.f, 0.f);
+  };
+  if (nt && tid < 64) {
+    const int id = load_id(tid);
+    put_group(tid, id, load_scales(id));
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();
+  const uint32_t tmem = *tmem_slot;
+
+  if (nt && warp >= S::SOFT_WARPS && warp < MMA_WARP) {
+    // ------------------------------------------------------------------ converter warps
+    const int ct = tid - S::SOFT_WARPS * 32;
+    constexpr int WORDS = KT * HD / 16 / 128;  // 16-byte words of a thread and tile
+    const int W = a.hd >> 4, total = KT * W;
+    const uint32_t wmagic = (65536u + W - 1) / W;  // x / W for x < 2048
+    constexpr int TB = 64 / GT;  // tiles of a batch of 64 groups
+    int cur[2] = {load_id(lane), load_id(lane + 32)}, nxt[2] = {-1, -1};  // this batch's ids and the next one's
+    const auto fetch = [&](const uint8_t* codes, int tile, int batch, uint4 (&r)[WORDS]) {
+#pragma unroll
+      for (int i = 0; i < WORDS; i++) {
+        const int xw = ct + 128 * i;
+        const int k = (int)(((uint32_t)xw * wmagic) >> 16), w = xw - k * W;
+        const int group = (tile * GT + (k >> 4)) & 63;
+        const bool now = tile / TB == batch;
+        const int id0 = __shfl_sync(0xffffffffu, now ? cur[0] : nxt[0], group & 31);
+        const int id1 = __shfl_sync(0xffffffffu, now ? cur[1] : nxt[1], group & 31);
+        const int id = group & 32 ? id1 : id0, key = k00 + tile * KT + k;
+        r[i] = make_uint4(0, 0, 0, 0);
+        if (tile < nt && xw < total && id >= 0 && key < sq.len) {
+          const long long at = (((long long)id * a.kv_heads + h) << a.block_shift) + (key & ((1 << a.block_shift) - 1));
+          r[i] = __ldg(reinterpret_cast<const uint4*>(codes + at * a.hd) + w);
+        }
+      }
+    };
+    const auto put = [&](unsigned char* tile, const uint4 (&r)[WORDS]) {
+#pragma unroll
+      for (int i = 0; i < WORDS; i++) {
+        const int xw = ct + 128 * i;
+        if (xw < total) {
+          const int k = (int)(((uint32_t)xw * wmagic) >> 16), w = xw - k * W;
+          uint4 lo, hi;
+          widen4<CODE>(r[i].x, lo.x, lo.y);
+          widen4<CODE>(r[i].y, lo.z, lo.w);
+          widen4<CODE>(r[i].z, hi.x, hi.y);
+          widen4<CODE>(r[i].w, hi.z, hi.w);
+          unsigned char* row = tile + (w >> 2) * (KT * 128) + (k >> 3) * 1024 + (k & 7) * 128;
+          const int c = (w & 3) * 2;
+          // lanes of neighbouring slabs store their two chunks in opposite order (bank conflicts)
+          const bool odd = (w >> 2) & 1;
+          *reinterpret_cast<uint4*>(row + (((c + odd) ^ (k & 7)) << 4)) = odd ? hi : lo;
+          *reinterpret_cast<uint4*>(row + (((c + !odd) ^ (k & 7)) << 4)) = odd ? lo : hi;
+        }
+      }
+      fence_proxy_async_smem();
+    };
+    uint4 rk[WORDS], rv[WORDS];
+    float2 sc[2] = {};
+    fetch(a.kc, 0, 0, rk);
+    fetch(a.vc, 0, 0, rv);
+    for (int i = 0; i < nt; i++) {
+      const int st = i % ST, par = (i / ST) & 1, b = i / TB, q = i % TB;
+      // the next batch of groups: ids, then (one warp) scales, then shared memory, a quarter batch apart
+      if (q == 0) {
+        for (int j = 0; j < 2; j++) {
+          if (b) cur[j] = nxt[j];
+          nxt[j] = load_id((b + 1) * 64 + lane + 32 * j);
+        }
+      }
+      if (ct < 32 && q == TB / 4)
+        for (int j = 0; j < 2; j++) sc[j] = load_scales(nxt[j]);
+      if (ct < 32 && q == TB / 2)
+        for (int j = 0; j < 2; j++) put_group((b + 1) * 64 + lane + 32 * j, nxt[j], sc[j]);
+      if (i >= ST && !prompt_wait_warp(&kempty[st], par ^ 1, abort)) break;
+      put(sm + S::OFF_K + st * S::KV_BYTES, rk);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&kfull[st]);
+      fetch(a.kc, i + 1, b, rk);
+      if (i >= ST && !prompt_wait_warp(&vempty[st], par ^ 1, abort)) break;
+      put(sm + S::OFF_V + st * S::KV_BYTES, rv);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&vfull[st]);
+      fetch(a.vc, i + 1, b, rv);
+    }
+  } else if (nt && warp == MMA_WARP) {
+    // ------------------------------------------------------------------ MMA issue (one thread)
+    if (lane == 0) {
+      const int steps = a.hd >> 4;
+      const uint32_t idesc_s = umma_idesc_f16_m128(KT, false), idesc_o = umma_idesc_f16_m128(a.hd, true);
+      const uint32_t sq_base = smem_u32(sm), sk_base = smem_u32(sm + S::OFF_K), sv_base = smem_u32(sm + S::OFF_V);
+      const auto scores = [&](int q, int i, int buf) {  // S buffer = Q tile q x K tile i
+        const uint32_t d = tmem + buf * S::TMEM_S, qb = sq_base + q * S::Q_BYTES, kb = sk_base + (i % ST) * S::KV_BYTES;
+        for (int part = 0; part < (HILO ? 2 : 1); part++)
+          for (int k = 0; k < steps; k++)
+            umma_bf16(d, umma_desc_sw128(qb + part * (S::Q_BYTES / 2) + (k >> 2) * (128 * 128) + (k & 3) * 32),
+                      umma_desc_sw128(kb + (k >> 2) * (KT * 128) + (k & 3) * 32), idesc_s, part > 0 || k > 0);
+        umma_commit(&sfull[buf]);
+      };
+      const auto outputs = [&](int q, int i, int buf) {  // O tile q += P x V tile i
+        const uint32_t d = tmem + S::TMEM_O + q * HD, p = tmem + buf * S::TMEM_S, vb = sv_base + (i % ST) * S::KV_BYTES;
+        for (int k = 0; k < KT / 16; k++)
+          for (int part = 0; part < (HILO ? 2 : 1); part++)
+            umma_f16_ts(d, p + (k >> 2) * 64 + part * 32 + (k & 3) * 8, umma_desc_sw128_mn(vb + k * 2048, KT * 128), idesc_o,
+                        i > 0 || k > 0 || part > 0);
+        umma_commit(&odone[q]);
+      };
+      bool ok = prompt_wait(&kfull[0], 0, abort);
+      tc_fence_after();
+      if (ok) {
+        for (int q = 0; q < NQ; q++) scores(q, 0, q);
+        umma_commit(&kempty[0]);
+      }
+      for (int i = 0; ok && i < nt; i++) {
+        const int st = i % ST, st1 = (i + 1) % ST;
+        const bool more = i + 1 < nt;
+        if constexpr (NQ == 1) {  // the next tile's scores into the other buffer, before this one's weights are ready
+          if (more) {
+            if (!(ok = prompt_wait(&kfull[st1], ((i + 1) / ST) & 1, abort))) break;
+            tc_fence_after();
+            scores(0, i + 1, (i + 1) & 1);
+            umma_commit(&kempty[st1]);
+          }
+        }
+        for (int q = 0; q < NQ; q++) {
+          const int buf = NQ == 1 ? i & 1 : q;
+          if (!(ok = prompt_wait(&pfull[buf], NQ == 1 ? (i >> 1) & 1 : i & 1, abort))) break;
+          if (q == 0 && !(ok = prompt_wait(&vfull[st], (i / ST) & 1, abort))) break;
+          tc_fence_after();
+          outputs(q, i, buf);
+          if (q == NQ - 1) umma_commit(&vempty[st]);
+          if (NQ == 2 && more) {
+            if (q == 0) {
+              if (!(ok = prompt_wait(&kfull[st1], ((i + 1) / ST) & 1, abort))) break;
+              tc_fence_after();
+            }
+            scores(q, i + 1, q);
+            if (q == NQ - 1) umma_commit(&kempty[st1]);
+          }
+        }
+      }
+      if (!ok) {  // everything issued so far has finished before TMEM is freed
+        umma_commit(drain);
+        for (int it = 0; it < 1000000 && !mbar_try_wait(drain, 0); ++it) {
+        }
+      }
+    }
+  } else if (warp < S::SOFT_WARPS) {
+    // ------------------------------------------------------------------ softmax warps
+    const int q = warp >> 2;
+    const int row = q * 128 + (warp & 3) * 32 + lane;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16), to = tl + S::TMEM_O + q * HD;
+    const bool live = row < nitems;
+    const int it = base + (live ? row : 0), tok = it / a.group, hq = h * a.group + it % a.group;
+    const long long pos = sq.first_pos + tok;
+    const int hi_key = live ? (int)min(pos, (long long)kend - 1) : -1;
+    const int lo_key = a.window ? (int)max(0ll, pos - a.window + 1) : 0;
+    // keys that every row of the CTA sees (dead rows see what they like: nothing of theirs is stored)
+    const int all_hi = (int)min(pos_lo, (long long)kend - 1), all_lo = a.window ? (int)max(0ll, pos_hi - a.window + 1) : 0;
+    const float mul = nt ? s_mul[row] : 0.f;
+    float r = KV8_NEG, l = 0.f;
+    bool ok = true;
+    for (int i = 0; i < nt; i++) {
+      const int buf = NQ == 1 ? i & 1 : q;
+      if (!(ok = prompt_wait_warp(&sfull[buf], NQ == 1 ? (i >> 1) & 1 : i & 1, abort))) break;
+      tc_fence_after();
+      const uint32_t ts = tl + buf * S::TMEM_S;
+#pragma unroll 1
+      for (int half = 0; half < HALVES; half++) {
+        const int key0 = k00 + i * KT + half * 64;
+        const bool whole = key0 + 63 <= all_hi && key0 >= all_lo;
+        const float4* mt = meta + ((i * GT + half * 4) & (S::GROUPS - 1));
+        uint32_t v[2][32];
+        float top;
+        // x = t - r + 7 in place of the scores: weights are 2^x = 2^7 w
+        const auto exponents = [&](float from) {
+          tmem_ld32(ts + half * 64, v[0]);
+          tmem_ld32(ts + half * 64 + 32, v[1]);
+          tmem_ld_done();
+          top = KV8_NEG;
+#pragma unroll
+          for (int g = 0; g < 4; g++) {
+            const float4 m = mt[g];
+            const float f = m.x * mul, c = m.y - from;
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+              uint32_t& w = v[g >> 1][(g & 1) * 16 + e];
+              w = __float_as_uint(fmaf(__uint_as_float(w), f, c));
+            }
+          }
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 64; e++) {
+              const int key = key0 + e;
+              if (key > hi_key || key < lo_key) v[e >> 5][e & 31] = __float_as_uint(KV8_NEG);
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 64; e++) top = fmaxf(top, __uint_as_float(v[e >> 5][e & 31]));
+        };
+        exponents(r - 7.f);
+        if (__any_sync(0xffffffffu, top > 7.f + KV8_SLACK)) {
+          const bool raise = top > 7.f + KV8_SLACK;
+          exponents(0.f);
+          const float nr = raise ? ceilf(top) : r;
+          const float f = ex2(r - nr);  // 0 for the first keys of a row, else a power of two
+          l *= f;
+          if (i > 0) {  // O is rescaled once the previous tile's product is in it
+            if (!(ok = prompt_wait_warp(&odone[q], (i - 1) & 1, abort))) break;
+            tc_fence_after();
+            for (int c = 0; c < a.hd; c += 32) {
+              tmem_ld32(to + c, v[0]);
+              tmem_ld_done();
+#pragma unroll
+              for (int e = 0; e < 32; e++) v[0][e] = __float_as_uint(__uint_as_float(v[0][e]) * f);
+              tmem_st32(to + c, v[0]);
+            }
+          }
+          if (half > 0) {  // and so are this tile's earlier weights
+            const __half2 f2 = __float2half2_rn(f);
+            tmem_ld32(ts, v[0]);
+            if constexpr (HILO) tmem_ld32(ts + 32, v[1]);
+            tmem_ld_done();
+#pragma unroll
+            for (int e = 0; e < 32; e++) {
+              __half2 y = __hmul2(*reinterpret_cast<__half2*>(&v[0][e]), f2);
+              v[0][e] = *reinterpret_cast<uint32_t*>(&y);
+              if constexpr (HILO) {
+                y = __hmul2(*reinterpret_cast<__half2*>(&v[1][e]), f2);
+                v[1][e] = *reinterpret_cast<uint32_t*>(&y);
+              }
+            }
+            tmem_st32(ts, v[0]);
+            if constexpr (HILO) tmem_st32(ts + 32, v[1]);
+          }
+          tmem_st_done();
+          r = nr;
+          exponents(r - 7.f);
+        }
+#pragma unroll
+        for (int g2 = 0; g2 < 2; g2++) {  // 32 keys: 16 columns of weights (HILO: and 16 of what they leave)
+          uint32_t ph[16], pl[16];
+#pragma unroll
+          for (int g = 0; g < 2; g++) {
+            const float iv = mt[2 * g2 + g].z;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const float w0 = ex2(__uint_as_float(v[g2][g * 16 + 2 * e])), w1 = ex2(__uint_as_float(v[g2][g * 16 + 2 * e + 1]));
+              sum += w0 + w1;
+              if constexpr (HILO) split_f16(w0, w1, ph[g * 8 + e], pl[g * 8 + e]);
+              else ph[g * 8 + e] = half2_bits(w0, w1);
+            }
+            l = fmaf(sum, iv, l);
+          }
+          tmem_st16(ts + half * 64 + g2 * 16, ph);
+          if constexpr (HILO) tmem_st16(ts + half * 64 + 32 + g2 * 16, pl);
+        }
+      }
+      if (!ok) break;
+      tmem_st_done();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pfull[buf]);
+    }
+    if (ok && nt) {
+      // with one query tile the last scores were issued before the last but one product: a parity
+      // wait alone could take the phase before that for the last one
+      if (nt > 1) ok = prompt_wait_warp(&odone[q], (nt - 2) & 1, abort);
+      ok = ok && prompt_wait_warp(&odone[q], (nt - 1) & 1, abort);
+      tc_fence_after();
+    }
+    const long long ri = (long long)sq.row0 + tok, pi = (ri * heads + hq) * a.splits + split;
+    l *= 1.f / KV8_WMUL;
+    const float nan = __uint_as_float(0x7fffffffu);
+    const float inv = !ok ? nan : a.splits > 1 ? 1.f / KV8_WMUL : l == 0.f ? 0.f : (1.f / KV8_WMUL) / l;
+    for (int c = 0; c < a.hd; c += 32) {
+      uint32_t v[32];
+      if (nt && ok) {
+        tmem_ld32(to + c, v);
+        tmem_ld_done();
+      } else {
+#pragma unroll
+        for (int e = 0; e < 32; e++) v[e] = 0;
+      }
+      if (live) {
+        const int n = min(32, a.hd - c);
+#pragma unroll
+        for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * inv);
+        if (a.splits > 1) {
+          float* dst = a.part_o + pi * a.hd + c;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            if (e < n) *reinterpret_cast<uint4*>(dst + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+        } else {
+          const long long oi = ri * a.o_row + (long long)hq * a.o_head + c;
+          if (!a.o_vec) {
+#pragma unroll
+            for (int e = 0; e < 32; e++)
+              if (e < n) store_elem(a.out, a.q_type, oi + e, __uint_as_float(v[e]));
+          } else if (a.q_type == GG_T_F32) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (e < n) *reinterpret_cast<uint4*>(static_cast<float*>(a.out) + oi + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          } else {
+            const bool bf = a.q_type == GG_T_BF16;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              if (e < n) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                  const float y0 = __uint_as_float(v[e + 2 * j]), y1 = __uint_as_float(v[e + 2 * j + 1]);
+                  w[j] = bf ? pack_bf16x2(__float2bfloat16_rn(y0), __float2bfloat16_rn(y1)) : half2_bits(y0, y1);
+                }
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + oi + e) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+          }
+        }
+      }
+    }
+    if (live) {
+      if (a.splits > 1) a.part_ml[pi] = make_float2(r, ok ? l : nan);
+      else if (a.lse) a.lse[ri * heads + hq] = !ok ? nan : l == 0.f ? -INFINITY : (r + log2f(l)) * 0.6931471805599453f;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int HD, int CODE, bool HILO>
+static cudaError_t launch_prompt(const Kv8Args& a, cudaStream_t s) {
+  typedef PromptShape<HD, HILO> S;
+  const long long grid = (long long)a.seqs * a.kv_heads * a.row_tiles * a.splits;
+  return launch_big_smem(gg_kv8_prompt_kernel<HD, CODE, HILO>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s, a);
+}
+template <int HD>
+static cudaError_t launch_prompt_hd(const Kv8Args& a, int code, cudaStream_t s) {
+  const bool hilo = a.q_type == GG_T_F32;
+  if (code == GG_KV8_INT8) return hilo ? launch_prompt<HD, GG_KV8_INT8, true>(a, s) : launch_prompt<HD, GG_KV8_INT8, false>(a, s);
+  return hilo ? launch_prompt<HD, GG_KV8_E4M3, true>(a, s) : launch_prompt<HD, GG_KV8_E4M3, false>(a, s);
+}
+
+int kv8_prompt_tile(int head_dim) { return head_dim <= 128 ? 256 : 128; }
+
+cudaError_t kv8_launch_prompt(const Kv8Args& a, int code, cudaStream_t s) {
+  return a.hd <= 64 ? launch_prompt_hd<64>(a, code, s) : a.hd <= 128 ? launch_prompt_hd<128>(a, code, s) : launch_prompt_hd<256>(a, code, s);
+}
+
+}  // namespace gg

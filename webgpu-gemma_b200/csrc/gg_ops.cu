@@ -619,8 +619,7 @@ extern "C" int gg_plan_blocks(const gg_block_plan* plan, void* stream) {
   if (int rc = ops_check_stream(fn, s)) return rc;
   const int inline_rows = p.rows <= PLAN_INLINE_ROWS;
   static_assert(sizeof(PlanScan) > 48 * 1024 && sizeof(PlanScan) < 64 * 1024, "opt-in shared memory");
-  cudaError_t r = cudaFuncSetAttribute(gg_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PlanScan));
-  if (r == cudaSuccess) r = launch_pdl(gg_plan_kernel, dim3(1), dim3(PLAN_THREADS), sizeof(PlanScan), s, p, inline_rows);
+  cudaError_t r = launch_big_smem(gg_plan_kernel, dim3(1), dim3(PLAN_THREADS), sizeof(PlanScan), s, p, inline_rows);
   if (r == cudaSuccess && !inline_rows) {
     const int grid = (int)(((long long)p.rows + 255) / 256);
     r = launch_pdl(gg_plan_rows_kernel, dim3(grid < 1184 ? grid : 1184), dim3(256), 0, s, p);
@@ -629,12 +628,12 @@ extern "C" int gg_plan_blocks(const gg_block_plan* plan, void* stream) {
   return GG_OK;
 }
 
-extern "C" int gg_rope(const gg_rows* q, const gg_rows* k, const gg_rows* q_out, const gg_rows* k_out, int rows,
-                       int head_dim, int rot_dim, int layout, const int32_t* positions, const double* freqs,
-                       double mscale, int inverse, void* stream) {
+extern "C" int gg_rope(const gg_rope_call* call, void* stream) {
   using namespace gg;
   const char* fn = "gg_rope";
-  if (!q || !q_out || !positions || !freqs || !k != !k_out) return ops_fail(GG_E_ARG, "%s: null argument", fn);
+  if (!call || !call->positions || !call->freqs || !call->k.data != !call->k_out.data) return ops_fail(GG_E_ARG, "%s: null argument", fn);
+  const gg_rows *q = &call->q, *q_out = &call->q_out, *k = call->k.data ? &call->k : nullptr, *k_out = &call->k_out;
+  const int rows = call->rows, head_dim = call->head_dim, rot_dim = call->rot_dim, layout = call->layout;
   if (rows < 0 || head_dim < 1 || head_dim > 4096) return ops_fail(GG_E_ARG, "%s: rows %d or head_dim %d out of range", fn, rows, head_dim);
   if (rot_dim < 2 || rot_dim > head_dim || rot_dim % 2 || rot_dim / 2 > ROPE_CS)
     return ops_fail(GG_E_ARG, "%s: rot_dim %d is not an even number from 2 to min(head_dim %d, %d)", fn, rot_dim, head_dim, 2 * ROPE_CS);
@@ -655,15 +654,15 @@ extern "C" int gg_rope(const gg_rows* q, const gg_rows* k, const gg_rows* q_out,
   RopeArgs a = {};
   a.q = {q->data, q_out->data, q->row_stride, q->head_stride, q_out->row_stride, q_out->head_stride};
   if (k) a.k = {k->data, k_out->data, k->row_stride, k->head_stride, k_out->row_stride, k_out->head_stride};
-  a.pos = positions;
-  a.freqs = freqs;
-  a.mscale = mscale;
+  a.pos = call->positions;
+  a.freqs = call->freqs;
+  a.mscale = call->mscale;
   a.rows = rows;
   a.q_heads = q->heads;
   a.heads = q->heads + (k ? k->heads : 0);
   a.hd = head_dim;
   a.rot = rot_dim;
-  a.inverse = inverse != 0;
+  a.inverse = call->inverse != 0;
   a.interleaved = layout == GG_ROPE_INTERLEAVED;
   // rows of a CTA: enough that the angles keep its threads busy once there are rows for every SM
   int per = 1;
@@ -707,11 +706,13 @@ extern "C" int gg_rope_freqs(int scaling, int rot_dim, double theta, double fact
   return GG_OK;
 }
 
-extern "C" int gg_kv8_append(const gg_kv8_cache* c, const gg_rows* k, const gg_rows* v, const int32_t* slots, int rows,
-                             void* stream) {
+extern "C" int gg_kv8_append(const gg_kv8_cache* c, const gg_kv8_append_call* call, void* stream) {
   using namespace gg;
   const char* fn = "gg_kv8_append";
-  if (!c || !k || !v || !slots) return ops_fail(GG_E_ARG, "%s: null argument", fn);
+  if (!c || !call || !call->slots) return ops_fail(GG_E_ARG, "%s: null argument", fn);
+  const gg_rows *k = &call->k, *v = &call->v;
+  const int32_t* slots = call->slots;
+  const int rows = call->rows;
   if (rows < 0) return ops_fail(GG_E_ARG, "%s: rows %d", fn, rows);
   if (int rc = ops_check_cache(fn, c)) return rc;
   if (int rc = ops_check_rows(fn, "k", k, rows, c->head_dim)) return rc;

@@ -8,6 +8,9 @@
 
 #include "../../include/gemma_b200.h"
 #include "gg_device.cuh"
+#include "gg_launch.h"
+
+#include <atomic>
 
 // Keeps the message for gg_last_error(NULL) and returns `code`.
 int ops_fail(int code, const char* fmt, ...);
@@ -26,10 +29,30 @@ inline bool ops_aligned16(const gg_rows& v) {
 
 namespace gg {
 
-template <int TYPE> struct elem;
-template <> struct elem<GG_T_F32> { typedef float type; };
-template <> struct elem<GG_T_BF16> { typedef __nv_bfloat16 type; };
-template <> struct elem<GG_T_F16> { typedef __half type; };
+// launch_pdl of a kernel that needs more dynamic shared memory than the default limit. The limit is
+// raised on the kernel's first launch on a device, and again when a launch is refused: a context made after cudaDeviceReset has forgotten it.
+template <typename... KArgs, typename... Args>
+inline cudaError_t launch_big_smem(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {
+  static std::atomic<void*> known[64][32];  // kernels of this signature whose limit is raised, per device
+  int dev = 0;
+  cudaError_t r = cudaGetDevice(&dev);
+  if (r != cudaSuccess) return r;
+  std::atomic<void*>* seen = known[dev & 63];
+  bool raised = false;
+  for (int i = 0; i < 32 && dev < 64; i++) raised |= seen[i].load(std::memory_order_acquire) == reinterpret_cast<void*>(kernel);
+  if (raised) {
+    r = launch_pdl(kernel, grid, block, smem, s, args...);
+    if (r != cudaErrorInvalidValue) return r;
+    cudaGetLastError();
+  }
+  r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (r != cudaSuccess) return r;
+  for (int i = 0; i < 32 && !raised && dev < 64; i++) {
+    void* none = nullptr;
+    if (seen[i].compare_exchange_strong(none, reinterpret_cast<void*>(kernel), std::memory_order_acq_rel)) break;
+  }
+  return launch_pdl(kernel, grid, block, smem, s, args...);
+}
 
 GG_DEV float to_f32(float v) { return v; }
 GG_DEV float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }

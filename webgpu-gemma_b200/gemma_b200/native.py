@@ -50,12 +50,12 @@ SIGNATURES = {
     "gg_selftest_wait": (_I, [_P, ctypes.c_uint64]),
     "gg_set_gemm_kernel": (_I, [_I]),
     "gg_sample_logits_noalloc": (_I, [_P, _I, _P, _P, _D, _P, _P]),
-    "gg_rope": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _D, _I, _P]),
+    "gg_rope": (_I, [_P, _P]),
     "gg_rope_freqs": (_I, [_I, _I, _D, _D, _D, _D, _D, _P, ctypes.POINTER(_D)]),
     "gg_plan_blocks": (_I, [_P, _P]),
-    "gg_kv8_append": (_I, [_P, _P, _P, _P, _I, _P]),
-    "gg_kv8_attention": (_I, [_P, _P, _P, _P, _P, _D, _I, _P, ctypes.c_size_t, _P]),
-    "gg_kv8_attention_workspace": (_I, [_P, _P, _P, _I, ctypes.POINTER(ctypes.c_size_t)]),
+    "gg_kv8_append": (_I, [_P, _P, _P]),
+    "gg_kv8_attention": (_I, [_P, _P, _P]),
+    "gg_kv8_attention_workspace": (_I, [_P, _P, ctypes.POINTER(ctypes.c_size_t)]),
     "gg_set_timeout": (_I, [_P, ctypes.c_uint64]),
     "gg_last_device_ms": (_I, [_P, ctypes.POINTER(ctypes.c_float)]),
     "gg_destroy": (_I, [_P]),
@@ -101,10 +101,20 @@ class GGKv8Cache(ctypes.Structure):
                 + [(n, ctypes.c_int32) for n in ("num_blocks", "block_tokens", "kv_heads", "head_dim", "code")])
 
 
-class GGKv8Batch(ctypes.Structure):
-    _fields_ = [("cu_rows", _P), ("lens", _P), ("table", _P), ("table_stride", ctypes.c_int64),
-                ("seqs", ctypes.c_int32), ("rows", ctypes.c_int32), ("max_rows", ctypes.c_int32),
-                ("max_len", ctypes.c_int32)]
+class GGRopeCall(ctypes.Structure):
+    _fields_ = ([(n, GGRows) for n in ("q", "k", "q_out", "k_out")]
+                + [("positions", _P), ("freqs", _P), ("mscale", ctypes.c_double)]
+                + [(n, ctypes.c_int32) for n in ("rows", "head_dim", "rot_dim", "layout", "inverse")])
+
+
+class GGKv8AppendCall(ctypes.Structure):
+    _fields_ = [("k", GGRows), ("v", GGRows), ("slots", _P), ("rows", ctypes.c_int32)]
+
+
+class GGKv8AttentionCall(ctypes.Structure):
+    _fields_ = [("q", GGRows), ("out", GGRows), ("lse", _P), ("cu_rows", _P), ("lens", _P), ("table", _P),
+                ("table_stride", ctypes.c_int64), ("workspace", _P), ("workspace_bytes", ctypes.c_size_t),
+                ("scale", ctypes.c_double)] + [(n, ctypes.c_int32) for n in ("seqs", "rows", "max_rows", "max_len", "window")]
 
 
 class GemmaB200Error(RuntimeError):

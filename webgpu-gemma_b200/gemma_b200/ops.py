@@ -17,12 +17,14 @@ gradients: tensors that require one are refused while grad mode is on. The gradi
 from __future__ import annotations
 
 import ctypes
+import struct
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
 
 from . import native
-from .native import GG_OK, GemmaB200Error, GGBlockPlan, GGKv8Batch, GGKv8Cache, GGRows
+from .native import GG_OK, GemmaB200Error, GGKv8AttentionCall, GGKv8Cache, GGRows
 
 _TYPES = {torch.float32: native.GG_T_F32, torch.bfloat16: native.GG_T_BF16, torch.float16: native.GG_T_F16}
 _CODES = {torch.int8: native.GG_KV8_INT8, torch.float8_e4m3fn: native.GG_KV8_E4M3}
@@ -30,68 +32,97 @@ _LAYOUTS = {"half": native.GG_ROPE_HALF, "interleaved": native.GG_ROPE_INTERLEAV
 _SCALINGS = {"none": native.GG_ROPE_NONE, "linear": native.GG_ROPE_LINEAR, "bands": native.GG_ROPE_BANDS,
              "yarn": native.GG_ROPE_YARN}
 
+# A call of a few microseconds is made of host work as much as of the kernel, so the argument
+# structures of include/gemma_b200.h (native.GGRopeCall and its like) are packed here in one step
+# each and handed over as bytes: a third of the time that filling ctypes structures takes.
+_ROWS = "Pqqii"
+_pack_plan = struct.Struct("@PPPq" + "P" * 9 + "iiiiixxxx").pack
+_pack_rope = struct.Struct("@" + _ROWS * 4 + "PPdiiiiixxxx").pack
+_pack_append = struct.Struct("@" + _ROWS * 2 + "Pixxxx").pack
+_pack_attend = struct.Struct("@" + _ROWS * 2 + "PPPPqPNdiiiiixxxx").pack
+_NO_ROWS = (0, 0, 0, 0, 0)
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_lib = None
+
+
+def _library():
+    global _lib
+    if _lib is None:
+        _lib = native.load()
+    return _lib
+
 
 def _check(rc: int):
     if rc != GG_OK:
-        raise GemmaB200Error(rc, native.load().gg_last_error(None).decode())
+        raise GemmaB200Error(rc, _library().gg_last_error(None).decode())
 
 
-def _call(device: torch.device, fn, *args):
-    """fn(*args, stream) with `device` current, on its current stream."""
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            _check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+def _call(index: int, fn, *args):
+    """fn(*args, stream) with device `index` current, on its current stream."""
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     else:
-        _check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+        rc = fn(*args, _raw_stream(index))
+    if rc != GG_OK:
+        _check(rc)
 
 
-def _on_gpu(name: str, t: torch.Tensor, device: torch.device | None = None) -> torch.device:
-    if t.device.type != "cuda":
+def _gpu_index(name: str, t: torch.Tensor) -> int:
+    if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor, not on {t.device}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the other tensors on {device}")
-    return t.device
+    return t.get_device()
 
 
-def _rows(name: str, t: torch.Tensor, device: torch.device) -> GGRows:
-    """View of a [rows][heads][head_dim] tensor of any strides with contiguous heads."""
-    if t.dim() != 3:
+def _elsewhere(name: str, t: torch.Tensor, index: int):
+    _gpu_index(name, t)
+    raise ValueError(f"{name} is on {t.device}, the other tensors on cuda:{index}")
+
+
+def _rows(name: str, t: torch.Tensor, index: int) -> tuple:
+    """gg_rows of a [rows][heads][head_dim] tensor of any strides with contiguous heads."""
+    stride = t.stride()
+    if len(stride) != 3:
         raise ValueError(f"{name} must be [rows][heads][head_dim], not {tuple(t.shape)}")
     type_ = _TYPES.get(t.dtype)
     if type_ is None:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
-    if t.device != device:
-        _on_gpu(name, t, device)
+    if t.get_device() != index:
+        _elsewhere(name, t, index)
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient, which this operator does not record")
-    sr, sh, sd = t.stride()
-    if sd != 1 and t.shape[2] > 1:
-        raise ValueError(f"the values of a head of {name} must be contiguous (stride {sd})")
+    shape = t.shape
+    if stride[2] != 1 and shape[2] > 1:
+        raise ValueError(f"the values of a head of {name} must be contiguous (stride {stride[2]})")
     # a data pointer of an empty tensor is null; no row of it is read
-    return GGRows(t.data_ptr() or 16, sr, sh, t.shape[1], type_)
+    return t.data_ptr() or 16, stride[0], stride[1], shape[1], type_
 
 
-def _ints(name: str, t: torch.Tensor, device: torch.device, numel: int | None = None, at_least: bool = False) -> int:
+def _ints(name: str, t: torch.Tensor, index: int, numel: int) -> int:
     if t.dtype != torch.int32:
         raise ValueError(f"{name} must be int32, not {t.dtype}")
-    if t.device != device:
-        _on_gpu(name, t, device)
-    if t.dim() != 1 or (t.stride(0) != 1 and t.shape[0] > 1):
-        raise ValueError(f"{name} must be a contiguous 1-D tensor")
-    if numel is not None and (t.shape[0] < numel if at_least else t.shape[0] != numel):
-        raise ValueError(f"{name} has {t.shape[0]} entries, {'at least ' if at_least else ''}{numel} needed")
+    if t.get_device() != index:
+        _elsewhere(name, t, index)
+    if t.shape != (numel,):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, ({numel},) needed")
+    if numel > 1 and t.stride() != (1,):
+        raise ValueError(f"{name} must be contiguous")
     return t.data_ptr() or 16
 
 
-def _table(t: torch.Tensor, device: torch.device, seqs: int) -> tuple[int, int]:
-    if t.dtype != torch.int32 or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
-        raise ValueError(f"table must be an int32 [requests][blocks] tensor with contiguous rows, not {t.dtype} {tuple(t.shape)}")
-    _on_gpu("table", t, device)
-    if t.shape[0] != seqs:
-        raise ValueError(f"table has {t.shape[0]} rows for {seqs} requests")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+def _table(t: torch.Tensor, index: int, seqs: int) -> tuple:
+    """(pointer, row stride, blocks of a row)"""
+    shape, stride = t.shape, t.stride()
+    if t.dtype != torch.int32 or len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
+        raise ValueError(f"table must be an int32 [requests][blocks] tensor with contiguous rows, not {t.dtype} {tuple(shape)}")
+    if t.get_device() != index:
+        _elsewhere("table", t, index)
+    if shape[0] != seqs:
+        raise ValueError(f"table has {shape[0]} rows for {seqs} requests")
+    if shape[0] > 1 and stride[0] < shape[1]:
         raise ValueError("the rows of table overlap")
-    return t.data_ptr() or 16, max(t.stride(0), t.shape[1])
+    return t.data_ptr() or 16, max(stride[0], shape[1]), shape[1]
 
 
 class BlockPlan(NamedTuple):
@@ -112,21 +143,23 @@ def plan_blocks(old_len: torch.Tensor, new_len: torch.Tensor, table: torch.Tenso
     ``new_len[i]`` tokens (gg_plan_blocks). ``table`` and ``free_list`` are updated in place;
     ``free_count`` only if it is also ``out.free_count``. ``rows`` is the size of the row arrays.
     A plan that does not fit changes nothing and says so in ``status``."""
-    dev = _on_gpu("old_len", old_len)
+    dev = _gpu_index("old_len", old_len)
     n = old_len.shape[0] if old_len.dim() else 0
     if out is None:
-        flat = torch.empty(2 * n + 3 + 3 * rows, dtype=torch.int32, device=dev)
-        a, b = 2 * n + 1, 2 * n + 3
-        out = BlockPlan(flat[:n + 1], flat[n + 1:a], flat[b:b + rows], flat[b + rows:b + 2 * rows], flat[b + 2 * rows:],
-                        flat[a:a + 1], flat[a + 1:b])
-    tp, stride = _table(table, dev, n)
-    p = GGBlockPlan(_ints("old_len", old_len, dev, n), _ints("new_len", new_len, dev, n), tp, stride,
-                    _ints("free_list", free_list, dev), _ints("free_count", free_count, dev, 1),
-                    _ints("out.cu_rows", out.cu_rows, dev, n + 1), _ints("out.lens", out.lens, dev, n),
-                    _ints("out.row_seq", out.row_seq, dev, rows), _ints("out.positions", out.positions, dev, rows),
-                    _ints("out.slots", out.slots, dev, rows), _ints("out.free_count", out.free_count, dev, 1),
-                    _ints("out.status", out.status, dev, 1), n, table.shape[1], block_tokens, free_list.shape[0], rows)
-    _call(dev, native.load().gg_plan_blocks, ctypes.byref(p))
+        if rows < 0:
+            raise ValueError(f"rows must not be negative, not {rows}")
+        flat = torch.empty(2 * n + 3 + 3 * rows, dtype=torch.int32, device=old_len.device)
+        out = BlockPlan(*flat.split_with_sizes((n + 1, n, rows, rows, rows, 1, 1)))
+        p = flat.data_ptr()
+        q = p + 4 * (2 * n + 1)
+        outs = (p, p + 4 * (n + 1), q, q + 4 * rows, q + 8 * rows, q + 12 * rows, q + 12 * rows + 4)
+    else:
+        outs = tuple(_ints("out." + name, t, dev, k) for name, t, k in zip(out._fields, out, (n + 1, n, rows, rows, rows, 1, 1)))
+    tp, stride, blocks = _table(table, dev, n)
+    free = free_list.shape[0] if free_list.dim() else 0
+    _call(dev, _library().gg_plan_blocks,
+          _pack_plan(_ints("old_len", old_len, dev, n), _ints("new_len", new_len, dev, n), tp, stride, _ints("free_list", free_list, dev, free),
+                     _ints("free_count", free_count, dev, 1), *outs, n, blocks, block_tokens, free, rows))
     return out
 
 
@@ -148,29 +181,50 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs
     """Rotary positions on q [rows][heads][head_dim] and k (or None) in one kernel (gg_rope); rotates
     the first 2 * len(freqs) values of each head. Returns (q, k) as new tensors, or ``out``, which may
     be (q, k) itself. A row at a negative position is copied."""
-    dev = _on_gpu("q", q)
+    dev = _gpu_index("q", q)
     code = _LAYOUTS.get(layout)
     if code is None:
         raise ValueError(f"unknown layout {layout!r} (half or interleaved)")
-    if freqs.dtype != torch.float64 or freqs.dim() != 1 or (freqs.shape[0] > 1 and freqs.stride(0) != 1):
+    pairs = freqs.shape[0] if freqs.dim() == 1 else 0
+    if freqs.dtype != torch.float64 or not pairs or (pairs > 1 and freqs.stride(0) != 1):
         raise ValueError("freqs must be a contiguous float64 vector (rope_frequencies)")
-    _on_gpu("freqs", freqs, dev)
+    if freqs.get_device() != dev:
+        _elsewhere("freqs", freqs, dev)
     vq = _rows("q", q, dev)
-    vk = _rows("k", k, dev) if k is not None else None
-    if k is not None and (k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.dtype != q.dtype):
-        raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} differ in rows, head_dim or type")
+    n, _, dim = q.shape
+    vk = wk = _NO_ROWS
+    if k is not None:
+        vk = _rows("k", k, dev)
+        if k.shape[0] != n or k.shape[2] != dim or vk[4] != vq[4]:
+            raise ValueError(f"q {tuple(q.shape)} {q.dtype} and k {tuple(k.shape)} {k.dtype} differ in rows, head_dim or type")
     if out is None:
-        out = (torch.empty(q.shape, dtype=q.dtype, device=dev), None if k is None else torch.empty(k.shape, dtype=k.dtype, device=dev))
-    oq, ok = out
-    if oq.shape != q.shape or (k is None) != (ok is None) or (k is not None and ok.shape != k.shape):
-        raise ValueError("out must be (q, k) of the same shapes")
-    wq = _rows("out[0]", oq, dev)
-    wk = _rows("out[1]", ok, dev) if ok is not None else None
-    ref = ctypes.byref
-    _call(dev, native.load().gg_rope, ref(vq), ref(vk) if vk is not None else None, ref(wq), ref(wk) if wk is not None else None,
-          q.shape[0], q.shape[2], 2 * freqs.shape[0], code, _ints("positions", positions, dev, q.shape[0]), freqs.data_ptr() or 16,
-          mscale, 1 if inverse else 0)
+        oq = torch.empty_like(q, memory_format=torch.contiguous_format)
+        wq = (oq.data_ptr() or 16, vq[3] * dim, dim, vq[3], vq[4])
+        ok = None
+        if k is not None:
+            ok = torch.empty_like(k, memory_format=torch.contiguous_format)
+            wk = (ok.data_ptr() or 16, vk[3] * dim, dim, vk[3], vk[4])
+    else:
+        oq, ok = out
+        if oq.shape != q.shape or (k is None) != (ok is None) or (k is not None and ok.shape != k.shape):
+            raise ValueError("out must be (q, k) of the same shapes")
+        wq = _rows("out[0]", oq, dev)
+        if ok is not None:
+            wk = _rows("out[1]", ok, dev)
+    _call(dev, _library().gg_rope,
+          _pack_rope(*vq, *vk, *wq, *wk, _ints("positions", positions, dev, n), freqs.data_ptr(), mscale, n, dim, 2 * pairs, code,
+                     1 if inverse else 0))
     return oq, ok
+
+
+@lru_cache(maxsize=1024)
+def _attend_bytes(num_blocks, block_tokens, kv_heads, head_dim, code, heads, type_, seqs, rows, max_rows, max_len, window) -> int:
+    """Workspace of a call of these sizes (a pure function of them)."""
+    c = GGKv8Cache(16, 16, 16, 16, num_blocks, block_tokens, kv_heads, head_dim, code)
+    call = GGKv8AttentionCall(q=GGRows(heads=heads, type=type_), seqs=seqs, rows=rows, max_rows=max_rows, max_len=max_len, window=window)
+    need = ctypes.c_size_t()
+    _check(_library().gg_kv8_attention_workspace(ctypes.byref(c), ctypes.byref(call), ctypes.byref(need)))
+    return need.value
 
 
 class KV8Cache:
@@ -178,7 +232,7 @@ class KV8Cache:
     [head_dim] (int8 or float8_e4m3fn) and scales [blocks][kv_heads] (float32), for K and for V."""
 
     def __init__(self, k_codes: torch.Tensor, v_codes: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor):
-        dev = _on_gpu("k_codes", k_codes)
+        dev = _gpu_index("k_codes", k_codes)
         if k_codes.dim() != 4 or k_codes.dtype not in _CODES:
             raise ValueError(f"codes must be int8 or float8_e4m3fn [blocks][kv_heads][block_tokens][head_dim], not {k_codes.dtype} {tuple(k_codes.shape)}")
         if v_codes.shape != k_codes.shape or v_codes.dtype != k_codes.dtype:
@@ -187,15 +241,16 @@ class KV8Cache:
             if t.dtype != torch.float32 or t.shape != k_codes.shape[:2]:
                 raise ValueError(f"{name} must be float32 {tuple(k_codes.shape[:2])}, not {t.dtype} {tuple(t.shape)}")
         for name, t in (("k_codes", k_codes), ("v_codes", v_codes), ("k_scale", k_scale), ("v_scale", v_scale)):
-            _on_gpu(name, t, dev)
+            if t.get_device() != dev:
+                _elsewhere(name, t, dev)
             if not t.is_contiguous():
                 raise ValueError(f"{name} must be contiguous")
         self.k_codes, self.v_codes, self.k_scale, self.v_scale = k_codes, v_codes, k_scale, v_scale
-        self.device = dev
+        self.device = k_codes.device
+        self._index = dev
         self.num_blocks, self.kv_heads, self.block_tokens, self.head_dim = k_codes.shape
-        self._c = GGKv8Cache(k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), self.num_blocks,
-                             self.block_tokens, self.kv_heads, self.head_dim, _CODES[k_codes.dtype])
-        self._ref = ctypes.byref(self._c)
+        self._sizes = (self.num_blocks, self.block_tokens, self.kv_heads, self.head_dim, _CODES[k_codes.dtype])
+        self._c = bytes(GGKv8Cache(k_codes.data_ptr(), v_codes.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *self._sizes))
 
     @classmethod
     def empty(cls, num_blocks: int, block_tokens: int, kv_heads: int, head_dim: int, code: str = "int8", device="cuda") -> "KV8Cache":
@@ -210,12 +265,13 @@ class KV8Cache:
 
     def append(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantises k and v [rows][kv_heads][head_dim] into ``slots`` (-1: no slot), as gg_kv8_append."""
-        dev = self.device
-        for name, t in (("k", k), ("v", v)):
-            if t.dim() != 3 or t.shape[2] != self.head_dim or t.shape[0] != k.shape[0]:
-                raise ValueError(f"{name} must be [rows][{self.kv_heads}][{self.head_dim}], not {tuple(t.shape)}")
+        dev = self._index
         vk, vv = _rows("k", k, dev), _rows("v", v, dev)
-        _call(dev, native.load().gg_kv8_append, self._ref, ctypes.byref(vk), ctypes.byref(vv), _ints("slots", slots, dev, k.shape[0]), k.shape[0])
+        shape = k.shape
+        if shape[2] != self.head_dim or v.shape[2] != self.head_dim or v.shape[0] != shape[0]:
+            raise ValueError(f"k and v must be [rows][{self.kv_heads}][{self.head_dim}], not {tuple(shape)} and {tuple(v.shape)}")
+        n = shape[0]
+        _call(dev, _library().gg_kv8_append, self._c, _pack_append(*vk, *vv, _ints("slots", slots, dev, n), n))
 
     def attend(self, q: torch.Tensor, cu_rows: torch.Tensor, lens: torch.Tensor, table: torch.Tensor, *, max_rows: int, max_len: int,
                scale: float | None = None, window: int = 0, out: torch.Tensor | None = None, return_lse: bool = False,
@@ -225,39 +281,40 @@ class KV8Cache:
         ``scale`` defaults to head_dim^-0.5. Returns out, or (out, lse) with the rows' f32 log-sum-exp.
         Rows behind the last request are not written (a new ``out`` holds anything there). Without a
         ``workspace`` (uint8) the call takes one from torch's allocator."""
-        dev = self.device
+        dev = self._index
         vq = _rows("q", q, dev)
-        if q.shape[2] != self.head_dim:
-            raise ValueError(f"q has head_dim {q.shape[2]}, the cache {self.head_dim}")
-        n, rows = lens.shape[0] if lens.dim() else 0, q.shape[0]
+        rows, heads, dim = shape = q.shape
+        if dim != self.head_dim:
+            raise ValueError(f"q has head_dim {dim}, the cache {self.head_dim}")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        elif out.shape != q.shape:
-            raise ValueError(f"out is {tuple(out.shape)}, q {tuple(q.shape)}")
-        vo = _rows("out", out, dev)
-        tp, stride = _table(table, dev, n)
-        if max_len > table.shape[1] * self.block_tokens:
-            raise ValueError(f"max_len {max_len} is more than a table row of {table.shape[1]} blocks holds")
-        batch = GGKv8Batch(_ints("cu_rows", cu_rows, dev, n + 1), _ints("lens", lens, dev, n), tp, stride, n, rows, max_rows, max_len)
-        lib, ref = native.load(), ctypes.byref
-        need = ctypes.c_size_t()
-        _check(lib.gg_kv8_attention_workspace(self._ref, ref(vq), ref(batch), window, ref(need)))
-        if workspace is None:
-            workspace = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-        elif workspace.dtype != torch.uint8 or workspace.dim() != 1 or not workspace.is_contiguous():
-            raise ValueError("workspace must be a contiguous uint8 vector")
-        elif workspace.device != dev:
-            _on_gpu("workspace", workspace, dev)
-        lse = torch.empty(rows, q.shape[1], dtype=torch.float32, device=dev) if return_lse else None
-        _call(dev, lib.gg_kv8_attention, self._ref, ref(vq), ref(vo), lse.data_ptr() or None if lse is not None else None, ref(batch),
-              self.head_dim ** -0.5 if scale is None else scale, window, workspace.data_ptr() if workspace is not None else None,
-              workspace.numel() if workspace is not None else 0)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            vo = (out.data_ptr() or 16, heads * dim, dim, heads, vq[4])
+        else:
+            if out.shape != shape:
+                raise ValueError(f"out is {tuple(out.shape)}, q {tuple(shape)}")
+            vo = _rows("out", out, dev)
+        n = lens.shape[0] if lens.dim() else 0
+        tp, stride, blocks = _table(table, dev, n)
+        if max_len > blocks * self.block_tokens:
+            raise ValueError(f"max_len {max_len} is more than a table row of {blocks} blocks holds")
+        need = _attend_bytes(*self._sizes, heads, vq[4], n, rows, max_rows, max_len, window)
+        wp = size = 0
+        if workspace is not None:
+            if workspace.dtype != torch.uint8 or workspace.dim() != 1 or not workspace.is_contiguous():
+                raise ValueError("workspace must be a contiguous uint8 vector")
+            if workspace.get_device() != dev:
+                _elsewhere("workspace", workspace, dev)
+            wp, size = workspace.data_ptr(), workspace.numel()
+        elif need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+            wp, size = workspace.data_ptr(), need
+        lse = torch.empty(rows, heads, dtype=torch.float32, device=self.device) if return_lse else None
+        _call(dev, _library().gg_kv8_attention, self._c,
+              _pack_attend(*vq, *vo, lse.data_ptr() if lse is not None else 0, _ints("cu_rows", cu_rows, dev, n + 1), _ints("lens", lens, dev, n),
+                           tp, stride, wp, size, dim ** -0.5 if scale is None else scale, n, rows, max_rows, max_len, window))
         return (out, lse) if return_lse else out
 
     def workspace_bytes(self, q: torch.Tensor, seqs: int, max_rows: int, max_len: int, window: int = 0) -> int:
         """Bytes of ``workspace`` that ``attend`` needs for such a batch."""
-        vq = _rows("q", q, self.device)
-        batch = GGKv8Batch(16, 16, 16, -(-max_len // self.block_tokens), seqs, q.shape[0], max_rows, max_len)
-        need = ctypes.c_size_t()
-        _check(native.load().gg_kv8_attention_workspace(self._ref, ctypes.byref(vq), ctypes.byref(batch), window, ctypes.byref(need)))
-        return need.value
+        vq = _rows("q", q, self._index)
+        return _attend_bytes(*self._sizes, vq[3], vq[4], seqs, q.shape[0], max_rows, max_len, window)
