@@ -23,8 +23,9 @@ namespace gg {
 template <int HD, bool HILO>
 struct PromptShape {
   static constexpr int NQ = HD == 256 ? 1 : 2;                       // query tiles of 128 rows
-  static constexpr int KT = HD == 64 || (HD == 128 && !HILO) ? 128 : 64;  // keys of a tile
-  static constexpr int ST = HD == 256 && HILO ? 1 : 2;               // ring stages of K and of V
+  static constexpr int KT = 64;                                      // keys of a tile
+  static constexpr int ST = HD == 256 ? (HILO ? 1 : 2) : HILO ? 2 : 4;  // ring stages of K and of V
+  static constexpr bool EARLY_K = ST <= 2;
   static constexpr int Q_BYTES = 128 * HD * 2 * (HILO ? 2 : 1);      // per query tile
   static constexpr int KV_BYTES = KT * HD * 2;
   static constexpr int GROUPS = 256;                                 // 16-key groups in the scale ring
@@ -36,9 +37,9 @@ struct PromptShape {
   static constexpr int SMEM = OFF_BAR + 256 + 1024;  // + alignment of the operand tiles
   static constexpr int SOFT_WARPS = 4 * NQ, CONV_WARPS = 4;
   static constexpr int THREADS = (SOFT_WARPS + CONV_WARPS + 1) * 32;
-  static constexpr int TMEM_S = KT;               // columns of one S buffer (two of them)
-  static constexpr int TMEM_O = 2 * KT;           // first column of O
-  static_assert(2 * KT + NQ * HD <= 512, "TMEM columns");
+  static constexpr int TMEM_S = KT;               // columns of one S buffer: two for each query tile
+  static constexpr int TMEM_O = 2 * NQ * KT;      // first column of O
+  static_assert(2 * NQ * KT + NQ * HD <= 512, "TMEM columns");
 };
 
 // MN-major operand, 128-byte swizzle: rows of 64 values of the N index, 8 rows (K index) to an
@@ -56,13 +57,33 @@ GG_DEV uint64_t umma_desc_sw128_mn(uint32_t saddr, uint32_t slab) {
 GG_DEV uint32_t umma_idesc_f16_m128(int n, bool b_mn) {
   return (1u << 4) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-// D(tmem) (+)= A(tmem) x B(smem desc)
-GG_DEV void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// D(tmem) (+)= A x B, A from shared memory (descriptor) or TMEM, issued by the lanes with `on` set
+// (one of them). The whole warp runs the code around them, so that addresses and descriptors stay
+// in uniform registers: issued from a branch that one lane takes, each MMA first moves seven
+// registers there (150 instead of 80 cycles an MMA).
+GG_DEV void umma_f16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate, uint32_t on) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+GG_DEV void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, uint32_t accumulate, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+GG_DEV void umma_commit_on(uint64_t* bar, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)), "r"(on)
       : "memory");
 }
 GG_DEV void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -95,6 +116,27 @@ GG_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
 }
 GG_DEV void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two f32 at a time, each rounded to nearest as the single operations are.
+GG_DEV uint64_t pack2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+GG_DEV void fma2(uint32_t& a, uint32_t& b, uint64_t f, uint64_t c) {  // (a, b) = (a, b) f + c
+  asm("{\n\t.reg .b64 x;\n\tmov.b64 x, {%0, %1};\n\tfma.rn.f32x2 x, x, %2, %3;\n\tmov.b64 {%0, %1}, x;\n\t}" : "+r"(a), "+r"(b) : "l"(f), "l"(c));
+}
+GG_DEV void add2(uint64_t& s, float a, float b) { asm("{\n\t.reg .b64 x;\n\tmov.b64 x, {%1, %2};\n\tadd.rn.f32x2 %0, %0, x;\n\t}" : "+l"(s) : "f"(a), "f"(b)); }
+GG_DEV float sum2(uint64_t s) {
+  float a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(s));
+  return a + b;
+}
+GG_DEV float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // Wait for an mbarrier phase; after two seconds (or when another warp gave up) sets *abort and
 // returns false: the CTA then drains its MMAs and leaves NaN in its rows.
 GG_DEV bool prompt_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
@@ -121,17 +163,17 @@ GG_DEV bool prompt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort
 template <int HD, int CODE, bool HILO>
 __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prompt_kernel(const Kv8Args a) {
   typedef PromptShape<HD, HILO> S;
-  constexpr int NQ = S::NQ, KT = S::KT, ST = S::ST, GT = KT / 16, HALVES = KT / 64;
+  constexpr int NQ = S::NQ, KT = S::KT, ST = S::ST, GT = KT / 16;
   extern __shared__ unsigned char prompt_smem[];
   unsigned char* sm = prompt_smem + ((1024 - (smem_u32(prompt_smem) & 1023)) & 1023);
   float4* meta = reinterpret_cast<float4*>(sm + S::OFF_META);  // per 16-key group: ks, log2 vs, 1 / vs
   float* s_mul = reinterpret_cast<float*>(sm + S::OFF_MUL);
   uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + S::OFF_BAR);
-  uint64_t *kempty = kfull + 2, *vfull = kfull + 4, *vempty = kfull + 6, *sfull = kfull + 8, *pfull = kfull + 10,
-           *odone = kfull + 12, *drain = kfull + 14;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 15);
+  // kfull, vfull, done: by ring stage; sfull: by the key tile's parity; pfull: [query tile][parity]
+  uint64_t *vfull = kfull + 4, *done = kfull + 8, *sfull = kfull + 12, *pfull = kfull + 14, *drain = kfull + 18, *kdone = kfull + 19;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 21);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   constexpr int MMA_WARP = S::SOFT_WARPS + S::CONV_WARPS;
 
   pdl_wait();
@@ -155,14 +197,15 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
     if (lane == 0) {
-      for (int i = 0; i < 2; i++) {
+      for (int i = 0; i < 4; i++) {
         mbar_init(&kfull[i], S::CONV_WARPS);
-        mbar_init(&kempty[i], 1);
         mbar_init(&vfull[i], S::CONV_WARPS);
-        mbar_init(&vempty[i], 1);
-        mbar_init(&sfull[i], 1);
+        mbar_init(&done[i], 1);
         mbar_init(&pfull[i], 4);
-        mbar_init(&odone[i], 1);
+      }
+      for (int i = 0; i < 2; i++) {
+        mbar_init(&sfull[i], 1);
+        mbar_init(&kdone[i], 1);
       }
       mbar_init(drain, 1);
       *abort = 0;
@@ -245,46 +288,45 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
 
   if (nt && warp >= S::SOFT_WARPS && warp < MMA_WARP) {
     // ------------------------------------------------------------------ converter warps
+    // A thread keeps one 16-byte word of a key row and takes every KS-th key; a warp takes KPW keys
+    // at once, all of one 16-key group, so block ids are the same for all its lanes. Eight lanes
+    // hold four words of one 64-value slab of two neighbouring keys: their f16 chunks fall on
+    // eight different bank groups.
     const int ct = tid - S::SOFT_WARPS * 32;
-    constexpr int WORDS = KT * HD / 16 / 128;  // 16-byte words of a thread and tile
-    const int W = a.hd >> 4, total = KT * W;
-    const uint32_t wmagic = (65536u + W - 1) / W;  // x / W for x < 2048
+    constexpr int WP = HD / 16, KPW = 32 / WP, KS = S::CONV_WARPS * KPW, WORDS = KT / KS;
+    const int k0 = (ct >> 5) * KPW + ((lane >> 2) & (KPW - 1)), w = (lane / (4 * KPW)) * 4 + (lane & 3);
+    const bool mine = w * 16 < a.hd;
     constexpr int TB = 64 / GT;  // tiles of a batch of 64 groups
     int cur[2] = {load_id(lane), load_id(lane + 32)}, nxt[2] = {-1, -1};  // this batch's ids and the next one's
+    const long long block_bytes = (long long)a.kv_heads * a.hd << a.block_shift, head_bytes = (long long)h * a.hd << a.block_shift;
+    const int tok_mask = (1 << a.block_shift) - 1;
     const auto fetch = [&](const uint8_t* codes, int tile, int batch, uint4 (&r)[WORDS]) {
+      const bool now = tile / TB == batch;
+      const int id_lo = now ? cur[0] : nxt[0], id_hi = now ? cur[1] : nxt[1];
+      const uint8_t* base = codes + head_bytes + w * 16;
 #pragma unroll
       for (int i = 0; i < WORDS; i++) {
-        const int xw = ct + 128 * i;
-        const int k = (int)(((uint32_t)xw * wmagic) >> 16), w = xw - k * W;
-        const int group = (tile * GT + (k >> 4)) & 63;
-        const bool now = tile / TB == batch;
-        const int id0 = __shfl_sync(0xffffffffu, now ? cur[0] : nxt[0], group & 31);
-        const int id1 = __shfl_sync(0xffffffffu, now ? cur[1] : nxt[1], group & 31);
-        const int id = group & 32 ? id1 : id0, key = k00 + tile * KT + k;
+        const int k = k0 + KS * i, group = (tile * GT + (k >> 4)) & 63;
+        const int id = __shfl_sync(0xffffffffu, group & 32 ? id_hi : id_lo, group & 31);
+        const int key = k00 + tile * KT + k;
         r[i] = make_uint4(0, 0, 0, 0);
-        if (tile < nt && xw < total && id >= 0 && key < sq.len) {
-          const long long at = (((long long)id * a.kv_heads + h) << a.block_shift) + (key & ((1 << a.block_shift) - 1));
-          r[i] = __ldg(reinterpret_cast<const uint4*>(codes + at * a.hd) + w);
-        }
+        if (mine && id >= 0 && key < sq.len) r[i] = __ldg(reinterpret_cast<const uint4*>(base + id * block_bytes + (key & tok_mask) * a.hd));
       }
     };
+    const uint32_t row0 = (w >> 2) * (KT * 128) + (k0 >> 3) * 1024 + (k0 & 7) * 128;
+    const uint32_t at0 = row0 + ((((w & 3) * 2) ^ (k0 & 7)) << 4), at1 = row0 + ((((w & 3) * 2 + 1) ^ (k0 & 7)) << 4);
+    static_assert(KS % 8 == 0 && KPW <= 8, "key rows of a thread share their swizzle");
     const auto put = [&](unsigned char* tile, const uint4 (&r)[WORDS]) {
+      if (mine) {
 #pragma unroll
-      for (int i = 0; i < WORDS; i++) {
-        const int xw = ct + 128 * i;
-        if (xw < total) {
-          const int k = (int)(((uint32_t)xw * wmagic) >> 16), w = xw - k * W;
+        for (int i = 0; i < WORDS; i++) {
           uint4 lo, hi;
           widen4<CODE>(r[i].x, lo.x, lo.y);
           widen4<CODE>(r[i].y, lo.z, lo.w);
           widen4<CODE>(r[i].z, hi.x, hi.y);
           widen4<CODE>(r[i].w, hi.z, hi.w);
-          unsigned char* row = tile + (w >> 2) * (KT * 128) + (k >> 3) * 1024 + (k & 7) * 128;
-          const int c = (w & 3) * 2;
-          // lanes of neighbouring slabs store their two chunks in opposite order (bank conflicts)
-          const bool odd = (w >> 2) & 1;
-          *reinterpret_cast<uint4*>(row + (((c + odd) ^ (k & 7)) << 4)) = odd ? hi : lo;
-          *reinterpret_cast<uint4*>(row + (((c + !odd) ^ (k & 7)) << 4)) = odd ? lo : hi;
+          *reinterpret_cast<uint4*>(tile + at0 + i * (KS * 128)) = lo;
+          *reinterpret_cast<uint4*>(tile + at1 + i * (KS * 128)) = hi;
         }
       }
       fence_proxy_async_smem();
@@ -306,77 +348,84 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         for (int j = 0; j < 2; j++) sc[j] = load_scales(nxt[j]);
       if (ct < 32 && q == TB / 2)
         for (int j = 0; j < 2; j++) put_group((b + 1) * 64 + lane + 32 * j, nxt[j], sc[j]);
-      if (i >= ST && !prompt_wait_warp(&kempty[st], par ^ 1, abort)) break;
+      // A stage is free once both products of the tile that had it are done; with few stages its K
+      // is waited for, and handed back, by itself once the scores are.
+      if (i >= ST && !prompt_wait_warp(S::EARLY_K ? &kdone[st] : &done[st], par ^ 1, abort)) break;
       put(sm + S::OFF_K + st * S::KV_BYTES, rk);
       __syncwarp();
       if (lane == 0) mbar_arrive(&kfull[st]);
       fetch(a.kc, i + 1, b, rk);
-      if (i >= ST && !prompt_wait_warp(&vempty[st], par ^ 1, abort)) break;
+      if (S::EARLY_K && i >= ST && !prompt_wait_warp(&done[st], par ^ 1, abort)) break;
       put(sm + S::OFF_V + st * S::KV_BYTES, rv);
       __syncwarp();
       if (lane == 0) mbar_arrive(&vfull[st]);
       fetch(a.vc, i + 1, b, rv);
     }
   } else if (nt && warp == MMA_WARP) {
-    // ------------------------------------------------------------------ MMA issue (one thread)
-    if (lane == 0) {
-      const int steps = a.hd >> 4;
-      const uint32_t idesc_s = umma_idesc_f16_m128(KT, false), idesc_o = umma_idesc_f16_m128(a.hd, true);
-      const uint32_t sq_base = smem_u32(sm), sk_base = smem_u32(sm + S::OFF_K), sv_base = smem_u32(sm + S::OFF_V);
-      const auto scores = [&](int q, int i, int buf) {  // S buffer = Q tile q x K tile i
-        const uint32_t d = tmem + buf * S::TMEM_S, qb = sq_base + q * S::Q_BYTES, kb = sk_base + (i % ST) * S::KV_BYTES;
+    // ------------------------------------------------------------------ MMA issue (lane 0's MMAs)
+    const uint32_t on = lane == 0;
+    // the same in every lane, which the compiler sees of a shuffle's result but not of a load's
+    const int tiles = __shfl_sync(0xffffffffu, nt, 0);
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    const int steps = a.hd >> 4;
+    const uint32_t idesc_s = umma_idesc_f16_m128(KT, false), idesc_o = umma_idesc_f16_m128(a.hd, true);
+    const uint64_t qd = umma_desc_sw128(smem_u32(sm)), kd = umma_desc_sw128(smem_u32(sm + S::OFF_K));
+    const uint64_t vd = umma_desc_sw128_mn(smem_u32(sm + S::OFF_V), KT * 128);
+    // descriptors count 16-byte units; the address field does not overflow (227 KB of shared memory)
+    const auto scores = [&](int i) {  // S buffers = Q tiles x K tile i
+      const uint64_t kb = kd + (uint32_t)(i % ST) * (S::KV_BYTES / 16);
+#pragma unroll
+      for (int q = 0; q < NQ; q++)
+#pragma unroll
         for (int part = 0; part < (HILO ? 2 : 1); part++)
-          for (int k = 0; k < steps; k++)
-            umma_bf16(d, umma_desc_sw128(qb + part * (S::Q_BYTES / 2) + (k >> 2) * (128 * 128) + (k & 3) * 32),
-                      umma_desc_sw128(kb + (k >> 2) * (KT * 128) + (k & 3) * 32), idesc_s, part > 0 || k > 0);
-        umma_commit(&sfull[buf]);
-      };
-      const auto outputs = [&](int q, int i, int buf) {  // O tile q += P x V tile i
-        const uint32_t d = tmem + S::TMEM_O + q * HD, p = tmem + buf * S::TMEM_S, vb = sv_base + (i % ST) * S::KV_BYTES;
-        for (int k = 0; k < KT / 16; k++)
-          for (int part = 0; part < (HILO ? 2 : 1); part++)
-            umma_f16_ts(d, p + (k >> 2) * 64 + part * 32 + (k & 3) * 8, umma_desc_sw128_mn(vb + k * 2048, KT * 128), idesc_o,
-                        i > 0 || k > 0 || part > 0);
-        umma_commit(&odone[q]);
-      };
-      bool ok = prompt_wait(&kfull[0], 0, abort);
-      tc_fence_after();
-      if (ok) {
-        for (int q = 0; q < NQ; q++) scores(q, 0, q);
-        umma_commit(&kempty[0]);
+#pragma unroll
+          for (int k = 0; k < HD / 16; k++)
+            if (k < steps)
+              umma_f16_ss(tm + (2 * q + (i & 1)) * S::TMEM_S, qd + q * (S::Q_BYTES / 16) + part * (S::Q_BYTES / 32) + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2,
+                          kb + (k >> 2) * (KT * 128 / 16) + (k & 3) * 2, idesc_s, part > 0 || k > 0, on);
+      umma_commit_on(&sfull[i & 1], on);
+      if constexpr (S::EARLY_K) umma_commit_on(&kdone[i % ST], on);
+    };
+    const auto outputs = [&](int q, int i) {  // O tile q += P x V tile i
+      const uint32_t d = tm + S::TMEM_O + q * HD, p = tm + (2 * q + (i & 1)) * S::TMEM_S;
+      const uint64_t vb = vd + (uint32_t)(i % ST) * (S::KV_BYTES / 16);
+#pragma unroll
+      for (int k = 0; k < KT / 16; k++)
+#pragma unroll
+        for (int part = 0; part < (HILO ? 2 : 1); part++)
+          umma_f16_ts(d, p + part * 32 + k * 8, vb + k * (2048 / 16), idesc_o, i > 0 || k > 0 || part > 0, on);
+    };
+    // A tile's scores are issued before the weights of the tile before are ready, so the softmax
+    // warps hardly wait for them; they overwrite the weights of two tiles before, whose product was
+    // issued earlier (the MMAs of one thread run in order). Each commit takes the tensor pipe as
+    // long as an MMA of N = 64 (62 cycles), hence only two or three of them for a tile.
+    bool ok = prompt_wait_warp(&kfull[0], 0, abort);
+    tc_fence_after();
+    if (ok) scores(0);
+    for (int i = 0; ok && i < tiles; i++) {
+      if (ST > 1 && i + 1 < tiles) {
+        if (!(ok = prompt_wait_warp(&kfull[(i + 1) % ST], ((i + 1) / ST) & 1, abort))) break;
+        tc_fence_after();
+        scores(i + 1);
       }
-      for (int i = 0; ok && i < nt; i++) {
-        const int st = i % ST, st1 = (i + 1) % ST;
-        const bool more = i + 1 < nt;
-        if constexpr (NQ == 1) {  // the next tile's scores into the other buffer, before this one's weights are ready
-          if (more) {
-            if (!(ok = prompt_wait(&kfull[st1], ((i + 1) / ST) & 1, abort))) break;
-            tc_fence_after();
-            scores(0, i + 1, (i + 1) & 1);
-            umma_commit(&kempty[st1]);
-          }
-        }
-        for (int q = 0; q < NQ; q++) {
-          const int buf = NQ == 1 ? i & 1 : q;
-          if (!(ok = prompt_wait(&pfull[buf], NQ == 1 ? (i >> 1) & 1 : i & 1, abort))) break;
-          if (q == 0 && !(ok = prompt_wait(&vfull[st], (i / ST) & 1, abort))) break;
-          tc_fence_after();
-          outputs(q, i, buf);
-          if (q == NQ - 1) umma_commit(&vempty[st]);
-          if (NQ == 2 && more) {
-            if (q == 0) {
-              if (!(ok = prompt_wait(&kfull[st1], ((i + 1) / ST) & 1, abort))) break;
-              tc_fence_after();
-            }
-            scores(q, i + 1, q);
-            if (q == NQ - 1) umma_commit(&kempty[st1]);
-          }
-        }
+#pragma unroll
+      for (int q = 0; q < NQ; q++) {
+        if (!(ok = prompt_wait_warp(&pfull[2 * q + (i & 1)], (i >> 1) & 1, abort))) break;
+        if (q == 0 && !(ok = prompt_wait_warp(&vfull[i % ST], (i / ST) & 1, abort))) break;
+        tc_fence_after();
+        outputs(q, i);
       }
-      if (!ok) {  // everything issued so far has finished before TMEM is freed
-        umma_commit(drain);
-        for (int it = 0; it < 1000000 && !mbar_try_wait(drain, 0); ++it) {
-        }
+      if (!ok) break;
+      umma_commit_on(&done[i % ST], on);
+      if (ST == 1 && i + 1 < tiles) {  // one stage: the next K tile comes after this tile's products
+        if (!(ok = prompt_wait_warp(&kfull[0], (i + 1) & 1, abort))) break;
+        tc_fence_after();
+        scores(i + 1);
+      }
+    }
+    if (!ok) {  // everything issued so far has finished before TMEM is freed
+      umma_commit_on(drain, on);
+      for (int it = 0; it < 1000000 && !mbar_try_wait(drain, 0); ++it) {
       }
     }
   } else if (warp < S::SOFT_WARPS) {
@@ -395,113 +444,90 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     float r = KV8_NEG, l = 0.f;
     bool ok = true;
     for (int i = 0; i < nt; i++) {
-      const int buf = NQ == 1 ? i & 1 : q;
-      if (!(ok = prompt_wait_warp(&sfull[buf], NQ == 1 ? (i >> 1) & 1 : i & 1, abort))) break;
+      const int buf = 2 * q + (i & 1);
+      if (!(ok = prompt_wait_warp(&sfull[i & 1], (i >> 1) & 1, abort))) break;
       tc_fence_after();
       const uint32_t ts = tl + buf * S::TMEM_S;
-#pragma unroll 1
-      for (int half = 0; half < HALVES; half++) {
-        const int key0 = k00 + i * KT + half * 64;
-        const bool whole = key0 + 63 <= all_hi && key0 >= all_lo;
-        const float4* mt = meta + ((i * GT + half * 4) & (S::GROUPS - 1));
-        uint32_t v[2][32];
-        float top;
-        // x = t - r + 7 in place of the scores: weights are 2^x = 2^7 w
-        const auto exponents = [&](float from) {
-          tmem_ld32(ts + half * 64, v[0]);
-          tmem_ld32(ts + half * 64 + 32, v[1]);
-          tmem_ld_done();
-          top = KV8_NEG;
+      const int key0 = k00 + i * KT;
+      const bool whole = key0 + 63 <= all_hi && key0 >= all_lo;
+      const float4* mt = meta + ((i * GT) & (S::GROUPS - 1));
+      uint32_t v[2][32];
+      float top;
+      // x = t - r + 7 in place of the scores: weights are 2^x = 2^7 w
+      const auto exponents = [&](float from) {
+        tmem_ld32(ts, v[0]);
+        tmem_ld32(ts + 32, v[1]);
+        tmem_ld_done();
+        float tops[8];
 #pragma unroll
-          for (int g = 0; g < 4; g++) {
-            const float4 m = mt[g];
-            const float f = m.x * mul, c = m.y - from;
+        for (int g = 0; g < 4; g++) {
+          const float4 m = mt[g];
+          const float f = m.x * mul, c = m.y - from;
+          const uint64_t f2 = pack2(f, f), c2 = pack2(c, c);
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-              uint32_t& w = v[g >> 1][(g & 1) * 16 + e];
-              w = __float_as_uint(fmaf(__uint_as_float(w), f, c));
-            }
+          for (int e = 0; e < 16; e += 2) fma2(v[g >> 1][(g & 1) * 16 + e], v[g >> 1][(g & 1) * 16 + e + 1], f2, c2);
+        }
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 64; e++) {
+            const int key = key0 + e;
+            if (key > hi_key || key < lo_key) v[e >> 5][e & 31] = __float_as_uint(KV8_NEG);
           }
-          if (!whole) {
+        }
 #pragma unroll
-            for (int e = 0; e < 64; e++) {
-              const int key = key0 + e;
-              if (key > hi_key || key < lo_key) v[e >> 5][e & 31] = __float_as_uint(KV8_NEG);
-            }
-          }
+        for (int e = 0; e < 8; e++) tops[e] = KV8_NEG;
 #pragma unroll
-          for (int e = 0; e < 64; e++) top = fmaxf(top, __uint_as_float(v[e >> 5][e & 31]));
-        };
-        exponents(r - 7.f);
-        if (__any_sync(0xffffffffu, top > 7.f + KV8_SLACK)) {
-          const bool raise = top > 7.f + KV8_SLACK;
-          exponents(0.f);
-          const float nr = raise ? ceilf(top) : r;
-          const float f = ex2(r - nr);  // 0 for the first keys of a row, else a power of two
-          l *= f;
-          if (i > 0) {  // O is rescaled once the previous tile's product is in it
-            if (!(ok = prompt_wait_warp(&odone[q], (i - 1) & 1, abort))) break;
-            tc_fence_after();
-            for (int c = 0; c < a.hd; c += 32) {
-              tmem_ld32(to + c, v[0]);
-              tmem_ld_done();
-#pragma unroll
-              for (int e = 0; e < 32; e++) v[0][e] = __float_as_uint(__uint_as_float(v[0][e]) * f);
-              tmem_st32(to + c, v[0]);
-            }
-          }
-          if (half > 0) {  // and so are this tile's earlier weights
-            const __half2 f2 = __float2half2_rn(f);
-            tmem_ld32(ts, v[0]);
-            if constexpr (HILO) tmem_ld32(ts + 32, v[1]);
+        for (int e = 0; e < 64; e += 2) tops[(e >> 1) & 7] = max3(tops[(e >> 1) & 7], __uint_as_float(v[e >> 5][e & 31]), __uint_as_float(v[e >> 5][(e & 31) + 1]));
+        top = max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7]));
+      };
+      exponents(r - 7.f);
+      if (__any_sync(0xffffffffu, top > 7.f + KV8_SLACK)) {
+        const bool raise = top > 7.f + KV8_SLACK;
+        exponents(0.f);
+        const float nr = raise ? ceilf(top) : r;
+        const float f = ex2(r - nr);  // 0 for the first keys of a row, else a power of two
+        l *= f;
+        if (i > 0) {  // O is rescaled once the previous tile's product is in it
+          if (!(ok = prompt_wait_warp(&done[(i - 1) % ST], ((i - 1) / ST) & 1, abort))) break;
+          tc_fence_after();
+          for (int c = 0; c < a.hd; c += 32) {
+            tmem_ld32(to + c, v[0]);
             tmem_ld_done();
 #pragma unroll
-            for (int e = 0; e < 32; e++) {
-              __half2 y = __hmul2(*reinterpret_cast<__half2*>(&v[0][e]), f2);
-              v[0][e] = *reinterpret_cast<uint32_t*>(&y);
-              if constexpr (HILO) {
-                y = __hmul2(*reinterpret_cast<__half2*>(&v[1][e]), f2);
-                v[1][e] = *reinterpret_cast<uint32_t*>(&y);
-              }
-            }
-            tmem_st32(ts, v[0]);
-            if constexpr (HILO) tmem_st32(ts + 32, v[1]);
+            for (int e = 0; e < 32; e++) v[0][e] = __float_as_uint(__uint_as_float(v[0][e]) * f);
+            tmem_st32(to + c, v[0]);
           }
-          tmem_st_done();
-          r = nr;
-          exponents(r - 7.f);
         }
-#pragma unroll
-        for (int g2 = 0; g2 < 2; g2++) {  // 32 keys: 16 columns of weights (HILO: and 16 of what they leave)
-          uint32_t ph[16], pl[16];
-#pragma unroll
-          for (int g = 0; g < 2; g++) {
-            const float iv = mt[2 * g2 + g].z;
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-              const float w0 = ex2(__uint_as_float(v[g2][g * 16 + 2 * e])), w1 = ex2(__uint_as_float(v[g2][g * 16 + 2 * e + 1]));
-              sum += w0 + w1;
-              if constexpr (HILO) split_f16(w0, w1, ph[g * 8 + e], pl[g * 8 + e]);
-              else ph[g * 8 + e] = half2_bits(w0, w1);
-            }
-            l = fmaf(sum, iv, l);
-          }
-          tmem_st16(ts + half * 64 + g2 * 16, ph);
-          if constexpr (HILO) tmem_st16(ts + half * 64 + 32 + g2 * 16, pl);
-        }
+        tmem_st_done();
+        r = nr;
+        exponents(r - 7.f);
       }
-      if (!ok) break;
+#pragma unroll
+      for (int g2 = 0; g2 < 2; g2++) {  // 32 keys: 16 columns of weights (HILO: and 16 of what they leave)
+        uint32_t ph[16], pl[16];
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+          const float iv = mt[2 * g2 + g].z;
+          uint64_t sum = 0;  // (0, 0)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float w0 = ex2(__uint_as_float(v[g2][g * 16 + 2 * e])), w1 = ex2(__uint_as_float(v[g2][g * 16 + 2 * e + 1]));
+            add2(sum, w0, w1);
+            if constexpr (HILO) split_f16(w0, w1, ph[g * 8 + e], pl[g * 8 + e]);
+            else ph[g * 8 + e] = half2_bits(w0, w1);
+          }
+          l = fmaf(sum2(sum), iv, l);
+        }
+        tmem_st16(ts + g2 * 16, ph);
+        if constexpr (HILO) tmem_st16(ts + 32 + g2 * 16, pl);
+      }
       tmem_st_done();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&pfull[buf]);
     }
     if (ok && nt) {
-      // with one query tile the last scores were issued before the last but one product: a parity
-      // wait alone could take the phase before that for the last one
-      if (nt > 1) ok = prompt_wait_warp(&odone[q], (nt - 2) & 1, abort);
-      ok = ok && prompt_wait_warp(&odone[q], (nt - 1) & 1, abort);
+      ok = prompt_wait_warp(&done[(nt - 1) % ST], ((nt - 1) / ST) & 1, abort);
       tc_fence_after();
     }
     const long long ri = (long long)sq.row0 + tok, pi = (ri * heads + hq) * a.splits + split;
