@@ -20,28 +20,37 @@ namespace gg {
 
 // ------------------------------------------------------------------------------ few rows
 //
-// One CTA: one request, one key head, one tile of query rows (the `group` heads of a few tokens)
-// and one range of keys. Bound by the cache's bytes. Each of the four warps streams its own steps of 16 keys
-// through a private cp.async ring (no barriers between warps): 16 keys are one MMA's depth for
-// the second product and never cross a block. The warps' results meet in shared memory at the
-// end; ranges meet in gg_kv8_merge_kernel.
+// One CTA: one request, one key head, one tile of 8 NT query rows (the `group` heads of a few
+// tokens) and one range of keys. Bound by the cache's bytes. Each of the four warps streams its own
+// steps of 16 keys through a private cp.async ring (no barriers between warps): 16 keys are one
+// MMA's depth for the second product and never cross a block. The warps' results meet in shared
+// memory at the end; ranges meet in gg_kv8_merge_kernel.
 //
-// Fragments (lane = 4 g + t): key g of an 8-key tile reads dims 64 j + 16 t .. + 15 as one 16-byte
-// word, whose four 4-byte parts are the lane's operand values of four MMA depth steps; q is
-// laid out to match. For V the lane reads 16 dims of the four keys 2t, 2t+1, 2t+8, 2t+9: column g of
-// output tile (4 w + i) is dim 16 g + 4 w + i. The 16-byte words of a row sit at swizzled places
-// so that neither read has bank conflicts.
+// Both products are transposed, so that the few query rows are the narrow side (N = 8) of an
+// m16n8k16 MMA and the accumulators hold nothing else: S^T = K Q^T (16 keys x 8 rows), then
+// O^T += V^T P^T (16 dims x 8 rows) -- half the registers and, for f16 and bf16, half the MMAs of
+// rows padded to 16. f32 queries and weights take the hi and lo MMAs into the same accumulators.
+//
+// Fragments (lane = 4 g + t): keys g and g + 8 of a step are read 16 dims (one 16-byte word) at a time,
+// dims 64 j + 16 t .. + 15, whose four 4-byte parts are the operand values of four MMA depth steps;
+// q is laid out to match. Weights leave S^T as (key g, rows 2t, 2t + 1) and movmatrix turns them to
+// (row g, keys 2t, 2t + 1). For V the lane reads 16 dims of the keys 2t, 2t + 1, 2t + 8, 2t + 9: tile j of
+// O^T has dims 16 g + 2 j and 16 g + 2 j + 1 as its rows g and g + 8. The 16-byte words of a key sit at
+// swizzled places so that neither read has bank conflicts.
 constexpr int KV8_WARPS = 4;
 constexpr int KV8_STEP = 16;
 
-template <int HD>
+template <int HD, bool HILO, int NT>
 struct RowsShape {
-  static constexpr int STAGES = HD == 256 ? 3 : HD == 128 ? 6 : 8;
+  static constexpr int STAGES = HD == 256 ? 2 : HD == 128 ? 4 : 8;
   static constexpr int STAGE_BYTES = 2 * KV8_STEP * HD;
-  static constexpr int QF_BYTES = HD / 16 * 512;
+  static constexpr int QF_LANE = NT * (HILO ? 16 : 8);  // bytes of a lane's query operands in one depth step
+  static constexpr int QF_BYTES = HD / 16 * 32 * QF_LANE;
   static constexpr int RING_BYTES = KV8_WARPS * STAGES * STAGE_BYTES;
-  static constexpr int META_BYTES = KV8_WARPS * STAGES * 16;
-  static constexpr int SMEM = QF_BYTES + RING_BYTES + META_BYTES;
+  static constexpr int OST = HD + 4;                    // floats of a row of partial outputs
+  static constexpr int OUT_BYTES = KV8_WARPS * 8 * NT * OST * 4;
+  static constexpr int SMEM = QF_BYTES + RING_BYTES > OUT_BYTES ? QF_BYTES + RING_BYTES : OUT_BYTES;
+  static constexpr int CTAS = NT * HD >= 512 ? 2 : 3;   // resident per SM
 };
 
 template <int HD>
@@ -54,16 +63,20 @@ GG_DEV uint32_t vswz(int key, int c) {
   if constexpr (HD >= 128) return key * HD + ((c ^ (((key >> 1) & 3) << 1)) << 4);
   else return (key >> 1) * 128 + (((key ^ (key >> 1)) & 1) << 6) + ((c ^ (((key >> 2) & 1) << 1)) << 4);
 }
+GG_DEV uint32_t transpose8x8(uint32_t x) {  // of f16 pairs: (row g, columns 2t, 2t + 1) -> (column g, rows 2t, 2t + 1)
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
 
-template <int HD, int CODE, bool HILO>
-__global__ void __launch_bounds__(KV8_WARPS * 32, 2) gg_kv8_rows_kernel(const Kv8Args a) {
-  typedef RowsShape<HD> S;
-  constexpr int RT = HILO ? 8 : 16;  // query rows of a tile
-  constexpr int NR = HILO ? 1 : 2;   // rows of a lane
+template <int HD, int CODE, bool HILO, int NT>
+__global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS) gg_kv8_rows_kernel(const Kv8Args a) {
+  typedef RowsShape<HD, HILO, NT> S;
+  constexpr int RT = 8 * NT;
   extern __shared__ __align__(128) unsigned char kv8_smem[];
-  __shared__ float s_mul[16];
-  __shared__ float2 s_ml[KV8_WARPS][16];
-  __shared__ int s_pos[16];
+  __shared__ float s_mul[RT];
+  __shared__ float2 s_ml[KV8_WARPS][RT];
+  __shared__ int s_hi[RT];
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -73,6 +86,15 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) gg_kv8_rows_kernel(const Kv
   const int rt = x % a.row_tiles;
   x /= a.row_tiles;
   const int h = x % a.kv_heads, s = x / a.kv_heads;
+  const int32_t* table = a.table + (long long)s * a.table_stride;
+  // Without a window the range starts at a known key: the first block ids are fetched together with
+  // the lengths that say how many of them count.
+  int id_even = -1, id_odd = -1;  // block ids of an even and of an odd batch of 32 steps, one step per lane
+  const auto step_key = [&](int kmin, int first, int i) { return kmin + (first + i * KV8_WARPS) * KV8_STEP; };
+  if (!a.window) {
+    const int key = step_key(0, split * a.split_steps + warp, lane);
+    if (lane * KV8_WARPS < a.split_steps && key < a.max_len) id_even = table[key >> a.block_shift];
+  }
   const Kv8Seq sq = kv8_seq(a, s);
   const int items = sq.n * a.group, base = rt * RT;
   if (base >= items) return;
@@ -84,6 +106,46 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) gg_kv8_rows_kernel(const Kv
   const int kmin = a.window ? (int)max(0ll, pos_lo - a.window + 1) & ~(KV8_STEP - 1) : 0;
   const int steps = kmax > kmin ? (kmax - kmin + KV8_STEP - 1) / KV8_STEP : 0;
   const int st0 = min(split * a.split_steps, steps), st1 = min(st0 + a.split_steps, steps);
+  const int first = st0 + warp;
+  const int n = st1 > first ? (st1 - first + KV8_WARPS - 1) / KV8_WARPS : 0;
+
+  // ---- the warp's ring
+  unsigned char* ring = kv8_smem + S::QF_BYTES + warp * S::STAGES * S::STAGE_BYTES;
+  const uint32_t ring_u = smem_u32(ring);
+  const auto load_id = [&](int i) { return i < n ? table[step_key(kmin, first, i) >> a.block_shift] : -1; };
+  const auto load_scales = [&](int id) {
+    const bool in = id >= 0 && id < a.num_blocks;
+    const long long at = (long long)(in ? id : 0) * a.kv_heads + h;
+    return in ? make_float2(a.ks[at], a.vs[at]) : make_float2(0.f, 0.f);  // a scale of 0 marks a block the cache has not
+  };
+  if (a.window) id_even = load_id(lane);
+  if (n > 32) id_odd = load_id(32 + lane);
+  constexpr int W = HD / 16;  // 16-byte words of a key
+  const int k_lane = lane / W, w_lane = lane % W;  // (a warp copies 32 / W keys at a time)
+  const bool w_in = w_lane * 16 < a.hd;
+  const auto issue = [&](int i) {
+    if (i < n) {
+      const int id = __shfl_sync(0xffffffffu, (i >> 5) & 1 ? id_odd : id_even, i & 31);
+      const int key0 = step_key(kmin, first, i);
+      const bool ok = w_in && id >= 0 && id < a.num_blocks;
+      const long long at = (((long long)(ok ? id : 0) * a.kv_heads + h) << a.block_shift) + (key0 & ((1 << a.block_shift) - 1));
+      const int left = ok ? sq.len - key0 : 0;  // keys of this step that exist
+      const uint32_t dst = ring_u + (i % S::STAGES) * S::STAGE_BYTES;
+      const long long off = at * a.hd + w_lane * 16;
+#pragma unroll
+      for (int c = 0; c < KV8_STEP * W / 32; c++) {
+        const int k = k_lane + c * (32 / W);
+        const uint32_t bytes = k < left ? 16 : 0;
+        const long long src = k < left ? off + k * a.hd : 0;
+        cp_async16(dst + kswz<HD>(k, w_lane), a.kc + src, bytes);
+        cp_async16(dst + KV8_STEP * HD + vswz<HD>(k, w_lane), a.vc + src, bytes);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S::STAGES - 1; i++) issue(i);
+  float2 raw = load_scales(n ? id_even : -1);  // scales of the next batch of steps as the cache has them
 
   // ---- query rows -> f16 operand fragments
   unsigned char* qf = kv8_smem;
@@ -106,163 +168,154 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) gg_kv8_rows_kernel(const Kv
     const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
     if (lane == 0) {
       s_mul[row] = __uint_as_float((uint32_t)(ex - 14 + 127) << 23) * a.scale_log2;
-      s_pos[row] = live ? (int)min(sq.first_pos + it / a.group, (long long)sq.len - 1) : -1;
+      s_hi[row] = live ? (int)min(sq.first_pos + it / a.group, (long long)sq.len - 1) : -1;
     }
 #pragma unroll
     for (int p = 0; p < PER; p++) {
       const int d = 4 * (lane + 32 * p);
       if (d >= HD) break;
       const int ks = 4 * (d >> 6) + ((d >> 2) & 3), tt = (d >> 4) & 3;
-      uint32_t* f = reinterpret_cast<uint32_t*>(qf + ((ks * 32) + (row & 7) * 4 + tt) * 16);
+      uint32_t* f = reinterpret_cast<uint32_t*>(qf + ((ks * 32) + (row & 7) * 4 + tt) * S::QF_LANE) + (row >> 3) * (HILO ? 4 : 2);
       if constexpr (HILO) {
-        split_f16(v[p].x * up, v[p].y * up, f[0], f[1]);
-        split_f16(v[p].z * up, v[p].w * up, f[2], f[3]);
+        split_f16(v[p].x * up, v[p].y * up, f[0], f[2]);
+        split_f16(v[p].z * up, v[p].w * up, f[1], f[3]);
       } else {
-        f[row >> 3] = half2_bits(v[p].x * up, v[p].y * up);
-        f[2 + (row >> 3)] = half2_bits(v[p].z * up, v[p].w * up);
+        f[0] = half2_bits(v[p].x * up, v[p].y * up);
+        f[1] = half2_bits(v[p].z * up, v[p].w * up);
       }
     }
   }
   __syncthreads();
 
-  unsigned char* ring = kv8_smem + S::QF_BYTES + warp * S::STAGES * S::STAGE_BYTES;
-  const uint32_t ring_u = smem_u32(ring);
-  float4* meta = reinterpret_cast<float4*>(kv8_smem + S::QF_BYTES + S::RING_BYTES) + warp * S::STAGES;
-  const int first = st0 + warp;
-  const int n = st1 > first ? (st1 - first + KV8_WARPS - 1) / KV8_WARPS : 0;
-  const int32_t* table = a.table + (long long)s * a.table_stride;
-
-  float mul[NR], rmax[NR], lsum[NR];
-  int hi_key[NR], lo_key[NR];
+  // ---- the lane's rows 2t and 2t + 1 of each tile of eight
+  float mul[NT][2], rmax[NT][2], lsum[NT][2];
+  int hi_key[NT][2], lo_key[NT][2];
 #pragma unroll
-  for (int i = 0; i < NR; i++) {
-    mul[i] = s_mul[g + 8 * i];
-    hi_key[i] = s_pos[g + 8 * i];
-    // s_pos is cut at the last key: the window is measured from the row's own position
-    const int it = base + g + 8 * i;
-    lo_key[i] = a.window ? (int)max(0ll, sq.first_pos + it / a.group - a.window + 1) : 0;
-    rmax[i] = KV8_NEG;
-    lsum[i] = 0.f;
-  }
-  float o[HD / 8][4];
+  for (int u = 0; u < NT; u++)
 #pragma unroll
-  for (int i = 0; i < HD / 8; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) o[i][j] = 0.f;
-
-  // block ids and scales of 32 steps at a time, one step per lane
-  int b_id = -1;
-  float4 b_meta = make_float4(0.f, 0.f, 0.f, 0.f);
-  const auto issue = [&](int i) {
-    if (i < n) {
-      if ((i & 31) == 0) {
-        const int ii = i + lane;
-        b_id = -1;
-        b_meta = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (ii < n) {
-          const int key0 = kmin + (first + ii * KV8_WARPS) * KV8_STEP;
-          const int id = table[key0 >> a.block_shift];
-          if (id >= 0 && id < a.num_blocks) {
-            b_id = id;
-            const float vs = a.vs[(long long)id * a.kv_heads + h];
-            b_meta = make_float4(a.ks[(long long)id * a.kv_heads + h], log2f(vs), 1.f / vs, 1.f);
-          }
-        }
-      }
-      const int stage = i % S::STAGES;
-      if (lane == (i & 31)) meta[stage] = b_meta;
-      const int id = __shfl_sync(0xffffffffu, b_id, i & 31);
-      const int key0 = kmin + (first + i * KV8_WARPS) * KV8_STEP;
-      const long long at = (((long long)max(id, 0) * a.kv_heads + h) << a.block_shift) + (key0 & ((1 << a.block_shift) - 1));
-      const uint8_t* ksrc = a.kc + at * a.hd;
-      const uint8_t* vsrc = a.vc + at * a.hd;
-      const uint32_t dst = ring_u + stage * S::STAGE_BYTES;
-      constexpr int W = HD / 16;  // 16-byte words of a key
-#pragma unroll
-      for (int c = 0; c < KV8_STEP * W / 32; c++) {
-        const int k = (lane + 32 * c) / W, w = (lane + 32 * c) % W;
-        const bool in = id >= 0 && key0 + k < sq.len && w * 16 < a.hd;
-        const int off = in ? k * a.hd + w * 16 : 0;
-        cp_async16(dst + kswz<HD>(k, w), ksrc + off, in ? 16 : 0);
-        cp_async16(dst + KV8_STEP * HD + vswz<HD>(k, w), vsrc + off, in ? 16 : 0);
-      }
+    for (int e = 0; e < 2; e++) {
+      const int row = 8 * u + 2 * t + e;
+      mul[u][e] = s_mul[row];
+      hi_key[u][e] = s_hi[row];
+      lo_key[u][e] = a.window ? (int)max(0ll, sq.first_pos + (base + row) / a.group - a.window + 1) : 0;
+      rmax[u][e] = KV8_NEG;
+      lsum[u][e] = 0.f;
     }
-    cp_async_commit();
-  };
-  for (int i = 0; i < S::STAGES - 1; i++) issue(i);
-  const uint32_t qf_u = smem_u32(qf) + lane * 16;
+  constexpr int OT = HD / 16;
+  float o[NT][OT][4];
+#pragma unroll
+  for (int u = 0; u < NT; u++)
+#pragma unroll
+    for (int i = 0; i < OT; i++)
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[u][i][j] = 0.f;
+
+  float b_ks = 0.f, b_lv = 0.f, b_iv = 0.f;
+  const uint32_t qf_u = smem_u32(qf) + lane * S::QF_LANE;
   for (int i = 0; i < n; i++) {
+    if ((i & 31) == 0) {  // this batch's scales: log2 and reciprocal once per step, a lane each
+      b_ks = raw.x;
+      b_lv = log2f(raw.y);
+      b_iv = raw.y == 0.f ? 0.f : 1.f / raw.y;
+    }
     cp_async_wait<S::STAGES - 2>();
     __syncwarp();
     issue(i + S::STAGES - 1);
+    // the next batch: its ids once those of the batch before are used up, its scales a little later
+    if ((i & 31) == 16 && i >= 32 && i + 16 < n) {
+      const int id = load_id(i + 16 + lane);
+      if ((i >> 5) & 1) id_even = id;
+      else id_odd = id;
+    }
+    if ((i & 31) == 24) raw = load_scales(i + 8 + lane < n ? ((i >> 5) & 1 ? id_even : id_odd) : -1);
     const uint32_t kst = ring_u + (i % S::STAGES) * S::STAGE_BYTES, vst = kst + KV8_STEP * HD;
-    const float4 mt = meta[i % S::STAGES];
-    const int key0 = kmin + (first + i * KV8_WARPS) * KV8_STEP;
-    // scores: two 8-key tiles, two accumulators each to shorten the chains
-    float c[2][2][4] = {};
+    const float ks = __shfl_sync(0xffffffffu, b_ks, i & 31), lv = __shfl_sync(0xffffffffu, b_lv, i & 31), iv = __shfl_sync(0xffffffffu, b_iv, i & 31);
+    const int key0 = step_key(kmin, first, i);
+    // scores, in two accumulators (hi and lo, or odd and even depth steps) to shorten the chains
+    float c[NT][2][4] = {};
 #pragma unroll
     for (int j = 0; j < HD / 64; j++) {
       const uint4 k0 = lds128(kst + kswz<HD>(g, 4 * j + t)), k1 = lds128(kst + kswz<HD>(g + 8, 4 * j + t));
       const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
       for (int p = 0; p < 4; p++) {
-        const uint4 qa = lds128(qf_u + (4 * j + p) * 512);
-        uint32_t b0, b1;
-        widen4<CODE>(w0[p], b0, b1);
-        mma_f16(c[0][p & 1], qa, b0, b1);
-        widen4<CODE>(w1[p], b0, b1);
-        mma_f16(c[1][p & 1], qa, b0, b1);
-      }
-    }
-    // softmax weights of the lane's rows at keys key0 + 8 tile + 2t, + 1
-    float wt[NR][4];
+        uint4 ka;
+        widen4<CODE>(w0[p], ka.x, ka.z);
+        widen4<CODE>(w1[p], ka.y, ka.w);
+        const uint32_t qa = qf_u + (4 * j + p) * 32 * S::QF_LANE;
 #pragma unroll
-    for (int r = 0; r < NR; r++) {
-      float sc[4], top = KV8_NEG;
-      bool seen[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int ti = e >> 1, el = e & 1, key = key0 + 8 * ti + 2 * t + el;
-        float v = c[ti][0][2 * r + el] + c[ti][1][2 * r + el];
-        if constexpr (HILO) v += c[ti][0][2 + el] + c[ti][1][2 + el];
-        seen[e] = key <= hi_key[r] && key >= lo_key[r] && mt.w != 0.f;
-        sc[e] = seen[e] ? fmaf(v * mt.x, mul[r], mt.y) : KV8_NEG;
-        top = fmaxf(top, sc[e]);
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (__any_sync(0xffffffffu, top > rmax[r] + KV8_SLACK)) {
-        const float nr = top > rmax[r] + KV8_SLACK ? top : rmax[r];
-        const float f = ex2(rmax[r] - nr);  // rmax = KV8_NEG: 2^-huge = 0
-        rmax[r] = nr;
-        lsum[r] *= f;
-#pragma unroll
-        for (int d = 0; d < HD / 8; d++) {
-          o[d][2 * r] *= f;
-          o[d][2 * r + 1] *= f;
+        for (int u = 0; u < NT; u++) {
           if constexpr (HILO) {
-            o[d][2] *= f;
-            o[d][3] *= f;
+            const uint4 q = lds128(qa + 16 * u);
+            mma_f16(c[u][0], ka, q.x, q.y);
+            mma_f16(c[u][1], ka, q.z, q.w);
+          } else {
+            const uint2 q = lds64(qa + 8 * u);
+            mma_f16(c[u][p & 1], ka, q.x, q.y);
           }
         }
       }
+    }
+    // weights of rows 2t, 2t + 1 at keys key0 + g and key0 + g + 8
+    uint32_t pb[NT][HILO ? 4 : 2];
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        wt[r][e] = seen[e] ? ex2(sc[e] - rmax[r]) : 0.f;
-        lsum[r] += seen[e] ? wt[r][e] * mt.z : 0.f;
-        wt[r][e] *= KV8_WMUL;
+    for (int u = 0; u < NT; u++) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float sc[2], top = KV8_NEG;
+        bool seen[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const int key = key0 + g + 8 * k;
+          seen[k] = key <= hi_key[u][e] && key >= lo_key[u][e] && iv != 0.f;
+          sc[k] = seen[k] ? fmaf((c[u][0][2 * k + e] + c[u][1][2 * k + e]) * ks, mul[u][e], lv) : KV8_NEG;
+          top = fmaxf(top, sc[k]);
+        }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (__any_sync(0xffffffffu, top > rmax[u][e] + KV8_SLACK)) {
+          const float nr = top > rmax[u][e] + KV8_SLACK ? top : rmax[u][e];
+          const float f = ex2(rmax[u][e] - nr);  // rmax = KV8_NEG: 2^-huge = 0
+          rmax[u][e] = nr;
+          lsum[u][e] *= f;
+#pragma unroll
+          for (int d = 0; d < OT; d++) {
+            o[u][d][e] *= f;
+            o[u][d][2 + e] *= f;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const float y = seen[k] ? ex2(sc[k] - rmax[u][e]) : 0.f;
+          if (seen[k]) lsum[u][e] = fmaf(y, iv, lsum[u][e]);
+          w[2 * k + e] = y * KV8_WMUL;
+        }
+      }
+      if constexpr (HILO) {
+        uint32_t hi0, lo0, hi1, lo1;
+        split_f16(w[0], w[1], hi0, lo0);
+        split_f16(w[2], w[3], hi1, lo1);
+        pb[u][0] = transpose8x8(hi0);
+        pb[u][1] = transpose8x8(hi1);
+        pb[u][2] = transpose8x8(lo0);
+        pb[u][3] = transpose8x8(lo1);
+      } else {
+        pb[u][0] = transpose8x8(half2_bits(w[0], w[1]));
+        pb[u][1] = transpose8x8(half2_bits(w[2], w[3]));
       }
     }
-    uint4 pa;
-    if constexpr (HILO) {
-      split_f16(wt[0][0], wt[0][1], pa.x, pa.y);
-      split_f16(wt[0][2], wt[0][3], pa.z, pa.w);
-    } else {
-      pa.x = half2_bits(wt[0][0], wt[0][1]);
-      pa.y = half2_bits(wt[NR - 1][0], wt[NR - 1][1]);
-      pa.z = half2_bits(wt[0][2], wt[0][3]);
-      pa.w = half2_bits(wt[NR - 1][2], wt[NR - 1][3]);
-    }
+    const auto product = [&](int tile, const uint32_t (&lo)[4], const uint32_t (&hi)[4]) {  // dims tile * 2 .. of keys 2t, 2t + 1 and 2t + 8, 2t + 9
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        const uint4 va = make_uint4(lo[2 * y], lo[2 * y + 1], hi[2 * y], hi[2 * y + 1]);
+#pragma unroll
+        for (int u = 0; u < NT; u++) {
+          mma_f16(o[u][tile + y], va, pb[u][0], pb[u][1]);
+          if constexpr (HILO) mma_f16(o[u][tile + y], va, pb[u][2], pb[u][3]);
+        }
+      }
+    };
     if constexpr (HD >= 128) {
 #pragma unroll
       for (int jj = 0; jj < HD / 128; jj++) {
@@ -275,8 +328,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) gg_kv8_rows_kernel(const Kv
           uint32_t b0[4], b1[4];
           widen4_pairs<CODE>(x0[w], x1[w], b0);
           widen4_pairs<CODE>(x2[w], x3[w], b1);
-#pragma unroll
-          for (int e = 0; e < 4; e++) mma_f16(o[16 * jj + 4 * w + e], pa, b0[e], b1[e]);
+          product(8 * jj + 2 * w, b0, b1);
         }
       }
     } else {  // HD = 64: 8 dims of the four keys per lane
@@ -289,36 +341,32 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) gg_kv8_rows_kernel(const Kv
         uint32_t b0[4], b1[4];
         widen4_pairs<CODE>(x0[w], x1[w], b0);
         widen4_pairs<CODE>(x2[w], x3[w], b1);
-#pragma unroll
-        for (int e = 0; e < 4; e++) mma_f16(o[4 * w + e], pa, b0[e], b1[e]);
+        product(2 * w, b0, b1);
       }
     }
   }
   cp_async_wait<0>();
 #pragma unroll
-  for (int r = 0; r < NR; r++) {
-    lsum[r] += __shfl_xor_sync(0xffffffffu, lsum[r], 1);
-    lsum[r] += __shfl_xor_sync(0xffffffffu, lsum[r], 2);
-    if (t == 0) s_ml[warp][g + 8 * r] = make_float2(rmax[r], lsum[r]);
-  }
-  __syncthreads();  // every warp has left its ring: it becomes [warp][row][HD + 4] f32
-  constexpr int OST = HD + 4;
-  static_assert(KV8_WARPS * RT * OST * 4 <= S::QF_BYTES + S::RING_BYTES, "partial outputs fit the ring");
+  for (int u = 0; u < NT; u++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+#pragma unroll
+      for (int d = 4; d < 32; d <<= 1) lsum[u][e] += __shfl_xor_sync(0xffffffffu, lsum[u][e], d);
+      if (g == 0) s_ml[warp][8 * u + 2 * t + e] = make_float2(rmax[u][e], lsum[u][e]);
+    }
+  __syncthreads();  // every warp has left its ring: it becomes [warp][row][OST] f32
   float* so = reinterpret_cast<float*>(kv8_smem);
+  constexpr int PD = HD >= 128 ? 16 : 8;  // dims that a lane holds next to each other
 #pragma unroll
-  for (int r = 0; r < NR; r++) {
-    float* dst = so + (warp * RT + g + 8 * r) * OST;
+  for (int u = 0; u < NT; u++)
 #pragma unroll
-    for (int i = 0; i < HD / 8; i++)
+    for (int e = 0; e < 2; e++) {
+      if (8 * u + 2 * t + e >= nitems) continue;
+      float* dst = so + (warp * RT + 8 * u + 2 * t + e) * S::OST + PD * g;
 #pragma unroll
-      for (int el = 0; el < 2; el++) {
-        float v = o[i][2 * r + el];
-        if constexpr (HILO) v += o[i][2 + el];
-        const int col = 2 * t + el;
-        const int d = HD >= 128 ? 128 * (i >> 4) + 16 * col + (i & 15) : 8 * col + i;
-        dst[d] = v;
-      }
-  }
+      for (int i = 0; i < OT; i += 2)
+        *reinterpret_cast<float4*>(dst + (i * 2 / PD) * 128 + (i * 2) % PD) = make_float4(o[u][i][e], o[u][i][2 + e], o[u][i + 1][e], o[u][i + 1][2 + e]);
+    }
   __syncthreads();
   for (int row = warp; row < nitems; row += KV8_WARPS) {
     const int it = base + row, tok = it / a.group, hq = h * a.group + it % a.group;
@@ -333,13 +381,19 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) gg_kv8_rows_kernel(const Kv
     const long long ri = (long long)(sq.row0 + tok);
     const long long pi = (ri * heads + hq) * a.splits + split;
     const float inv = a.splits == 1 ? (l == 0.f ? 0.f : (1.f / KV8_WMUL) / l) : 1.f / KV8_WMUL;
-    for (int d = lane; d < a.hd; d += 32) {
-      float v = 0.f;
+    for (int d = 4 * lane; d < a.hd; d += 128) {
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < KV8_WARPS; w++) v += f[w] * so[(w * RT + row) * OST + d];
-      v *= inv;
-      if (a.splits == 1) store_elem(a.out, a.q_type, ri * a.o_row + (long long)hq * a.o_head + d, v);
-      else a.part_o[pi * a.hd + d] = v;
+      for (int w = 0; w < KV8_WARPS; w++) {
+        const float4 y = *reinterpret_cast<const float4*>(so + (w * RT + row) * S::OST + d);
+        v.x = fmaf(f[w], y.x, v.x);
+        v.y = fmaf(f[w], y.y, v.y);
+        v.z = fmaf(f[w], y.z, v.z);
+        v.w = fmaf(f[w], y.w, v.w);
+      }
+      v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+      if (a.splits == 1) store_elem4(a.out, a.q_type, ri * a.o_row + (long long)hq * a.o_head + d, v, a.o_vec);
+      else *reinterpret_cast<float4*>(a.part_o + pi * a.hd + d) = v;
     }
     if (lane == 0) {
       if (a.splits > 1) a.part_ml[pi] = make_float2(r, l);
@@ -348,47 +402,88 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, 2) gg_kv8_rows_kernel(const Kv
   }
 }
 
-// One warp per (request, token, query head): the results of the key ranges joined.
-__global__ void __launch_bounds__(128) gg_kv8_merge_kernel(const Kv8Args a) {
+// One CTA per (request, token, query head): the results of the key ranges joined. Bound by latency
+// (a few KB per CTA), so the ranges are spread over the threads: `lanes` threads hold four dims each
+// and MERGE_THREADS / lanes of them share the ranges; every thread has its loads in flight at once.
+constexpr int MERGE_THREADS = 256;
+__global__ void __launch_bounds__(MERGE_THREADS) gg_kv8_merge_kernel(const Kv8Args a) {
+  __shared__ float4 s_o[MERGE_THREADS];
+  __shared__ float s_l[MERGE_THREADS / 32], s_r[MERGE_THREADS / 32];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
+  const int t = threadIdx.x;
   const int heads = a.kv_heads * a.group;
-  long long x = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int hq = (int)(x % heads);
+  int x = blockIdx.x;
+  const int hq = x % heads;
   x /= heads;
-  const int tok = (int)(x % a.merge_tokens);
+  const int tok = x % a.merge_tokens;
   x /= a.merge_tokens;
-  if (x >= a.seqs) return;
-  const Kv8Seq sq = kv8_seq(a, (int)x);
+  const Kv8Seq sq = kv8_seq(a, x);
   if (tok >= sq.n) return;
   const long long ri = sq.row0 + tok, pi = (ri * heads + hq) * a.splits;
-  float r = KV8_NEG, l = 0.f;
-  for (int z = lane; z < a.splits; z += 32) r = fmaxf(r, a.part_ml[pi + z].x);
+  float r = KV8_NEG;
+  for (int z = t; z < a.splits; z += MERGE_THREADS) r = fmaxf(r, a.part_ml[pi + z].x);
+  const int lanes = a.hd <= 64 ? 16 : a.hd <= 128 ? 32 : 64, parts = MERGE_THREADS / lanes;
+  const int d = 4 * (t % lanes), z0 = t / lanes;
   r = warp_max(r);
-  for (int z = lane; z < a.splits; z += 32) l += ex2(a.part_ml[pi + z].x - r) * a.part_ml[pi + z].y;
-  l = warp_sum(l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  for (int d = lane; d < a.hd; d += 32) {
-    float v = 0.f;
-    for (int z = 0; z < a.splits; z++) v += ex2(a.part_ml[pi + z].x - r) * a.part_o[(pi + z) * a.hd + d];
-    store_elem(a.out, a.q_type, ri * a.o_row + (long long)hq * a.o_head + d, v * inv);
+  if ((t & 31) == 0) s_r[t >> 5] = r;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < MERGE_THREADS / 32; w++) r = fmaxf(r, s_r[w]);
+  float l = 0.f;
+  for (int z = t; z < a.splits; z += MERGE_THREADS) {
+    const float2 ml = a.part_ml[pi + z];
+    l = fmaf(ex2(ml.x - r), ml.y, l);
   }
-  if (lane == 0 && a.lse) a.lse[ri * heads + hq] = l == 0.f ? -INFINITY : (r + log2f(l)) * 0.6931471805599453f;
+  l = warp_sum(l);
+  if ((t & 31) == 0) s_l[t >> 5] = l;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (d < a.hd)
+#pragma unroll 4
+    for (int z = z0; z < a.splits; z += parts) {
+      const float f = ex2(a.part_ml[pi + z].x - r);
+      const float4 y = *reinterpret_cast<const float4*>(a.part_o + (pi + z) * a.hd + d);
+      v.x = fmaf(f, y.x, v.x);
+      v.y = fmaf(f, y.y, v.y);
+      v.z = fmaf(f, y.z, v.z);
+      v.w = fmaf(f, y.w, v.w);
+    }
+  s_o[t] = v;
+  __syncthreads();
+  if (t >= lanes || d >= a.hd) return;
+  l = 0.f;
+#pragma unroll
+  for (int w = 0; w < MERGE_THREADS / 32; w++) l += s_l[w];
+  for (int p = 1; p < parts; p++) {
+    const float4 y = s_o[t + p * lanes];
+    v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  store_elem4(a.out, a.q_type, ri * a.o_row + (long long)hq * a.o_head + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), a.o_vec);
+  if (t == 0 && a.lse) a.lse[ri * heads + hq] = l == 0.f ? -INFINITY : (r + log2f(l)) * 0.6931471805599453f;
 }
 
-template <int HD, int CODE, bool HILO>
+template <int HD, int CODE, bool HILO, int NT>
 cudaError_t launch_rows(const Kv8Args& a, cudaStream_t s) {
-  auto* k = gg_kv8_rows_kernel<HD, CODE, HILO>;
   const long long grid = (long long)a.seqs * a.kv_heads * a.row_tiles * a.splits;
-  return launch_big_smem(k, dim3((unsigned)grid), dim3(KV8_WARPS * 32), RowsShape<HD>::SMEM, s, a);
+  return launch_big_smem(gg_kv8_rows_kernel<HD, CODE, HILO, NT>, dim3((unsigned)grid), dim3(KV8_WARPS * 32), RowsShape<HD, HILO, NT>::SMEM, s, a);
+}
+template <int HD, int CODE, bool HILO>
+cudaError_t launch_rows_nt(const Kv8Args& a, int nt, cudaStream_t s) {
+  if (nt == 1) return launch_rows<HD, CODE, HILO, 1>(a, s);
+  if constexpr (HD <= 128)
+    if (nt == 4) return launch_rows<HD, CODE, HILO, 4>(a, s);
+  return launch_rows<HD, CODE, HILO, 2>(a, s);
 }
 template <int HD>
-cudaError_t launch_rows_hd(const Kv8Args& a, int code, cudaStream_t s) {
+cudaError_t launch_rows_hd(const Kv8Args& a, int code, int nt, cudaStream_t s) {
   const bool hilo = a.q_type == GG_T_F32;
-  if (code == GG_KV8_INT8) return hilo ? launch_rows<HD, GG_KV8_INT8, true>(a, s) : launch_rows<HD, GG_KV8_INT8, false>(a, s);
-  return hilo ? launch_rows<HD, GG_KV8_E4M3, true>(a, s) : launch_rows<HD, GG_KV8_E4M3, false>(a, s);
+  if (code == GG_KV8_INT8) return hilo ? launch_rows_nt<HD, GG_KV8_INT8, true>(a, nt, s) : launch_rows_nt<HD, GG_KV8_INT8, false>(a, nt, s);
+  return hilo ? launch_rows_nt<HD, GG_KV8_E4M3, true>(a, nt, s) : launch_rows_nt<HD, GG_KV8_E4M3, false>(a, nt, s);
 }
+// Tiles of eight query rows of a CTA: as many as the call's requests can fill, within the registers
+// (a tile more costs 2 head_dim / 16 MMAs a step, a CTA more reads the keys once more).
+static int kv8_row_tiles(long long items, int head_dim) { return items <= 8 ? 1 : items <= 16 || head_dim > 128 ? 2 : 4; }
 
 // How a call is cut. Requests with few rows (rows * group up to KV8_FEW) take the kernel above, the
 // others the one of gg_kv8_prompt.cu; a call that may hold both launches both, and each skips the
@@ -421,15 +516,18 @@ static Kv8Cut kv8_cut(long long items, int tile, long long slots, int least_step
 }
 struct Kv8Plan {
   Kv8Cut few, many;
+  int nt;  // tiles of eight rows of a CTA of the first
   size_t few_bytes, bytes;
 };
 static Kv8Plan kv8_plan(const gg_kv8_cache& c, const gg_kv8_attention_call& b) {
   Kv8Plan p;
   const int group = b.q.heads / c.kv_heads;
   const long long items = (long long)b.max_rows * group;
-  // few rows: two CTAs fit an SM; four waves of them even out requests of different lengths; at
-  // least two steps for each warp. Many rows: one CTA an SM, at least 512 keys.
-  p.few = kv8_cut(items < KV8_FEW ? items : KV8_FEW, b.q.type == GG_T_F32 ? 8 : 16, 148 * 2 * 4, 2 * KV8_WARPS, b.rows, b.q.heads, c, b);
+  // few rows: three CTAs fit an SM, three waves of them even out requests of different lengths; a
+  // step at least for each warp. Many rows: one CTA an SM, at least 512 keys.
+  const long long few = items < KV8_FEW ? items : KV8_FEW;
+  p.nt = kv8_row_tiles(few, c.head_dim);
+  p.few = kv8_cut(few, 8 * p.nt, 148 * 3 * 3, KV8_WARPS, b.rows, b.q.heads, c, b);
   if (items > KV8_FEW) p.many = kv8_cut(items, kv8_prompt_tile(c.head_dim), 148, 32, b.rows, b.q.heads, c, b);
   const auto bytes = [&](const Kv8Cut& k) { return k.parts * c.head_dim * 4 + k.parts * 8; };
   p.few_bytes = bytes(p.few);
@@ -524,13 +622,13 @@ extern "C" int gg_kv8_attention(const gg_kv8_cache* c, const gg_kv8_attention_ca
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(b.workspace) + (many ? p.few_bytes : 0));
     a.part_ml = reinterpret_cast<float2*>(a.part_o + k.parts * c->head_dim);
     r = many ? kv8_launch_prompt(a, c->code, s)
-        : c->head_dim <= 64 ? launch_rows_hd<64>(a, c->code, s)
-        : c->head_dim <= 128 ? launch_rows_hd<128>(a, c->code, s)
-                             : launch_rows_hd<256>(a, c->code, s);
+        : c->head_dim <= 64 ? launch_rows_hd<64>(a, c->code, p.nt, s)
+        : c->head_dim <= 128 ? launch_rows_hd<128>(a, c->code, p.nt, s)
+                             : launch_rows_hd<256>(a, c->code, p.nt, s);
     if (r == cudaSuccess && k.splits > 1) {
-      const long long tokens = many ? b.max_rows : (k.row_tiles * (long long)(b.q.type == GG_T_F32 ? 8 : 16) + a.group - 1) / a.group;
+      const long long tokens = many ? b.max_rows : (KV8_FEW + a.group - 1) / a.group;
       a.merge_tokens = (int)(tokens < b.max_rows ? tokens : b.max_rows);
-      r = launch_pdl(gg_kv8_merge_kernel, dim3((unsigned)(((long long)b.seqs * a.merge_tokens * b.q.heads + 3) / 4)), dim3(128), 0, s, a);
+      r = launch_pdl(gg_kv8_merge_kernel, dim3((unsigned)((long long)b.seqs * a.merge_tokens * b.q.heads)), dim3(MERGE_THREADS), 0, s, a);
     }
   }
   if (r != cudaSuccess) return ops_fail(GG_E_CUDA, "%s: launch: %s", fn, cudaGetErrorString(r));

@@ -121,6 +121,22 @@ GG_DEV float4 load_elem4(const void* p, int type, long long i, int vec) {
   return make_float4(a.x, a.y, b.x, b.y);
 }
 
+GG_DEV void store_elem4(void* p, int type, long long i, const float4& v, int vec) {
+  if (!vec) {
+    store_elem(p, type, i, v.x);
+    store_elem(p, type, i + 1, v.y);
+    store_elem(p, type, i + 2, v.z);
+    store_elem(p, type, i + 3, v.w);
+  } else if (type == GG_T_F32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(p) + i) = v;
+  } else {
+    const __nv_bfloat162 b0 = __floats2bfloat162_rn(v.x, v.y), b1 = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i) =
+        type == GG_T_BF16 ? make_uint2(*reinterpret_cast<const uint32_t*>(&b0), *reinterpret_cast<const uint32_t*>(&b1))
+                          : make_uint2(half2_bits(v.x, v.y), half2_bits(v.z, v.w));
+  }
+}
+
 // The rows of request s: first row, number of rows (within the batch and max_rows), length.
 struct Kv8Seq {
   int row0, n, len;
