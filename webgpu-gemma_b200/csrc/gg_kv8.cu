@@ -20,11 +20,14 @@ namespace gg {
 
 // ------------------------------------------------------------------------------ few rows
 //
-// One CTA: one request, one key head, one tile of 8 NT query rows (the `group` heads of a few
-// tokens) and one range of keys. Bound by the cache's bytes. Each of the four warps streams its own
-// steps of 16 keys through a private cp.async ring (no barriers between warps): 16 keys are one
-// MMA's depth for the second product and never cross a block. The warps' results meet in shared
-// memory at the end; ranges meet in gg_kv8_merge_kernel.
+// A unit is one request, one key head and one tile of 8 NT query rows (the `group` heads of a few
+// tokens); its keys are steps of 16 (one MMA's depth for the second product, never across a block).
+// The steps of all units stand in one line that is cut into equal chunks, one for each resident CTA:
+// requests of any lengths then load the SMs alike, in one wave, whatever the host knows of them.
+// Bound by the cache's bytes. Each of the four warps streams its own steps through a private
+// cp.async ring (no barriers between warps); the warps' results meet in shared memory at the end
+// of a unit. A unit inside one chunk is finished there, parts of the others meet in
+// gg_kv8_merge_kernel.
 //
 // Both products are transposed, so that the few query rows are the narrow side (N = 8) of an
 // m16n8k16 MMA and the accumulators hold nothing else: S^T = K Q^T (16 keys x 8 rows), then
@@ -69,64 +72,138 @@ GG_DEV uint32_t transpose8x8(uint32_t x) {  // of f16 pairs: (row g, columns 2t,
   return d;
 }
 
+// Units of a request and steps of each (the same for its tiles), for requests with rows.
+struct Kv8Line {
+  int tiles, steps, kmin;
+};
+GG_DEV Kv8Line kv8_line(const Kv8Args& a, const Kv8Seq& q, int RT) {
+  Kv8Line n = {0, 1, 0};
+  const int items = q.n * a.group;
+  n.tiles = (items + RT - 1) / RT;
+  n.kmin = a.window ? (int)min(max(0ll, q.first_pos - a.window + 1), (long long)q.len) & ~(KV8_STEP - 1) : 0;
+  n.steps = max(1, (q.len - n.kmin + KV8_STEP - 1) / KV8_STEP);  // a request without keys has one step that sees nothing
+  return n;
+}
+// Steps of a chunk for `total` steps over `ctas` CTAs: at least one for each warp.
+GG_DEV long long kv8_chunk(long long total, int ctas) {
+  const long long c = (total + ctas - 1) / ctas;
+  return max(c + KV8_WARPS - 1, (long long)KV8_WARPS) / KV8_WARPS * KV8_WARPS;
+}
+
 template <int HD, int CODE, bool HILO, int NT>
 __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS) gg_kv8_rows_kernel(const Kv8Args a) {
   typedef RowsShape<HD, HILO, NT> S;
-  constexpr int RT = 8 * NT;
+  constexpr int RT = 8 * NT, PER = 4, THREADS = KV8_WARPS * 32;
   extern __shared__ __align__(128) unsigned char kv8_smem[];
   __shared__ float s_mul[RT];
   __shared__ float2 s_ml[KV8_WARPS][RT];
   __shared__ int s_hi[RT];
+  __shared__ long long s_sum[KV8_WARPS], s_off;
+  __shared__ int s_seq;
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  int x = blockIdx.x;
-  const int split = x % a.splits;
-  x /= a.splits;
-  const int rt = x % a.row_tiles;
-  x /= a.row_tiles;
-  const int h = x % a.kv_heads, s = x / a.kv_heads;
-  const int32_t* table = a.table + (long long)s * a.table_stride;
-  // Without a window the range starts at a known key: the first block ids are fetched together with
-  // the lengths that say how many of them count.
-  int id_even = -1, id_odd = -1;  // block ids of an even and of an odd batch of 32 steps, one step per lane
-  const auto step_key = [&](int kmin, int first, int i) { return kmin + (first + i * KV8_WARPS) * KV8_STEP; };
-  if (!a.window) {
-    const int key = step_key(0, split * a.split_steps + warp, lane);
-    if (lane * KV8_WARPS < a.split_steps && key < a.max_len) id_even = table[key >> a.block_shift];
+  // ---- this CTA's chunk of the line: prefix sums of the requests' steps, THREADS * PER at a time
+  const auto steps_of = [&](int i) {
+    if (i >= a.seqs) return 0ll;
+    const Kv8Line n = kv8_line(a, kv8_seq(a, i), RT);
+    return (long long)n.tiles * n.steps * a.kv_heads;
+  };
+  long long v[PER], total = 0;
+  const bool once = a.seqs <= THREADS * PER;
+  for (int i0 = 0; i0 < a.seqs; i0 += THREADS * PER) {
+    long long sum = 0;
+#pragma unroll
+    for (int k = 0; k < PER; k++) sum += v[k] = steps_of(i0 + tid * PER + k);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    total += sum;
   }
-  const Kv8Seq sq = kv8_seq(a, s);
-  const int items = sq.n * a.group, base = rt * RT;
-  if (base >= items) return;
-  const int nitems = min(RT, items - base);
+  if (lane == 0) s_sum[warp] = total;
+  if (tid == 0) s_seq = -1;
+  __syncthreads();
+  total = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+  const long long chunk = kv8_chunk(total, gridDim.x), line0 = blockIdx.x * chunk;
+  const long long line1 = min(line0 + chunk, total);
+  if (blockIdx.x == 0 && tid == 0 && a.pre) a.pre[a.seqs] = total;
+  if (line0 >= total && (blockIdx.x || !a.pre)) return;
+  {
+    long long run = 0;
+    for (int i0 = 0; i0 < a.seqs; i0 += THREADS * PER) {
+      __syncthreads();
+      long long sum = 0;
+#pragma unroll
+      for (int k = 0; k < PER; k++) {
+        if (!once) v[k] = steps_of(i0 + tid * PER + k);
+        sum += v[k];
+      }
+      long long inc = sum;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += u;
+      }
+      if (lane == 31) s_sum[warp] = inc;
+      __syncthreads();
+      long long before = run + inc - sum;
+      for (int w = 0; w < warp; w++) before += s_sum[w];
+#pragma unroll
+      for (int k = 0; k < PER; k++) {
+        const int i = i0 + tid * PER + k;
+        if (blockIdx.x == 0 && a.pre && i < a.seqs) a.pre[i] = before;
+        if (before <= line0 && line0 < before + v[k]) {
+          s_seq = i;
+          s_off = line0 - before;
+        }
+        before += v[k];
+      }
+      run += s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+      if (run > line0 && (blockIdx.x || !a.pre)) break;
+    }
+    __syncthreads();
+  }
+  if (line0 >= line1) return;
+  int s = s_seq;
+  long long off = s_off;
   const int heads = a.kv_heads * a.group;
-  // keys that any row of the tile sees
-  const long long pos_lo = sq.first_pos + base / a.group, pos_hi = sq.first_pos + (base + nitems - 1) / a.group;
-  const int kmax = (int)min((long long)sq.len, pos_hi + 1);
-  const int kmin = a.window ? (int)max(0ll, pos_lo - a.window + 1) & ~(KV8_STEP - 1) : 0;
-  const int steps = kmax > kmin ? (kmax - kmin + KV8_STEP - 1) / KV8_STEP : 0;
-  const int st0 = min(split * a.split_steps, steps), st1 = min(st0 + a.split_steps, steps);
+  for (long long line = line0; line < line1;) {
+  const Kv8Seq sq = kv8_seq(a, s);
+  const Kv8Line ln = kv8_line(a, sq, RT);
+  if (off >= (long long)ln.tiles * ln.steps * a.kv_heads) {  // the request's units are done, or it has none
+    s++;
+    off = 0;
+    continue;
+  }
+  const int unit = (int)(off / ln.steps), st0 = (int)(off % ln.steps);
+  const int st1 = (int)min((long long)ln.steps, st0 + (line1 - line));
+  const int h = unit / ln.tiles, base = (unit % ln.tiles) * RT;
+  const bool whole = st0 == 0 && st1 == ln.steps;
+  const long long part = 2ll * blockIdx.x + (line > line0);  // a chunk has at most two units that it shares
+  off += st1 - st0;
+  line += st1 - st0;
+  const int32_t* table = a.table + (long long)s * a.table_stride;
+  const int nitems = min(RT, sq.n * a.group - base), kmin = ln.kmin;
   const int first = st0 + warp;
-  const int n = st1 > first ? (st1 - first + KV8_WARPS - 1) / KV8_WARPS : 0;
+  const int n = sq.len > kmin && st1 > first ? (st1 - first + KV8_WARPS - 1) / KV8_WARPS : 0;
+  const auto step_key = [&](int i) { return kmin + (first + i * KV8_WARPS) * KV8_STEP; };
 
   // ---- the warp's ring
   unsigned char* ring = kv8_smem + S::QF_BYTES + warp * S::STAGES * S::STAGE_BYTES;
   const uint32_t ring_u = smem_u32(ring);
-  const auto load_id = [&](int i) { return i < n ? table[step_key(kmin, first, i) >> a.block_shift] : -1; };
+  const auto load_id = [&](int i) { return i < n ? table[step_key(i) >> a.block_shift] : -1; };
   const auto load_scales = [&](int id) {
     const bool in = id >= 0 && id < a.num_blocks;
     const long long at = (long long)(in ? id : 0) * a.kv_heads + h;
     return in ? make_float2(a.ks[at], a.vs[at]) : make_float2(0.f, 0.f);  // a scale of 0 marks a block the cache has not
   };
-  if (a.window) id_even = load_id(lane);
-  if (n > 32) id_odd = load_id(32 + lane);
+  int id_even = load_id(lane), id_odd = load_id(32 + lane);  // block ids of an even and of an odd batch of 32 steps, one step per lane
   constexpr int W = HD / 16;  // 16-byte words of a key
   const int k_lane = lane / W, w_lane = lane % W;  // (a warp copies 32 / W keys at a time)
   const bool w_in = w_lane * 16 < a.hd;
   const auto issue = [&](int i) {
     if (i < n) {
       const int id = __shfl_sync(0xffffffffu, (i >> 5) & 1 ? id_odd : id_even, i & 31);
-      const int key0 = step_key(kmin, first, i);
+      const int key0 = step_key(i);
       const bool ok = w_in && id >= 0 && id < a.num_blocks;
       const long long at = (((long long)(ok ? id : 0) * a.kv_heads + h) << a.block_shift) + (key0 & ((1 << a.block_shift) - 1));
       const int left = ok ? sq.len - key0 : 0;  // keys of this step that exist
@@ -230,7 +307,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
     if ((i & 31) == 24) raw = load_scales(i + 8 + lane < n ? ((i >> 5) & 1 ? id_even : id_odd) : -1);
     const uint32_t kst = ring_u + (i % S::STAGES) * S::STAGE_BYTES, vst = kst + KV8_STEP * HD;
     const float ks = __shfl_sync(0xffffffffu, b_ks, i & 31), lv = __shfl_sync(0xffffffffu, b_lv, i & 31), iv = __shfl_sync(0xffffffffu, b_iv, i & 31);
-    const int key0 = step_key(kmin, first, i);
+    const int key0 = step_key(i);
     // scores, in two accumulators (hi and lo, or odd and even depth steps) to shorten the chains
     float c[NT][2][4] = {};
 #pragma unroll
@@ -379,8 +456,8 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
       l += f[w] * s_ml[w][row].y;
     }
     const long long ri = (long long)(sq.row0 + tok);
-    const long long pi = (ri * heads + hq) * a.splits + split;
-    const float inv = a.splits == 1 ? (l == 0.f ? 0.f : (1.f / KV8_WMUL) / l) : 1.f / KV8_WMUL;
+    const long long pi = part * RT + row;
+    const float inv = whole ? (l == 0.f ? 0.f : (1.f / KV8_WMUL) / l) : 1.f / KV8_WMUL;
     for (int d = 4 * lane; d < a.hd; d += 128) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
@@ -392,13 +469,15 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
         v.w = fmaf(f[w], y.w, v.w);
       }
       v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-      if (a.splits == 1) store_elem4(a.out, a.q_type, ri * a.o_row + (long long)hq * a.o_head + d, v, a.o_vec);
+      if (whole) store_elem4(a.out, a.q_type, ri * a.o_row + (long long)hq * a.o_head + d, v, a.o_vec);
       else *reinterpret_cast<float4*>(a.part_o + pi * a.hd + d) = v;
     }
     if (lane == 0) {
-      if (a.splits > 1) a.part_ml[pi] = make_float2(r, l);
+      if (!whole) a.part_ml[pi] = make_float2(r, l);
       else if (a.lse) a.lse[ri * heads + hq] = l == 0.f ? -INFINITY : (r + log2f(l)) * 0.6931471805599453f;
     }
+  }
+  __syncthreads();  // the next unit reuses the ring and the row state
   }
 }
 
@@ -420,9 +499,27 @@ __global__ void __launch_bounds__(MERGE_THREADS) gg_kv8_merge_kernel(const Kv8Ar
   x /= a.merge_tokens;
   const Kv8Seq sq = kv8_seq(a, x);
   if (tok >= sq.n) return;
-  const long long ri = sq.row0 + tok, pi = (ri * heads + hq) * a.splits;
+  const long long ri = sq.row0 + tok;
+  // where the parts of this row stand: part z at index pi + z * pstep (many rows: its key ranges; few
+  // rows: the first CTA of its unit's line, which is its second unit unless the two begin together,
+  // then the first unit of each CTA after it)
+  int nparts = a.splits;
+  long long p0 = (ri * heads + hq) * a.splits, pi = p0, pstep = 1;
+  if (a.pre) {
+    const int RT = a.tile_rows, item = tok * a.group + hq % a.group;
+    const Kv8Line ln = kv8_line(a, sq, RT);
+    const long long chunk = kv8_chunk(a.pre[a.seqs], a.few_ctas);
+    const long long u0 = a.pre[x] + ((long long)(hq / a.group) * ln.tiles + item / RT) * ln.steps;
+    const long long c0 = u0 / chunk, c1 = (u0 + ln.steps - 1) / chunk;
+    if (c0 == c1) return;  // finished by its CTA
+    nparts = (int)(c1 - c0 + 1);
+    pstep = 2 * RT;
+    pi = 2 * c0 * RT + item % RT;
+    p0 = pi + (u0 > c0 * chunk ? RT : 0);
+  }
+  const auto at = [&](int z) { return z ? pi + z * pstep : p0; };
   float r = KV8_NEG;
-  for (int z = t; z < a.splits; z += MERGE_THREADS) r = fmaxf(r, a.part_ml[pi + z].x);
+  for (int z = t; z < nparts; z += MERGE_THREADS) r = fmaxf(r, a.part_ml[at(z)].x);
   const int lanes = a.hd <= 64 ? 16 : a.hd <= 128 ? 32 : 64, parts = MERGE_THREADS / lanes;
   const int d = 4 * (t % lanes), z0 = t / lanes;
   r = warp_max(r);
@@ -431,8 +528,8 @@ __global__ void __launch_bounds__(MERGE_THREADS) gg_kv8_merge_kernel(const Kv8Ar
 #pragma unroll
   for (int w = 0; w < MERGE_THREADS / 32; w++) r = fmaxf(r, s_r[w]);
   float l = 0.f;
-  for (int z = t; z < a.splits; z += MERGE_THREADS) {
-    const float2 ml = a.part_ml[pi + z];
+  for (int z = t; z < nparts; z += MERGE_THREADS) {
+    const float2 ml = a.part_ml[at(z)];
     l = fmaf(ex2(ml.x - r), ml.y, l);
   }
   l = warp_sum(l);
@@ -440,9 +537,9 @@ __global__ void __launch_bounds__(MERGE_THREADS) gg_kv8_merge_kernel(const Kv8Ar
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
   if (d < a.hd)
 #pragma unroll 4
-    for (int z = z0; z < a.splits; z += parts) {
-      const float f = ex2(a.part_ml[pi + z].x - r);
-      const float4 y = *reinterpret_cast<const float4*>(a.part_o + (pi + z) * a.hd + d);
+    for (int z = z0; z < nparts; z += parts) {
+      const float f = ex2(a.part_ml[at(z)].x - r);
+      const float4 y = *reinterpret_cast<const float4*>(a.part_o + at(z) * a.hd + d);
       v.x = fmaf(f, y.x, v.x);
       v.y = fmaf(f, y.y, v.y);
       v.z = fmaf(f, y.z, v.z);
@@ -465,8 +562,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) gg_kv8_merge_kernel(const Kv8Ar
 
 template <int HD, int CODE, bool HILO, int NT>
 cudaError_t launch_rows(const Kv8Args& a, cudaStream_t s) {
-  const long long grid = (long long)a.seqs * a.kv_heads * a.row_tiles * a.splits;
-  return launch_big_smem(gg_kv8_rows_kernel<HD, CODE, HILO, NT>, dim3((unsigned)grid), dim3(KV8_WARPS * 32), RowsShape<HD, HILO, NT>::SMEM, s, a);
+  return launch_big_smem(gg_kv8_rows_kernel<HD, CODE, HILO, NT>, dim3((unsigned)a.few_ctas), dim3(KV8_WARPS * 32), RowsShape<HD, HILO, NT>::SMEM, s, a);
 }
 template <int HD, int CODE, bool HILO>
 cudaError_t launch_rows_nt(const Kv8Args& a, int nt, cudaStream_t s) {
@@ -490,48 +586,47 @@ static int kv8_row_tiles(long long items, int head_dim) { return items <= 8 ? 1 
 // other's requests.
 constexpr int KV8_FEW = 32;
 
-struct Kv8Cut {
-  int row_tiles = 0, splits = 0, split_steps = 1;  // row_tiles 0: not launched
-  size_t parts = 0;                                // partial results
-};
-static Kv8Cut kv8_cut(long long items, int tile, long long slots, int least_steps, long long rows, int q_heads,
-                      const gg_kv8_cache& c, const gg_kv8_attention_call& b) {
-  Kv8Cut p;
-  p.row_tiles = (int)((items + tile - 1) / tile);
-  // keys that a tile may read: all, or its window with the rows between its first and last
-  long long keys = b.max_len;
-  if (b.window && keys > (long long)b.window + tile + 2 * KV8_STEP) keys = (long long)b.window + tile + 2 * KV8_STEP;
-  const long long steps = (keys + KV8_STEP - 1) / KV8_STEP;
-  const long long units = (long long)b.seqs * c.kv_heads * p.row_tiles;
-  long long splits = units ? (slots + units - 1) / units : 1;
-  const long long most = (steps + least_steps - 1) / least_steps;
-  if (splits > most) splits = most;
-  if (splits < 1) splits = 1;
-  p.split_steps = (int)((steps + splits - 1) / splits);
-  if (p.split_steps < 1) p.split_steps = 1;
-  p.splits = (int)((steps + p.split_steps - 1) / p.split_steps);
-  if (p.splits < 1) p.splits = 1;
-  if (p.splits > 1) p.parts = (size_t)rows * q_heads * p.splits;
-  return p;
-}
 struct Kv8Plan {
-  Kv8Cut few, many;
-  int nt;  // tiles of eight rows of a CTA of the first
-  size_t few_bytes, bytes;
+  // few rows: tiles of eight rows of a CTA, CTAs (0: not launched), parts that they may leave
+  int nt = 1, few_ctas = 0;
+  size_t few_parts = 0;
+  // many rows: row tiles of a request and head (0: not launched), key ranges, 16-key steps of a range
+  int row_tiles = 0, splits = 1, split_steps = 1;
+  size_t many_parts = 0;
+  size_t few_bytes = 0, bytes = 0;
 };
 static Kv8Plan kv8_plan(const gg_kv8_cache& c, const gg_kv8_attention_call& b) {
   Kv8Plan p;
-  const int group = b.q.heads / c.kv_heads;
-  const long long items = (long long)b.max_rows * group;
-  // few rows: three CTAs fit an SM, three waves of them even out requests of different lengths; a
-  // step at least for each warp. Many rows: one CTA an SM, at least 512 keys.
-  const long long few = items < KV8_FEW ? items : KV8_FEW;
+  if (!b.seqs || !b.max_rows) return p;
+  const long long items = (long long)b.max_rows * (b.q.heads / c.kv_heads), few = items < KV8_FEW ? items : KV8_FEW;
+  // keys that a tile may read: all, or its window with the rows between its first and last
+  const auto steps = [&](long long tile) {
+    long long keys = b.max_len;
+    if (b.window && keys > (long long)b.window + tile + 2 * KV8_STEP) keys = (long long)b.window + tile + 2 * KV8_STEP;
+    return (keys + KV8_STEP - 1) / KV8_STEP;
+  };
   p.nt = kv8_row_tiles(few, c.head_dim);
-  p.few = kv8_cut(few, 8 * p.nt, 148 * 3 * 3, KV8_WARPS, b.rows, b.q.heads, c, b);
-  if (items > KV8_FEW) p.many = kv8_cut(items, kv8_prompt_tile(c.head_dim), 148, 32, b.rows, b.q.heads, c, b);
-  const auto bytes = [&](const Kv8Cut& k) { return k.parts * c.head_dim * 4 + k.parts * 8; };
-  p.few_bytes = bytes(p.few);
-  p.bytes = p.few_bytes + bytes(p.many);
+  const int rt = 8 * p.nt, hd = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+  const double line = (double)b.seqs * c.kv_heads * ((few + rt - 1) / rt) * (steps(few) + 1);
+  const int resident = 148 * (p.nt * hd >= 512 ? 2 : 3);  // RowsShape::CTAS
+  p.few_ctas = line >= (double)resident * KV8_WARPS ? resident : (int)(line / KV8_WARPS) + 1;
+  p.few_parts = p.few_ctas > 1 ? (size_t)2 * p.few_ctas * rt : 0;
+  if (items > KV8_FEW) {  // one CTA an SM; ranges of at least 512 keys where there are fewer tiles than SMs
+    const int tile = kv8_prompt_tile(c.head_dim);
+    p.row_tiles = (int)((items + tile - 1) / tile);
+    const long long units = (long long)b.seqs * c.kv_heads * p.row_tiles, n = steps(tile), most = (n + 31) / 32;
+    long long splits = (148 + units - 1) / units;
+    if (splits > most) splits = most;
+    if (splits < 1) splits = 1;
+    p.split_steps = (int)((n + splits - 1) / splits);
+    if (p.split_steps < 1) p.split_steps = 1;
+    p.splits = (int)((n + p.split_steps - 1) / p.split_steps);
+    if (p.splits < 1) p.splits = 1;
+    if (p.splits > 1) p.many_parts = (size_t)b.rows * b.q.heads * p.splits;
+  }
+  // partial outputs, then their (r, l) pairs; few rows: then the line's prefix sums
+  p.few_bytes = p.few_parts ? (p.few_parts * (c.head_dim * 4 + 8) + ((size_t)b.seqs + 1) * 8 + 15) / 16 * 16 : 0;
+  p.bytes = p.few_bytes + p.many_parts * (c.head_dim * 4 + 8);
   return p;
 }
 
@@ -544,9 +639,8 @@ static int kv8_check(const char* fn, const gg_kv8_cache* c, const gg_kv8_attenti
     return ops_fail(GG_E_ARG, "%s: seqs %d, rows %d, max_rows %d, max_len %d out of range", fn, b->seqs, b->rows, b->max_rows, b->max_len);
   if (b->window < 0) return ops_fail(GG_E_ARG, "%s: window %d", fn, b->window);
   const Kv8Plan p = kv8_plan(*c, *b);
-  for (const Kv8Cut* k : {&p.few, &p.many})
-    if ((double)b->seqs * c->kv_heads * k->row_tiles * k->splits >= 2147483647.0)
-      return ops_fail(GG_E_ARG, "%s: the batch needs more than 2^31 tiles", fn);
+  if ((double)b->seqs * c->kv_heads * p.row_tiles * p.splits >= 2147483647.0 || (double)b->seqs * b->max_rows * b->q.heads >= 2147483647.0)
+    return ops_fail(GG_E_ARG, "%s: the batch needs more than 2^31 tiles", fn);
   return GG_OK;
 }
 
@@ -611,25 +705,37 @@ extern "C" int gg_kv8_attention(const gg_kv8_cache* c, const gg_kv8_attention_ca
   a.q_vec = ops_aligned16(b.q);
   a.o_vec = ops_aligned16(b.out);
   cudaError_t r = cudaSuccess;
-  for (int many = 0; many < 2 && r == cudaSuccess; many++) {
-    const Kv8Cut& k = many ? p.many : p.few;
-    if (!k.row_tiles) continue;
-    a.row_tiles = k.row_tiles;
-    a.splits = k.splits;
-    a.split_steps = k.split_steps;
-    a.items_lo = many ? KV8_FEW : 0;
-    a.items_hi = many ? 0x7fffffff : KV8_FEW;
-    a.part_o = reinterpret_cast<float*>(static_cast<char*>(b.workspace) + (many ? p.few_bytes : 0));
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + k.parts * c->head_dim);
-    r = many ? kv8_launch_prompt(a, c->code, s)
-        : c->head_dim <= 64 ? launch_rows_hd<64>(a, c->code, p.nt, s)
-        : c->head_dim <= 128 ? launch_rows_hd<128>(a, c->code, p.nt, s)
-                             : launch_rows_hd<256>(a, c->code, p.nt, s);
-    if (r == cudaSuccess && k.splits > 1) {
-      const long long tokens = many ? b.max_rows : (KV8_FEW + a.group - 1) / a.group;
-      a.merge_tokens = (int)(tokens < b.max_rows ? tokens : b.max_rows);
-      r = launch_pdl(gg_kv8_merge_kernel, dim3((unsigned)((long long)b.seqs * a.merge_tokens * b.q.heads)), dim3(MERGE_THREADS), 0, s, a);
-    }
+  const auto merge = [&](int tokens) {
+    a.merge_tokens = tokens < b.max_rows ? tokens : b.max_rows;
+    return launch_pdl(gg_kv8_merge_kernel, dim3((unsigned)((long long)b.seqs * a.merge_tokens * b.q.heads)), dim3(MERGE_THREADS), 0, s, a);
+  };
+  const auto parts = [&](size_t offset, size_t n) {
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(b.workspace) + offset);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + n * c->head_dim);
+  };
+  // requests with few rows
+  a.items_lo = 0;
+  a.items_hi = KV8_FEW;
+  a.splits = 1;
+  a.few_ctas = p.few_ctas;
+  a.tile_rows = 8 * p.nt;
+  parts(0, p.few_parts);
+  a.pre = p.few_parts ? reinterpret_cast<long long*>(a.part_ml + p.few_parts) : nullptr;
+  r = c->head_dim <= 64 ? launch_rows_hd<64>(a, c->code, p.nt, s)
+      : c->head_dim <= 128 ? launch_rows_hd<128>(a, c->code, p.nt, s)
+                           : launch_rows_hd<256>(a, c->code, p.nt, s);
+  if (r == cudaSuccess && p.few_parts) r = merge((KV8_FEW + a.group - 1) / a.group);
+  // requests with many
+  if (r == cudaSuccess && p.row_tiles) {
+    a.items_lo = KV8_FEW;
+    a.items_hi = 0x7fffffff;
+    a.row_tiles = p.row_tiles;
+    a.splits = p.splits;
+    a.split_steps = p.split_steps;
+    a.pre = nullptr;
+    parts(p.few_bytes, p.many_parts);
+    r = kv8_launch_prompt(a, c->code, s);
+    if (r == cudaSuccess && p.splits > 1) r = merge(b.max_rows);
   }
   if (r != cudaSuccess) return ops_fail(GG_E_CUDA, "%s: launch: %s", fn, cudaGetErrorString(r));
   return GG_OK;
