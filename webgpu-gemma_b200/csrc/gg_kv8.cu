@@ -22,12 +22,11 @@ namespace gg {
 //
 // A unit is one request, one key head and one tile of 8 NT query rows (the `group` heads of a few
 // tokens); its keys are steps of 16 (one MMA's depth for the second product, never across a block).
-// The steps of all units stand in one line that is cut into equal chunks, one for each resident CTA:
-// requests of any lengths then load the SMs alike, in one wave, whatever the host knows of them.
-// Bound by the cache's bytes. Each of the four warps streams its own steps through a private
-// cp.async ring (no barriers between warps); the warps' results meet in shared memory at the end
-// of a unit. A unit inside one chunk is finished there, parts of the others meet in
-// gg_kv8_merge_kernel.
+// Each unit is cut into parts of nearly equal steps, one CTA each, so many that the resident CTAs
+// fill the GPU once whatever the lengths of the requests are (only the device knows them: every CTA
+// sums up the requests and finds its part). Bound by the cache's bytes. Each of the four warps
+// streams its own steps through a private cp.async ring (no barriers between warps); the warps'
+// results meet in shared memory at the end, the parts of a unit in gg_kv8_merge_kernel.
 //
 // Both products are transposed, so that the few query rows are the narrow side (N = 8) of an
 // m16n8k16 MMA and the accumulators hold nothing else: S^T = K Q^T (16 keys x 8 rows), then
@@ -72,22 +71,24 @@ GG_DEV uint32_t transpose8x8(uint32_t x) {  // of f16 pairs: (row g, columns 2t,
   return d;
 }
 
-// Units of a request and steps of each (the same for its tiles), for requests with rows.
+// Row tiles of a request (0: no rows) and steps of each (the same for its tiles).
 struct Kv8Line {
   int tiles, steps, kmin;
 };
 GG_DEV Kv8Line kv8_line(const Kv8Args& a, const Kv8Seq& q, int RT) {
-  Kv8Line n = {0, 1, 0};
-  const int items = q.n * a.group;
-  n.tiles = (items + RT - 1) / RT;
+  Kv8Line n;
+  n.tiles = (q.n * a.group + RT - 1) / RT;
   n.kmin = a.window ? (int)min(max(0ll, q.first_pos - a.window + 1), (long long)q.len) & ~(KV8_STEP - 1) : 0;
   n.steps = max(1, (q.len - n.kmin + KV8_STEP - 1) / KV8_STEP);  // a request without keys has one step that sees nothing
   return n;
 }
-// Steps of a chunk for `total` steps over `ctas` CTAs: at least one for each warp.
-GG_DEV long long kv8_chunk(long long total, int ctas) {
-  const long long c = (total + ctas - 1) / ctas;
-  return max(c + KV8_WARPS - 1, (long long)KV8_WARPS) / KV8_WARPS * KV8_WARPS;
+// Steps of a part, for `total` steps in `units` units, so that the parts are not above the resident
+// CTAs (a unit rounds its number of parts up): `share` of 0 to 4 quarters of the units counts the
+// roundings; 4 is always enough. A step at least for each warp.
+GG_DEV int kv8_part_steps(long long total, int units, int resident, int share) {
+  if (resident == 0) return 1 << 29;  // units are not cut (steps stay below 2^28)
+  const long long c = 2 * units <= resident ? (total + resident - 1) / (resident - share * units / 4) : (2 * total + resident - 1) / resident;
+  return (int)max(c + 1, (long long)KV8_WARPS);
 }
 
 template <int HD, int CODE, bool HILO, int NT>
@@ -98,89 +99,107 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
   __shared__ float s_mul[RT];
   __shared__ float2 s_ml[KV8_WARPS][RT];
   __shared__ int s_hi[RT];
-  __shared__ long long s_sum[KV8_WARPS], s_off;
-  __shared__ int s_seq;
+  __shared__ long long s_sum[KV8_WARPS];
+  __shared__ int s_units[KV8_WARPS], s_try[3][KV8_WARPS], s_seq, s_off;
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  // ---- this CTA's chunk of the line: prefix sums of the requests' steps, THREADS * PER at a time
-  const auto steps_of = [&](int i) {
-    if (i >= a.seqs) return 0ll;
-    const Kv8Line n = kv8_line(a, kv8_seq(a, i), RT);
-    return (long long)n.tiles * n.steps * a.kv_heads;
+  // ---- this CTA's part: all steps and units first, then the parts before each request
+  int steps[PER], units[PER];
+  const auto look = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const int i = i0 + tid * PER + k;
+      steps[k] = 1;
+      units[k] = 0;
+      if (i < a.seqs) {
+        const Kv8Line n = kv8_line(a, kv8_seq(a, i), RT);
+        steps[k] = n.steps;
+        units[k] = n.tiles * a.kv_heads;
+      }
+    }
   };
-  long long v[PER], total = 0;
-  const bool once = a.seqs <= THREADS * PER;
+  long long total = 0;
+  int all_units = 0;
   for (int i0 = 0; i0 < a.seqs; i0 += THREADS * PER) {
-    long long sum = 0;
+    look(i0);
 #pragma unroll
-    for (int k = 0; k < PER; k++) sum += v[k] = steps_of(i0 + tid * PER + k);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    total += sum;
+    for (int k = 0; k < PER; k++) {
+      total += (long long)steps[k] * units[k];
+      all_units += units[k];
+    }
   }
-  if (lane == 0) s_sum[warp] = total;
+  // (a sum over the warp of numbers below 2^50, in two halves)
+  total = (long long)__reduce_add_sync(0xffffffffu, (uint32_t)total & 0xffffffu) + ((long long)__reduce_add_sync(0xffffffffu, (uint32_t)(total >> 24)) << 24);
+  all_units = __reduce_add_sync(0xffffffffu, all_units);
+  if (lane == 0) {
+    s_sum[warp] = total;
+    s_units[warp] = all_units;
+  }
   if (tid == 0) s_seq = -1;
   __syncthreads();
   total = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-  const long long chunk = kv8_chunk(total, gridDim.x), line0 = blockIdx.x * chunk;
-  const long long line1 = min(line0 + chunk, total);
-  if (blockIdx.x == 0 && tid == 0 && a.pre) a.pre[a.seqs] = total;
-  if (line0 >= total && (blockIdx.x || !a.pre)) return;
-  {
-    long long run = 0;
-    for (int i0 = 0; i0 < a.seqs; i0 += THREADS * PER) {
-      __syncthreads();
-      long long sum = 0;
+  all_units = s_units[0] + s_units[1] + s_units[2] + s_units[3];
+  int part_steps = kv8_part_steps(total, all_units, a.resident, 4);
+  // the shortest parts that still fit one wave (sums by a rounded reciprocal: a part too many costs time, nothing else)
+  if (a.resident && 2 * all_units <= a.resident && a.seqs <= THREADS * PER && total > (long long)a.resident * KV8_WARPS) {
+    int n[3] = {0, 0, 0};
 #pragma unroll
-      for (int k = 0; k < PER; k++) {
-        if (!once) v[k] = steps_of(i0 + tid * PER + k);
-        sum += v[k];
-      }
-      long long inc = sum;
+    for (int j = 0; j < 3; j++) {
+      const int c = kv8_part_steps(total, all_units, a.resident, j + 1);
+      const float inv = __fdividef(1.f, (float)c);
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, inc, d);
-        if (lane >= d) inc += u;
-      }
-      if (lane == 31) s_sum[warp] = inc;
-      __syncthreads();
-      long long before = run + inc - sum;
-      for (int w = 0; w < warp; w++) before += s_sum[w];
-#pragma unroll
-      for (int k = 0; k < PER; k++) {
-        const int i = i0 + tid * PER + k;
-        if (blockIdx.x == 0 && a.pre && i < a.seqs) a.pre[i] = before;
-        if (before <= line0 && line0 < before + v[k]) {
-          s_seq = i;
-          s_off = line0 - before;
-        }
-        before += v[k];
-      }
-      run += s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-      if (run > line0 && (blockIdx.x || !a.pre)) break;
+      for (int k = 0; k < PER; k++) n[j] += units[k] * (int)((float)(steps[k] + c - 1) * inv);
+      n[j] = __reduce_add_sync(0xffffffffu, n[j]);
+      if (lane == 0) s_try[j][warp] = n[j];
     }
     __syncthreads();
+#pragma unroll
+    for (int j = 2; j >= 0; j--)
+      if (s_try[j][0] + s_try[j][1] + s_try[j][2] + s_try[j][3] <= a.resident) part_steps = kv8_part_steps(total, all_units, a.resident, j + 1);
   }
-  if (line0 >= line1) return;
-  int s = s_seq;
-  long long off = s_off;
+  const bool report = blockIdx.x == 0 && a.pre;  // the merge needs the sums too
+  int run = 0;
+  for (int i0 = 0; i0 < a.seqs; i0 += THREADS * PER) {
+    __syncthreads();
+    if (a.seqs > THREADS * PER) look(i0);
+    int sum = 0, parts[PER];
+#pragma unroll
+    for (int k = 0; k < PER; k++) sum += parts[k] = units[k] * ((steps[k] + part_steps - 1) / part_steps);
+    int inc = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += u;
+    }
+    if (lane == 31) s_units[warp] = inc;
+    __syncthreads();
+    int before = run + inc - sum;
+    for (int w = 0; w < warp; w++) before += s_units[w];
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const int i = i0 + tid * PER + k;
+      if (report && i < a.seqs) a.pre[i] = before;
+      if (before <= (int)blockIdx.x && (int)blockIdx.x < before + parts[k]) {
+        s_seq = i;
+        s_off = blockIdx.x - before;
+      }
+      before += parts[k];
+    }
+    run += s_units[0] + s_units[1] + s_units[2] + s_units[3];
+    if (run > (int)blockIdx.x && !report) break;
+  }
+  if (report && tid == 0) a.pre[a.seqs] = part_steps;
+  __syncthreads();
+  const int s = s_seq;
+  if (s < 0) return;  // more CTAs than parts
   const int heads = a.kv_heads * a.group;
-  for (long long line = line0; line < line1;) {
   const Kv8Seq sq = kv8_seq(a, s);
   const Kv8Line ln = kv8_line(a, sq, RT);
-  if (off >= (long long)ln.tiles * ln.steps * a.kv_heads) {  // the request's units are done, or it has none
-    s++;
-    off = 0;
-    continue;
-  }
-  const int unit = (int)(off / ln.steps), st0 = (int)(off % ln.steps);
-  const int st1 = (int)min((long long)ln.steps, st0 + (line1 - line));
+  const int nparts = (ln.steps + part_steps - 1) / part_steps, unit = s_off / nparts, part = s_off % nparts;
+  const int st0 = (int)((long long)ln.steps * part / nparts), st1 = (int)((long long)ln.steps * (part + 1) / nparts);
   const int h = unit / ln.tiles, base = (unit % ln.tiles) * RT;
-  const bool whole = st0 == 0 && st1 == ln.steps;
-  const long long part = 2ll * blockIdx.x + (line > line0);  // a chunk has at most two units that it shares
-  off += st1 - st0;
-  line += st1 - st0;
+  const bool whole = nparts == 1;
   const int32_t* table = a.table + (long long)s * a.table_stride;
   const int nitems = min(RT, sq.n * a.group - base), kmin = ln.kmin;
   const int first = st0 + warp;
@@ -197,6 +216,19 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
     return in ? make_float2(a.ks[at], a.vs[at]) : make_float2(0.f, 0.f);  // a scale of 0 marks a block the cache has not
   };
   int id_even = load_id(lane), id_odd = load_id(32 + lane);  // block ids of an even and of an odd batch of 32 steps, one step per lane
+  // the warp's query rows, fetched while the ids are
+  constexpr int QR = RT / KV8_WARPS, QP = (HD / 4 + 31) / 32;
+  float4 qv[QR][QP];
+#pragma unroll
+  for (int j = 0; j < QR; j++) {
+    const int row = warp + j * KV8_WARPS, it = base + row;
+    const long long qi = (long long)(sq.row0 + it / a.group) * a.q_row + (long long)(h * a.group + it % a.group) * a.q_head;
+#pragma unroll
+    for (int p = 0; p < QP; p++) {
+      const int d = 4 * (lane + 32 * p);
+      qv[j][p] = row < nitems && d < a.hd ? load_elem4(a.q, a.q_type, qi + d, a.q_vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  }
   constexpr int W = HD / 16;  // 16-byte words of a key
   const int k_lane = lane / W, w_lane = lane % W;  // (a warp copies 32 / W keys at a time)
   const bool w_in = w_lane * 16 < a.hd;
@@ -226,17 +258,14 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
 
   // ---- query rows -> f16 operand fragments
   unsigned char* qf = kv8_smem;
-  for (int row = warp; row < RT; row += KV8_WARPS) {
+#pragma unroll
+  for (int j = 0; j < QR; j++) {
+    const int row = warp + j * KV8_WARPS;
     const bool live = row < nitems;
-    const int it = base + row;
-    const long long qi = live ? (long long)(sq.row0 + it / a.group) * a.q_row + (long long)(h * a.group + it % a.group) * a.q_head : 0;
-    constexpr int PER = (HD / 4 + 31) / 32;
-    float4 v[PER];
+    float4 (&v)[QP] = qv[j];
     uint32_t top = 0;
 #pragma unroll
-    for (int p = 0; p < PER; p++) {
-      const int d = 4 * (lane + 32 * p);
-      v[p] = live && d < a.hd ? load_elem4(a.q, a.q_type, qi + d, a.q_vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < QP; p++) {
       top = max(max(top, __float_as_uint(v[p].x) & 0x7fffffffu), __float_as_uint(v[p].y) & 0x7fffffffu);
       top = max(max(top, __float_as_uint(v[p].z) & 0x7fffffffu), __float_as_uint(v[p].w) & 0x7fffffffu);
     }
@@ -245,10 +274,10 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
     const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
     if (lane == 0) {
       s_mul[row] = __uint_as_float((uint32_t)(ex - 14 + 127) << 23) * a.scale_log2;
-      s_hi[row] = live ? (int)min(sq.first_pos + it / a.group, (long long)sq.len - 1) : -1;
+      s_hi[row] = live ? (int)min(sq.first_pos + (base + row) / a.group, (long long)sq.len - 1) : -1;
     }
 #pragma unroll
-    for (int p = 0; p < PER; p++) {
+    for (int p = 0; p < QP; p++) {
       const int d = 4 * (lane + 32 * p);
       if (d >= HD) break;
       const int ks = 4 * (d >> 6) + ((d >> 2) & 3), tt = (d >> 4) & 3;
@@ -456,7 +485,7 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
       l += f[w] * s_ml[w][row].y;
     }
     const long long ri = (long long)(sq.row0 + tok);
-    const long long pi = part * RT + row;
+    const long long pi = (long long)blockIdx.x * RT + row;
     const float inv = whole ? (l == 0.f ? 0.f : (1.f / KV8_WMUL) / l) : 1.f / KV8_WMUL;
     for (int d = 4 * lane; d < a.hd; d += 128) {
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -476,8 +505,6 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
       if (!whole) a.part_ml[pi] = make_float2(r, l);
       else if (a.lse) a.lse[ri * heads + hq] = l == 0.f ? -INFINITY : (r + log2f(l)) * 0.6931471805599453f;
     }
-  }
-  __syncthreads();  // the next unit reuses the ring and the row state
   }
 }
 
@@ -500,24 +527,18 @@ __global__ void __launch_bounds__(MERGE_THREADS) gg_kv8_merge_kernel(const Kv8Ar
   const Kv8Seq sq = kv8_seq(a, x);
   if (tok >= sq.n) return;
   const long long ri = sq.row0 + tok;
-  // where the parts of this row stand: part z at index pi + z * pstep (many rows: its key ranges; few
-  // rows: the first CTA of its unit's line, which is its second unit unless the two begin together,
-  // then the first unit of each CTA after it)
+  // the parts of this row: many rows, its key ranges; few rows, the CTAs of its unit
   int nparts = a.splits;
-  long long p0 = (ri * heads + hq) * a.splits, pi = p0, pstep = 1;
+  long long p0 = (ri * heads + hq) * a.splits, pstep = 1;
   if (a.pre) {
     const int RT = a.tile_rows, item = tok * a.group + hq % a.group;
     const Kv8Line ln = kv8_line(a, sq, RT);
-    const long long chunk = kv8_chunk(a.pre[a.seqs], a.few_ctas);
-    const long long u0 = a.pre[x] + ((long long)(hq / a.group) * ln.tiles + item / RT) * ln.steps;
-    const long long c0 = u0 / chunk, c1 = (u0 + ln.steps - 1) / chunk;
-    if (c0 == c1) return;  // finished by its CTA
-    nparts = (int)(c1 - c0 + 1);
-    pstep = 2 * RT;
-    pi = 2 * c0 * RT + item % RT;
-    p0 = pi + (u0 > c0 * chunk ? RT : 0);
+    nparts = (ln.steps + a.pre[a.seqs] - 1) / a.pre[a.seqs];
+    if (nparts == 1) return;  // finished by its CTA
+    p0 = ((long long)a.pre[x] + ((hq / a.group) * ln.tiles + item / RT) * nparts) * RT + item % RT;
+    pstep = RT;
   }
-  const auto at = [&](int z) { return z ? pi + z * pstep : p0; };
+  const auto at = [&](int z) { return p0 + z * pstep; };
   float r = KV8_NEG;
   for (int z = t; z < nparts; z += MERGE_THREADS) r = fmaxf(r, a.part_ml[at(z)].x);
   const int lanes = a.hd <= 64 ? 16 : a.hd <= 128 ? 32 : 64, parts = MERGE_THREADS / lanes;
@@ -584,11 +605,12 @@ static int kv8_row_tiles(long long items, int head_dim) { return items <= 8 ? 1 
 // How a call is cut. Requests with few rows (rows * group up to KV8_FEW) take the kernel above, the
 // others the one of gg_kv8_prompt.cu; a call that may hold both launches both, and each skips the
 // other's requests.
-constexpr int KV8_FEW = 32;
+constexpr int KV8_FEW = 32, KV8_WHOLE = 128 << 10;
 
 struct Kv8Plan {
-  // few rows: tiles of eight rows of a CTA, CTAs (0: not launched), parts that they may leave
-  int nt = 1, few_ctas = 0;
+  // few rows: tiles of eight rows of a CTA, CTAs (-1: too many), how many the GPU holds (0: units are
+  // not cut), rows of parts that they may leave
+  int nt = 1, few_ctas = 0, resident = 0;
   size_t few_parts = 0;
   // many rows: row tiles of a request and head (0: not launched), key ranges, 16-key steps of a range
   int row_tiles = 0, splits = 1, split_steps = 1;
@@ -607,10 +629,14 @@ static Kv8Plan kv8_plan(const gg_kv8_cache& c, const gg_kv8_attention_call& b) {
   };
   p.nt = kv8_row_tiles(few, c.head_dim);
   const int rt = 8 * p.nt, hd = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
-  const double line = (double)b.seqs * c.kv_heads * ((few + rt - 1) / rt) * (steps(few) + 1);
-  const int resident = 148 * (p.nt * hd >= 512 ? 2 : 3);  // RowsShape::CTAS
-  p.few_ctas = line >= (double)resident * KV8_WARPS ? resident : (int)(line / KV8_WARPS) + 1;
-  p.few_parts = p.few_ctas > 1 ? (size_t)2 * p.few_ctas * rt : 0;
+  const double units = (double)b.seqs * c.kv_heads * ((few + rt - 1) / rt), line = units * (steps(few) + 1);
+  if (line + units >= 2147483647.0) return p.few_ctas = -1, p;
+  // Units of at most KV8_WHOLE bytes of codes are not cut: reading them takes less than a second kernel.
+  const bool cut = (double)(steps(few) + 1) * 2 * KV8_STEP * c.head_dim > KV8_WHOLE;
+  p.resident = cut ? 148 * (p.nt * hd >= 512 ? 2 : 3) : 0;  // RowsShape::CTAS
+  const double most = cut ? line / KV8_WARPS : 0;
+  p.few_ctas = (int)((most < p.resident ? most : p.resident) + units) + 1;  // parts are at most that many
+  p.few_parts = cut ? (size_t)p.few_ctas * rt : 0;
   if (items > KV8_FEW) {  // one CTA an SM; ranges of at least 512 keys where there are fewer tiles than SMs
     const int tile = kv8_prompt_tile(c.head_dim);
     p.row_tiles = (int)((items + tile - 1) / tile);
@@ -625,7 +651,7 @@ static Kv8Plan kv8_plan(const gg_kv8_cache& c, const gg_kv8_attention_call& b) {
     if (p.splits > 1) p.many_parts = (size_t)b.rows * b.q.heads * p.splits;
   }
   // partial outputs, then their (r, l) pairs; few rows: then the line's prefix sums
-  p.few_bytes = p.few_parts ? (p.few_parts * (c.head_dim * 4 + 8) + ((size_t)b.seqs + 1) * 8 + 15) / 16 * 16 : 0;
+  p.few_bytes = p.few_parts ? (p.few_parts * (c.head_dim * 4 + 8) + ((size_t)b.seqs + 1) * 4 + 15) / 16 * 16 : 0;
   p.bytes = p.few_bytes + p.many_parts * (c.head_dim * 4 + 8);
   return p;
 }
@@ -639,7 +665,7 @@ static int kv8_check(const char* fn, const gg_kv8_cache* c, const gg_kv8_attenti
     return ops_fail(GG_E_ARG, "%s: seqs %d, rows %d, max_rows %d, max_len %d out of range", fn, b->seqs, b->rows, b->max_rows, b->max_len);
   if (b->window < 0) return ops_fail(GG_E_ARG, "%s: window %d", fn, b->window);
   const Kv8Plan p = kv8_plan(*c, *b);
-  if ((double)b->seqs * c->kv_heads * p.row_tiles * p.splits >= 2147483647.0 || (double)b->seqs * b->max_rows * b->q.heads >= 2147483647.0)
+  if (p.few_ctas < 0 || (double)b->seqs * c->kv_heads * p.row_tiles * p.splits >= 2147483647.0 || (double)b->seqs * b->max_rows * b->q.heads >= 2147483647.0)
     return ops_fail(GG_E_ARG, "%s: the batch needs more than 2^31 tiles", fn);
   return GG_OK;
 }
@@ -718,9 +744,10 @@ extern "C" int gg_kv8_attention(const gg_kv8_cache* c, const gg_kv8_attention_ca
   a.items_hi = KV8_FEW;
   a.splits = 1;
   a.few_ctas = p.few_ctas;
+  a.resident = p.resident;
   a.tile_rows = 8 * p.nt;
   parts(0, p.few_parts);
-  a.pre = p.few_parts ? reinterpret_cast<long long*>(a.part_ml + p.few_parts) : nullptr;
+  a.pre = p.few_parts ? reinterpret_cast<int*>(a.part_ml + p.few_parts) : nullptr;
   r = c->head_dim <= 64 ? launch_rows_hd<64>(a, c->code, p.nt, s)
       : c->head_dim <= 128 ? launch_rows_hd<128>(a, c->code, p.nt, s)
                            : launch_rows_hd<256>(a, c->code, p.nt, s);

@@ -20,15 +20,15 @@ struct Kv8Args {
   float* lse;
   const int32_t *cu, *lens, *table;
   // partial results (r, l: running maximum and sum): many rows [row][head][range], few rows
-  // [CTA][its first or second unit][row of the tile]
+  // [CTA][row of the tile]
   float* part_o;
   float2* part_ml;
-  long long* pre;  // few rows: steps of the requests before each one, and of all; or NULL
+  int* pre;  // few rows: parts before each request, then the steps of a part; or NULL
   long long q_row, q_head, o_row, o_head, table_stride;
   float scale_log2;
   int seqs, rows, max_rows, max_len, num_blocks, block_shift, kv_heads, group, hd, window, q_type;
   int row_tiles, splits, split_steps;  // split_steps: 16-key steps of a key range
-  int few_ctas, tile_rows;             // few rows: CTAs of the launch, rows of a tile
+  int few_ctas, tile_rows, resident;  // few rows: CTAs of the launch, rows of a tile
   int merge_tokens;                    // tokens of a request that the merge looks at
   int items_lo, items_hi;  // this launch takes requests with items_lo < rows * group <= items_hi
   int q_vec, o_vec;  // every head of q / out starts on a 16-byte boundary
