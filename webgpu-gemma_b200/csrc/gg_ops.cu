@@ -410,8 +410,8 @@ cudaError_t launch_rope(const RopeArgs& a, bool vec, cudaStream_t s) {
 // Code and scale of a block: e = min{e >= -60 : max |x| <= Q 2^e}, code = rne(x 2^-e), Q = 127 or
 // 448. Bound by its bytes: the new rows read once, a byte per value written. The CTA that finds
 // the first row of a block's run takes the whole run, so the block's scale needs no atomics and
-// no second launch: one pass for the largest value, one that rounds (the rows come from registers,
-// or for long runs from L1/L2).
+// no second launch: one pass for the largest value, one that rounds (the rows stay in registers, as
+// they were read; what long runs have above that comes from L1/L2 again).
 constexpr int APPEND_THREADS = 128;
 constexpr int KV8_MIN_EXP = -60;
 
@@ -469,9 +469,44 @@ struct AppendArgs {
   int rows, num_slots, block_shift, heads, hd, rows_per_cta;
 };
 
+// Eight values of a row as they were read, widened when they are used.
+template <class T, bool VEC>
+struct Raw8 {
+  uint4 w[sizeof(T) / 2];
+  GG_DEV void load(const T* p) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+      for (int i = 0; i < 8; i++) e[i] = p[i];
+    }
+  }
+  GG_DEV void get(float (&v)[8]) const {
+    const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = to_f32(e[i]);
+  }
+  // The largest |pattern| so far, of a 16-bit type two at a time; NaN is above all.
+  GG_DEV void raise(uint32_t& m) const {
+    const uint32_t* e = reinterpret_cast<const uint32_t*>(w);
+#pragma unroll
+    for (int i = 0; i < 2 * (int)sizeof(T); i++)
+      m = sizeof(T) == 2 ? __vmaxu2(m, e[i] & 0x7fff7fffu) : max(m, e[i] & 0x7fffffffu);
+  }
+};
+// The same as the pattern of an f32.
+template <class T>
+GG_DEV uint32_t top_pattern(uint32_t m) {
+  if constexpr (sizeof(T) == 4) return m;
+  const uint16_t u = (uint16_t)max(m & 0xffffu, m >> 16);
+  return __float_as_uint(to_f32(*reinterpret_cast<const T*>(&u)));
+}
+
 template <class T, int CODE, bool VEC>
 __global__ void __launch_bounds__(APPEND_THREADS) gg_append_kernel(const AppendArgs a) {
-  constexpr int KEEP = 4;  // groups of eight values a thread keeps between the two passes
+  constexpr int KEEP = 16 / (int)sizeof(T);  // groups of eight values a thread keeps between the two passes
   __shared__ uint32_t s_max;
   pdl_trigger();
   pdl_wait();
@@ -479,24 +514,23 @@ __global__ void __launch_bounds__(APPEND_THREADS) gg_append_kernel(const AppendA
   const int h = blockIdx.y >> 1, which = blockIdx.y & 1;
   const int B = 1 << a.block_shift;
   const int groups = a.hd / 8;
-  const T* x = static_cast<const T*>(a.x[which]) + (long long)h * a.head[which];
-  const long long xrow = a.row[which];
-  const auto slot_of = [&](int r) { const int s = a.slots[r]; return s >= 0 && s < a.num_slots ? s : -1; };
-  const int r_end = min(a.rows, (int)(blockIdx.x + 1) * a.rows_per_cta);
-  for (int r = blockIdx.x * a.rows_per_cta; r < r_end; r++) {
-    const int s0 = slot_of(r);
-    if (s0 < 0) continue;
+  const uint32_t gmagic = (65536u + groups - 1) / groups;  // i / groups for i < 2048
+  const T* x = static_cast<const T*>(which ? a.x[1] : a.x[0]) + (long long)h * (which ? a.head[1] : a.head[0]);
+  const long long xrow = which ? a.row[1] : a.row[0];
+  const auto slot_of = [&](int r) { const int s = r >= 0 && r < a.rows ? a.slots[r] : -1; return s >= 0 && s < a.num_slots ? s : -1; };
+  // the rows of this CTA's tile (at most 32) that begin a block's run; the others belong to earlier ones
+  const int r0 = blockIdx.x * a.rows_per_cta;
+  const int s_here = lane < a.rows_per_cta ? slot_of(r0 + lane) : -1, s_prev = slot_of(r0 + lane - 1);
+  uint32_t leaders = __ballot_sync(0xffffffffu, s_here >= 0 && (s_prev < 0 || (s_prev >> a.block_shift) != (s_here >> a.block_shift)));
+  for (; leaders; leaders &= leaders - 1) {
+    const int r = r0 + __ffs(leaders) - 1;
+    const int s0 = __shfl_sync(0xffffffffu, s_here, r - r0);
     const int blk = s0 >> a.block_shift;
-    if (r > 0) {
-      const int sp = slot_of(r - 1);
-      if (sp >= 0 && (sp >> a.block_shift) == blk) continue;  // an earlier row leads this run
-    }
     // the run: rows r .. r + m - 1 of this block; each warp finds it alone
     int m = 0, first = B;
     bool ascending = true;
     for (;;) {
-      const int rr = r + m + lane;
-      const int s = rr < a.rows ? slot_of(rr) : -1;
+      const int s = slot_of(r + m + lane);
       const bool in = s >= 0 && (s >> a.block_shift) == blk;
       const uint32_t out = __ballot_sync(0xffffffffu, !in);
       const int n = out ? __ffs(out) - 1 : 32;
@@ -505,9 +539,13 @@ __global__ void __launch_bounds__(APPEND_THREADS) gg_append_kernel(const AppendA
       m += n;
       if (n < 32) break;
     }
-    // of rows with the same slot only the last counts
+    const auto row_of = [&](int i) { return i < 2048 ? (int)((i * gmagic) >> 16) : i / groups; };
+    const auto fetch = [&](int i, Raw8<T, VEC>& v) {
+      const int j = row_of(i);
+      v.load(x + (long long)(r + j) * xrow + (i - j * groups) * 8);
+    };
+    // of rows with the same slot only the last counts (rows in ascending order have no such)
     const auto replaced = [&](int j) {
-      if (ascending) return false;
       const int s = a.slots[r + j];
       for (int k = j + 1; k < m; k++)
         if (a.slots[r + k] == s) return true;
@@ -516,33 +554,28 @@ __global__ void __launch_bounds__(APPEND_THREADS) gg_append_kernel(const AppendA
     if (t == 0) s_max = 0;
     __syncthreads();
     const int items = m * groups;
-    float keep[KEEP][8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int k = 0; k < KEEP; k++) {
-      const int i = t + k * APPEND_THREADS;
-      if (i < items) {
-        const int j = i / groups;
-        load_row<T, 8, VEC>(x + (long long)(r + j) * xrow + (i - j * groups) * 8, keep[k]);
-        if (!replaced(j))
-#pragma unroll
-          for (int q = 0; q < 8; q++) top = max(top, __float_as_uint(keep[k][q]) & 0x7fffffffu);
-      }
-    }
-    for (int i = t + KEEP * APPEND_THREADS; i < items; i += APPEND_THREADS) {
-      const int j = i / groups;
-      float v[8];
-      load_row<T, 8, VEC>(x + (long long)(r + j) * xrow + (i - j * groups) * 8, v);
-      if (!replaced(j))
-#pragma unroll
-        for (int q = 0; q < 8; q++) top = max(top, __float_as_uint(v[q]) & 0x7fffffffu);
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0 && top) atomicMax(&s_max, top);
-    __syncthreads();
-    top = s_max;
-    float* scale = a.scale[which] + (long long)blk * a.heads + h;
+    float* scale = (which ? a.scale[1] : a.scale[0]) + (long long)blk * a.heads + h;
     const float before = first > 0 ? *scale : 0.f;
+    Raw8<T, VEC> keep[KEEP];
+    uint32_t top = 0;
+    if (ascending) {
+#pragma unroll
+      for (int k = 0; k < KEEP; k++)
+        if (t + k * APPEND_THREADS < items) fetch(t + k * APPEND_THREADS, keep[k]);
+#pragma unroll
+      for (int k = 0; k < KEEP; k++)
+        if (t + k * APPEND_THREADS < items) keep[k].raise(top);
+    }
+#pragma unroll 1
+    for (int i = t + (ascending ? KEEP * APPEND_THREADS : 0); i < items; i += APPEND_THREADS) {
+      Raw8<T, VEC> v;
+      fetch(i, v);
+      if (ascending || !replaced(row_of(i))) v.raise(top);
+    }
+    top = __reduce_max_sync(0xffffffffu, top_pattern<T>(top));
+    if (lane == 0 && top) atomicMax(&s_max, top);
+    __syncthreads();  // (everyone has read the old scale, too)
+    top = s_max;
     bool finite = top < 0x7f800000u;
     int e = finite ? kv8_exponent<CODE>(top) : 0;
     float shrink = 1.f;  // what the codes of earlier tokens are multiplied by
@@ -555,34 +588,36 @@ __global__ void __launch_bounds__(APPEND_THREADS) gg_append_kernel(const AppendA
         else e = old;
       }
     }
-    __syncthreads();  // everyone has read the old scale and the maximum
     if (t == 0) *scale = finite ? pow2i(e) : __uint_as_float(0x7fffffffu);
-    uint8_t* codes = a.codes[which] + ((long long)blk * a.heads + h) * B * a.hd;
+    uint8_t* codes = (which ? a.codes[1] : a.codes[0]) + ((long long)blk * a.heads + h) * B * a.hd;
     if (shrink != 1.f)
+#pragma unroll 1
       for (int i = t; i < first * groups; i += APPEND_THREADS) {
         uint2* w = reinterpret_cast<uint2*>(codes) + i;
         *w = kv8_rescale8<CODE>(*w, shrink);
       }
     const float inv = pow2i(-e);
-    const auto put = [&](int i, const float (&v)[8]) {
-      const int j = i / groups;
-      if (replaced(j)) return;
+    const auto encode = [&](const Raw8<T, VEC>& raw) {
       float y[8];
+      raw.get(y);
 #pragma unroll
-      for (int q = 0; q < 8; q++) y[q] = finite ? v[q] * inv : 0.f;
-      const int off = a.slots[r + j] & (B - 1);
-      reinterpret_cast<uint2*>(codes + (long long)off * a.hd)[i - j * groups] = kv8_encode8<CODE>(y);
+      for (int q = 0; q < 8; q++) y[q] *= inv;
+      return finite ? kv8_encode8<CODE>(y) : make_uint2(0, 0);
     };
+    uint2* dst = reinterpret_cast<uint2*>(codes);
+    if (ascending) {
+      // consecutive rows fill consecutive slots: item i of the run is item i of the block from its first slot on
 #pragma unroll
-    for (int k = 0; k < KEEP; k++) {
-      const int i = t + k * APPEND_THREADS;
-      if (i < items) put(i, keep[k]);
+      for (int k = 0; k < KEEP; k++)
+        if (t + k * APPEND_THREADS < items) dst[first * groups + t + k * APPEND_THREADS] = encode(keep[k]);
     }
-    for (int i = t + KEEP * APPEND_THREADS; i < items; i += APPEND_THREADS) {
-      const int j = i / groups;
-      float v[8];
-      load_row<T, 8, VEC>(x + (long long)(r + j) * xrow + (i - j * groups) * 8, v);
-      put(i, v);
+#pragma unroll 1
+    for (int i = t + (ascending ? KEEP * APPEND_THREADS : 0); i < items; i += APPEND_THREADS) {
+      const int j = row_of(i);
+      if (!ascending && replaced(j)) continue;
+      Raw8<T, VEC> v;
+      fetch(i, v);
+      dst[(ascending ? first + j : a.slots[r + j] & (B - 1)) * groups + i - j * groups] = encode(v);
     }
     __syncthreads();  // s_max is reused by the next run
   }
@@ -740,10 +775,10 @@ extern "C" int gg_kv8_append(const gg_kv8_cache* c, const gg_kv8_append_call* ca
   a.num_slots = c->num_blocks << a.block_shift;
   a.heads = c->kv_heads;
   a.hd = c->head_dim;
-  // one row per CTA until its launches alone would cost more than the rows do: every row of a
-  // decode step starts a run, while a prompt's rows start one in block_tokens
+  // rows that a CTA looks through for the first of a run: every row of a decode step starts one, a
+  // prompt's rows one in block_tokens, and CTAs that find none still cost their launch
   int per = 1;
-  while (per < 16 && (long long)rows * c->kv_heads * 2 > 148ll * 16 * per) per *= 2;
+  while (per < 32 && (long long)rows * c->kv_heads * 2 > 148ll * 8 * per) per *= 2;
   a.rows_per_cta = per;
   const dim3 grid((rows + per - 1) / per, 2 * c->kv_heads);
   const bool vec = ops_aligned16(*k) && ops_aligned16(*v);
