@@ -39,6 +39,14 @@ typedef struct gg_engine gg_engine;
  * the reference's f32 (engine.ts:440-447): half the cache memory and half the attention bytes.
  * Attention reads the stored (rounded) rows, the current position's included. */
 #define GG_FLAG_KV_BF16 2
+/* gg_config.flags: keep the KV cache in 8 bits (int8 codes, one power-of-two scale per 16 tokens and
+ * key head, as gg_kv8_append writes them): a quarter of the f32 cache's memory. Every token then
+ * runs through the batched path (gg_prefill in chunks, gg_step and gg_decode as gg_decode_batch of one
+ * sequence), which needs the tensor-core shapes and head_dim <= 256; any grouping of query heads
+ * works. A slot's positions are written in order: a call may start at or below the slot's length, not
+ * beyond it. gg_get_hidden is not available. Not together with GG_FLAG_KV_BF16 or
+ * GG_FLAG_SERIAL_PREFILL. */
+#define GG_FLAG_KV_Q8 4
 
 /* Field-for-field the reference's GemmaConfig (src/types.ts:2-17), plus the number of
  * independent KV slots and option flags. */
@@ -106,8 +114,8 @@ int gg_get_logits(gg_engine* eng, float* out);
 /* Final-normed hidden state of the last step (hidden_size floats), engine.ts:797-801. */
 int gg_get_hidden(gg_engine* eng, float* out);
 
-/* One row of the KV cache (kv_dim floats, widened from bf16 under GG_FLAG_KV_BF16;
- * which = 0 for K, 1 for V). */
+/* One row of the KV cache (kv_dim floats, widened from bf16 under GG_FLAG_KV_BF16, code * scale
+ * under GG_FLAG_KV_Q8; which = 0 for K, 1 for V). */
 int gg_get_kv(gg_engine* eng, int seq, int layer, int pos, int which, float* out);
 
 /* Debug/parity aid: copy `n` floats of an internal buffer of the last launch.

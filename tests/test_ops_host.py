@@ -233,3 +233,18 @@ def test_torch_wrappers_refuse_cpu_tensors(lib):
         ops.rope_frequencies(64, 1e4, "cubic", device="cpu")
     f, m = ops.rope_frequencies(64, 1e4, device="cpu")
     assert f.dtype == torch.float64 and f.shape == (32,) and m == 1.0
+
+
+def test_q8_cache_flag(lib):
+    """GG_FLAG_KV_Q8 goes with neither the bf16 cache nor serial prefill (checked before any device)."""
+    from gemma_b200 import config, synth
+    cfg = synth.SHAPES["tiny"].config()
+    cfg.kv_dtype = "q8"
+    assert config.kv_flags(cfg) == config.GG_FLAG_KV_Q8 == 4
+    for flags in (config.GG_FLAG_KV_BF16, native.GG_FLAG_SERIAL_PREFILL):
+        h = ctypes.c_void_p()
+        assert lib.gg_create(ctypes.byref(config.to_cconfig(cfg, flags=flags)), 0, ctypes.byref(h)) == native.GG_E_ARG
+        assert b"GG_FLAG_KV_Q8" in lib.gg_last_error(None)
+    cfg.kv_dtype = "q4"
+    with pytest.raises(ValueError, match="q8"):
+        config.kv_flags(cfg)

@@ -170,7 +170,20 @@ struct gg_engine {
   int32_t* bd_out = nullptr;
   int32_t* bd_out_h = nullptr;  // pinned
   size_t bd_io_cap = 0;         // entries of bd_unif / bd_out / bd_out_h
+  // 8-bit KV cache (GG_FLAG_KV_Q8): one pool of blocks per layer, slot s owning kv8_blocks of them
+  bool kv8 = false;
+  int kv8_blocks = 0;
+  uint8_t *k8 = nullptr, *v8 = nullptr;   // codes [layer][slot][block][head][token][dim]
+  float *k8s = nullptr, *v8s = nullptr;   // scales [layer][slot][block][head]
+  std::vector<int> kv8_len;               // tokens in each slot
+  std::vector<const double*> kv8_freqs;   // RoPE frequencies of each layer
+  PfKv8Rows kv8_rows{};
+  float *kv8_qkv = nullptr, *kv8_att = nullptr;
+  void* kv8_ws = nullptr;
+  size_t kv8_ws_bytes = 0;
 };
+
+constexpr int KV8_BLOCK = 16;  // tokens that share a scale
 
 constexpr int GG_BATCH_MAX = 128;  // sequences per batched step
 static_assert(sizeof(GGSampleDev) == sizeof(gg_sample), "gg_sample layout");
@@ -221,6 +234,50 @@ static int dalloc(gg_engine* e, T** p, size_t bytes) {
     if (_c != GG_OK) return _c; \
   } while (0)
 
+// A call of an operator of the library (its message is the engineless one).
+#define GG_OPS(e, call)                                              \
+  do {                                                               \
+    int _c = (call);                                                 \
+    if (_c != GG_OK) return fail((e), _c, "%s", g_create_err.c_str()); \
+  } while (0)
+
+// Layer l's blocks of the 8-bit cache.
+static gg_kv8_cache kv8_cache(const gg_engine* e, int l) {
+  const gg_config& c = e->cfg;
+  const size_t scales = (size_t)c.max_seqs * e->kv8_blocks * c.num_kv_heads, codes = scales * KV8_BLOCK * c.head_dim;
+  return {e->k8 + l * codes, e->v8 + l * codes, e->k8s + l * scales, e->v8s + l * scales, c.max_seqs * e->kv8_blocks, KV8_BLOCK,
+          c.num_kv_heads, c.head_dim, GG_KV8_INT8};
+}
+static int grow(gg_engine* e, void** p, size_t* cap, size_t need);
+// One layer's attention over the 8-bit cache: the q/k/v planes in pf_y to activation tiles. The rows'
+// positions, slots and requests are in kv8_rows (pf_kv8_rows, once per step).
+static int kv8_attention(gg_engine* e, int l, int splits, long long plane, int reqs, int rows, int max_rows, int max_len,
+                         uint8_t* thi, uint8_t* tlo) {
+  const GGModelDev& m = e->md;
+  const GGLayerW& w = m.layers[l];
+  cudaStream_t s = e->stream;
+  const int W = m.Q + 2 * m.KV;
+  GG_CUDA(e, pf_qkv_norm(e->pf_y, splits, plane, w.q_norm, w.k_norm, rows, m.NQH, m.NKH, m.HD, m.eps, e->kv8_qkv, s));
+  const gg_rows q = {e->kv8_qkv, W, m.HD, m.NQH, GG_T_F32}, k = {e->kv8_qkv + m.Q, W, m.HD, m.NKH, GG_T_F32},
+                v = {e->kv8_qkv + m.Q + m.KV, W, m.HD, m.NKH, GG_T_F32};
+  const gg_rope_call rope = {q, k, q, k, e->kv8_rows.positions, e->kv8_freqs[l], 1.0, rows, m.HD, m.HD, GG_ROPE_HALF, 0};
+  GG_OPS(e, gg_rope(&rope, s));
+  const gg_kv8_cache c = kv8_cache(e, l);
+  const gg_kv8_append_call put = {k, v, e->kv8_rows.slots, rows};
+  GG_OPS(e, gg_kv8_append(&c, &put, s));
+  const gg_rows out = {e->kv8_att, m.Q, m.HD, m.NQH, GG_T_F32};
+  gg_kv8_attention_call att = {q, out, nullptr, e->kv8_rows.cu_rows, e->kv8_rows.lens, e->kv8_rows.table, e->kv8_blocks, nullptr, 0,
+                               m.attn_scale, reqs, rows, max_rows, max_len, w.window};
+  size_t need = 0;
+  GG_OPS(e, gg_kv8_attention_workspace(&c, &att, &need));
+  GG_TRY(grow(e, &e->kv8_ws, &e->kv8_ws_bytes, need));
+  att.workspace = e->kv8_ws;
+  att.workspace_bytes = e->kv8_ws_bytes;
+  GG_OPS(e, gg_kv8_attention(&c, &att, s));
+  GG_CUDA(e, gg_xtiles_from_f32(e->kv8_att, rows, m.Q, thi, tlo, s));
+  return GG_OK;
+}
+
 enum { T_Q = 0, T_K, T_V, T_O, T_GATE, T_UP, T_DOWN, T_ATTN_NORM, T_FFN_NORM, T_Q_NORM, T_K_NORM, T_POST_ATTN, T_POST_FFW, T_COUNT };
 static const char* kLayerNames[T_COUNT] = {"attn_q",    "attn_k",   "attn_v",      "attn_output",  "ffn_gate",
                                            "ffn_up",    "ffn_down", "attn_norm",   "ffn_norm",     "attn_q_norm",
@@ -238,12 +295,19 @@ extern "C" int gg_create(const gg_config* cfg, int device, gg_engine** out) {
     return fail(nullptr, GG_E_ARG, "unsupported config (dims must be positive multiples of 32, q_dim = heads*head_dim)");
   if (c.swa_period < 1 || c.sliding_window < 0)
     return fail(nullptr, GG_E_ARG, "unsupported config (swa_period >= 1, sliding_window >= 0)");
+  if (c.flags & GG_FLAG_KV_Q8) {
+    if (c.flags & (GG_FLAG_KV_BF16 | GG_FLAG_SERIAL_PREFILL))
+      return fail(nullptr, GG_E_ARG, "unsupported config (GG_FLAG_KV_Q8 goes with neither GG_FLAG_KV_BF16 nor GG_FLAG_SERIAL_PREFILL)");
+    if (c.head_dim > 256 || (long long)c.max_seqs * c.context_length >= (1ll << 30))
+      return fail(nullptr, GG_E_ARG, "unsupported config (an 8-bit KV cache takes head_dim up to 256 and 2^30 tokens in all)");
+  }
   int ndev = 0;
   if (cudaGetDeviceCount(&ndev) != cudaSuccess || device < 0 || device >= ndev)
     return fail(nullptr, GG_E_CUDA, "no CUDA device %d", device);
   gg_engine* e = new gg_engine();
   e->cfg = c;
   e->device = device;
+  e->kv8 = (c.flags & GG_FLAG_KV_Q8) != 0;
   auto bail = [&](int code) {
     g_create_err = e->err;
     gg_destroy(e);
@@ -283,8 +347,18 @@ extern "C" int gg_create(const gg_config* cfg, int device, gg_engine** out) {
   if (rc == GG_OK) rc = dalloc(e, &e->out_norm, (size_t)H * 4);
   m.kv_seq_stride = (size_t)L * m.CTX * KV;
   m.kv_es = (c.flags & GG_FLAG_KV_BF16) ? 2 : 4;
-  if (rc == GG_OK) rc = dalloc(e, &m.kcache, m.kv_seq_stride * m.kv_es * c.max_seqs);
-  if (rc == GG_OK) rc = dalloc(e, &m.vcache, m.kv_seq_stride * m.kv_es * c.max_seqs);
+  if (e->kv8) {
+    e->kv8_blocks = (m.CTX + KV8_BLOCK - 1) / KV8_BLOCK;
+    e->kv8_len.assign(c.max_seqs, 0);
+    const size_t scales = (size_t)L * c.max_seqs * e->kv8_blocks * c.num_kv_heads, codes = scales * KV8_BLOCK * c.head_dim;
+    if (rc == GG_OK) rc = dalloc(e, &e->k8, codes);
+    if (rc == GG_OK) rc = dalloc(e, &e->v8, codes);
+    if (rc == GG_OK) rc = dalloc(e, &e->k8s, 4 * scales);
+    if (rc == GG_OK) rc = dalloc(e, &e->v8s, 4 * scales);
+  } else {
+    if (rc == GG_OK) rc = dalloc(e, &m.kcache, m.kv_seq_stride * m.kv_es * c.max_seqs);
+    if (rc == GG_OK) rc = dalloc(e, &m.vcache, m.kv_seq_stride * m.kv_es * c.max_seqs);
+  }
   if (rc != GG_OK) return bail(rc);
   return (*out = e, GG_OK);
 }
@@ -570,6 +644,33 @@ extern "C" int gg_finalize(gg_engine* e) {
     GG_TRY(dalloc(e, &e->pf_gtiles, 2 * e->pf_gtiles_half));
     GG_TRY(dalloc(e, &e->pf_kvsplit, pf_kv_split_bytes(m.CTX, m.KV)));
   }
+  if (e->kv8) {
+    if (!e->gemm_ok) return fail(e, GG_E_ARG, "an 8-bit KV cache needs the tensor-core path (shapes in multiples of 128 x 64)");
+    const int rows = std::max(GG_PF_CHUNK, std::min(c.max_seqs, GG_BATCH_MAX)), reqs = std::min(c.max_seqs, GG_BATCH_MAX);
+    GG_TRY(dalloc(e, &e->kv8_rows.positions, 4 * (size_t)rows));
+    GG_TRY(dalloc(e, &e->kv8_rows.slots, 4 * (size_t)rows));
+    GG_TRY(dalloc(e, &e->kv8_rows.cu_rows, 4 * ((size_t)reqs + 1)));
+    GG_TRY(dalloc(e, &e->kv8_rows.lens, 4 * (size_t)reqs));
+    GG_TRY(dalloc(e, &e->kv8_rows.table, 4 * (size_t)reqs * e->kv8_blocks));
+    GG_TRY(dalloc(e, &e->kv8_qkv, 4 * (size_t)rows * (m.Q + 2 * m.KV)));
+    GG_TRY(dalloc(e, &e->kv8_att, 4 * (size_t)rows * m.Q));
+    std::vector<std::pair<float, double*>> tabs;
+    for (int l = 0; l < c.num_layers; l++) {
+      double* f = nullptr;
+      for (auto& t : tabs)
+        if (t.first == m.layers[l].theta) f = t.second;
+      if (!f) {
+        std::vector<double> host(m.HD / 2);
+        double one = 1.0;
+        GG_OPS(e, gg_rope_freqs(GG_ROPE_NONE, m.HD, m.layers[l].theta, 1.0, 0.0, 0.0, 0.0, host.data(), &one));
+        GG_TRY(dalloc(e, &f, sizeof(double) * host.size()));
+        GG_CUDA(e, cudaMemcpyAsync(f, host.data(), sizeof(double) * host.size(), cudaMemcpyHostToDevice, e->stream));
+        GG_CUDA(e, cudaStreamSynchronize(e->stream));  // `host` goes out of scope
+        tabs.push_back({m.layers[l].theta, f});
+      }
+      e->kv8_freqs.push_back(f);
+    }
+  }
   // exchange buffers of the step kernel (tagged words; one slot per CTA, or per attention split)
   GG_TRY(dalloc(e, &m.t_qkv, 8 * (size_t)m.grid * m.sl_qkv));
   GG_TRY(dalloc(e, &m.t_o, 8 * (size_t)m.max_splits * m.att_slot));
@@ -710,6 +811,7 @@ static int prefill_batched(gg_engine* e, int seq, int n, int start_pos) {
     T = std::min(GG_PF_CHUNK, n - c0);
     const int p0 = start_pos + c0;
     GG_CUDA(e, pf_embed(e->d_ids + c0, T, m.embd, m.rs_h, m.H, e->pf_hidden, s));
+    if (e->kv8) GG_CUDA(e, pf_kv8_rows(nullptr, nullptr, seq, p0, T, e->kv8_blocks, e->kv8_rows, s));
     GG_CUDA(e, pf_addnorm(nullptr, 0, 0, nullptr, e->pf_hidden, e->pf_hidden, m.layers[0].attn_norm, thi, tlo, T, m.H,
                           m.eps, s));
     for (int l = 0; l < m.L; l++) {
@@ -721,10 +823,14 @@ static int prefill_batched(gg_engine* e, int seq, int n, int start_pos) {
       int sp = pick_splits(gemm_tiles(T, QKV), m.H / 64, gemm_slots(e, T));
       long long plane = (long long)T * QKV;
       GG_CUDA(e, gg_gemm_q8(mp[0], thi, tlo, T, e->pf_y, QKV, sp, plane, err, to, s));
-      GG_CUDA(e, pf_qk_rope_store(e->pf_y, sp, plane, w.q_norm, w.k_norm, w.rope, T, p0, m.NQH, m.NKH, m.HD, m.eps,
-                                  e->pf_q, kc, vc, m.kv_es == 2, e->pf_kvsplit, m.CTX, s));
-      GG_CUDA(e, pf_attention(e->pf_q, kc, vc, m.kv_es == 2, T, p0, m.NQH, m.NKH, m.HD, m.attn_scale, w.window,
-                              e->pf_att, e->pf_kvsplit, m.CTX, true, thi, tlo, s));
+      if (e->kv8) {
+        GG_TRY(kv8_attention(e, l, sp, plane, 1, T, T, p0 + T, thi, tlo));
+      } else {
+        GG_CUDA(e, pf_qk_rope_store(e->pf_y, sp, plane, w.q_norm, w.k_norm, w.rope, T, p0, m.NQH, m.NKH, m.HD, m.eps,
+                                    e->pf_q, kc, vc, m.kv_es == 2, e->pf_kvsplit, m.CTX, s));
+        GG_CUDA(e, pf_attention(e->pf_q, kc, vc, m.kv_es == 2, T, p0, m.NQH, m.NKH, m.HD, m.attn_scale, w.window,
+                                e->pf_att, e->pf_kvsplit, m.CTX, true, thi, tlo, s));
+      }
       sp = pick_splits(gemm_tiles(T, m.H), m.Q / 64, gemm_slots(e, T));
       plane = (long long)T * m.H;
       GG_CUDA(e, gg_gemm_q8(mp[1], thi, tlo, T, e->pf_y, m.H, sp, plane, err, to, s));
@@ -771,6 +877,7 @@ static int batch_step(gg_engine* e, int B, int max_pos, const double* d_unif, in
   const uint64_t to = e->timeout_ns;
   const int QKV = m.Q + 2 * m.KV;
   GG_CUDA(e, pf_embed(e->bd_tok, B, m.embd, m.rs_h, m.H, e->pf_hidden, s));
+  if (e->kv8) GG_CUDA(e, pf_kv8_rows(e->bd_seq, e->bd_pos, 0, 0, B, e->kv8_blocks, e->kv8_rows, s));
   GG_CUDA(e, pf_addnorm(nullptr, 0, 0, nullptr, e->pf_hidden, e->pf_hidden, m.layers[0].attn_norm, thi, tlo, B, m.H,
                         m.eps, s));
   for (int l = 0; l < m.L; l++) {
@@ -781,9 +888,12 @@ static int batch_step(gg_engine* e, int B, int max_pos, const double* d_unif, in
     int sp = pick_splits(gemm_tiles(B, QKV), m.H / 64, gemm_slots(e, B));
     long long plane = (long long)B * QKV;
     GG_CUDA(e, gg_gemm_q8(mp[0], thi, tlo, B, e->pf_y, QKV, sp, plane, err, to, s));
-    GG_CUDA(e, bd_attention(e->pf_y, sp, plane, w.q_norm, w.k_norm, w.rope, m.eps, kc, vc, m.kv_es == 2, B, e->bd_pos,
-                            e->bd_seq, m.kv_seq_stride, max_pos, m.NQH, m.NKH, m.HD,
-                            m.attn_scale, w.window, e->bd_att, thi, tlo, s));
+    if (e->kv8)
+      GG_TRY(kv8_attention(e, l, sp, plane, B, B, 1, max_pos + 1, thi, tlo));
+    else
+      GG_CUDA(e, bd_attention(e->pf_y, sp, plane, w.q_norm, w.k_norm, w.rope, m.eps, kc, vc, m.kv_es == 2, B, e->bd_pos,
+                              e->bd_seq, m.kv_seq_stride, max_pos, m.NQH, m.NKH, m.HD,
+                              m.attn_scale, w.window, e->bd_att, thi, tlo, s));
     sp = pick_splits(gemm_tiles(B, m.H), m.Q / 64, gemm_slots(e, B));
     plane = (long long)B * m.H;
     GG_CUDA(e, gg_gemm_q8(mp[1], thi, tlo, B, e->pf_y, m.H, sp, plane, err, to, s));
@@ -817,7 +927,7 @@ extern "C" int gg_decode_batch(gg_engine* e, int n, const int32_t* seqs, const i
   GG_TRY(ready(e, 0));
   const gg_config& c = e->cfg;
   const GGModelDev& m = e->md;
-  if (!e->gemm_ok || m.NQH != 4 || m.NKH != 1)
+  if (!e->gemm_ok || (!e->kv8 && (m.NQH != 4 || m.NKH != 1)))
     return fail(e, GG_E_STATE, "batched decode needs the tensor-core path and 4 query heads sharing 1 KV head");
   if (n < 1 || n > std::min(c.max_seqs, GG_BATCH_MAX)) return fail(e, GG_E_ARG, "batch of %d sequences (1..%d)", n, std::min(c.max_seqs, GG_BATCH_MAX));
   if (steps < 1 || !seqs || !tokens || !pos || !sp || !uniforms || !out_tokens) return fail(e, GG_E_ARG, "bad arguments");
@@ -829,6 +939,8 @@ extern "C" int gg_decode_batch(gg_engine* e, int n, const int32_t* seqs, const i
     if (tokens[i] < 0 || tokens[i] >= c.vocab_size) return fail(e, GG_E_ARG, "token %d out of range", tokens[i]);
     if (pos[i] < 0 || pos[i] + steps > c.context_length)
       return fail(e, GG_E_ARG, "positions %d..%d exceed context %d", pos[i], pos[i] + steps - 1, c.context_length);
+    if (e->kv8 && pos[i] > e->kv8_len[seqs[i]])
+      return fail(e, GG_E_ARG, "position %d is beyond the %d tokens of slot %d (the 8-bit cache is written in order)", pos[i], e->kv8_len[seqs[i]], seqs[i]);
     max_pos = std::max(max_pos, pos[i]);
   }
   if (e->bd_max == 0) {  // first batched call: buffers for up to bd_max rows
@@ -868,6 +980,23 @@ extern "C" int gg_decode_batch(gg_engine* e, int n, const int32_t* seqs, const i
   GG_CUDA(e, cudaMemcpyAsync(e->bd_out_h, e->bd_out, sizeof(int32_t) * io, cudaMemcpyDeviceToHost, s));
   GG_TRY(finish(e, nullptr));
   memcpy(out_tokens, e->bd_out_h, sizeof(int32_t) * io);
+  for (int i = 0; e->kv8 && i < n; i++) e->kv8_len[seqs[i]] = pos[i] + steps;
+  return GG_OK;
+}
+
+// gg_step and gg_decode over the 8-bit cache: a batch of one sequence, whose last logits and hidden
+// state go where the step kernel leaves them.
+static int kv8_decode(gg_engine* e, int seq, int32_t token, int pos, int n, const gg_sample* sp, const double* uniforms,
+                      int32_t* out_tokens) {
+  const GGModelDev& m = e->md;
+  const gg_sample greedy = {0.0, 1.0, 1.0};
+  const std::vector<double> zeros(uniforms ? 0 : n, 0.0);
+  const int32_t s32 = seq, p32 = pos;
+  GG_TRY(gg_decode_batch(e, 1, &s32, &token, &p32, n, sp ? sp : &greedy, uniforms ? uniforms : zeros.data(), out_tokens));
+  GG_CUDA(e, cudaMemcpyAsync(m.logits, e->bd_logits, 4 * (size_t)m.V, cudaMemcpyDeviceToDevice, e->stream));
+  GG_CUDA(e, cudaMemcpyAsync(m.dbg_hidden, e->pf_hidden, 4 * (size_t)m.H, cudaMemcpyDeviceToDevice, e->stream));
+  GG_CUDA(e, cudaStreamSynchronize(e->stream));
+  e->last_hidden_seq = seq;
   return GG_OK;
 }
 
@@ -878,6 +1007,8 @@ extern "C" int gg_prefill(gg_engine* e, int seq, const int32_t* ids, int n, int 
     return fail(e, GG_E_ARG, "positions %d..%d exceed context %d", start_pos, start_pos + n - 1, e->cfg.context_length);
   for (int i = 0; i < n; i++)
     if (ids[i] < 0 || ids[i] >= e->cfg.vocab_size) return fail(e, GG_E_ARG, "token id %d out of range", ids[i]);
+  if (e->kv8 && start_pos > e->kv8_len[seq])
+    return fail(e, GG_E_ARG, "position %d is beyond the %d tokens of slot %d (the 8-bit cache is written in order)", start_pos, e->kv8_len[seq], seq);
   if (e->ids_cap < n) {
     if (e->d_ids) cudaFree(e->d_ids);
     e->d_ids = nullptr;
@@ -895,6 +1026,7 @@ extern "C" int gg_prefill(gg_engine* e, int seq, const int32_t* ids, int n, int 
     GG_CUDA(e, cudaEventRecord(e->ev1, e->stream));
     GG_TRY(finish(e, nullptr));
     e->last_hidden_seq = seq;
+    if (e->kv8) e->kv8_len[seq] = start_pos + n;
     return GG_OK;
   }
   GGState s = base_inputs(e, seq, GG_RUN_LAYERS | GG_PREFILL_ADVANCE);
@@ -930,6 +1062,7 @@ extern "C" int gg_step(gg_engine* e, int seq, int32_t token, int pos, const gg_s
   if (!out_token) return fail(e, GG_E_ARG, "null out_token");
   if (token < 0 || token >= e->cfg.vocab_size) return fail(e, GG_E_ARG, "token %d out of range", token);
   if (pos < 0 || pos >= e->cfg.context_length) return fail(e, GG_E_ARG, "pos %d out of range", pos);
+  if (e->kv8) return kv8_decode(e, seq, token, pos, 1, sp, &uniform, out_token);
   GGState s = base_inputs(e, seq, GG_RUN_LAYERS | GG_RUN_LM | GG_RUN_SAMPLE);
   s.token = token;
   s.pos = pos;
@@ -951,6 +1084,10 @@ extern "C" int gg_decode(gg_engine* e, int seq, int32_t token, int pos, int n, c
   if (n <= 0 || !out_tokens) return fail(e, GG_E_ARG, "bad n / out_tokens");
   if (token < 0 || token >= e->cfg.vocab_size) return fail(e, GG_E_ARG, "token %d out of range", token);
   if (pos < 0 || pos + n > e->cfg.context_length) return fail(e, GG_E_ARG, "positions %d..%d exceed context", pos, pos + n - 1);
+  if (e->kv8) {
+    if (sp && sp->temperature != 0.0 && !uniforms) return fail(e, GG_E_ARG, "uniforms required when temperature > 0");
+    return kv8_decode(e, seq, token, pos, n, sp, uniforms, out_tokens);
+  }
   if (e->ring_cap < n) {
     if (e->d_ring) cudaFree(e->d_ring);
     if (e->h_ring) cudaFreeHost(e->h_ring);
@@ -1000,6 +1137,7 @@ extern "C" int gg_get_logits(gg_engine* e, float* out) {
 extern "C" int gg_get_hidden(gg_engine* e, float* out) {
   GG_TRY(ready(e, 0));
   if (!out) return fail(e, GG_E_ARG, "null out");
+  if (e->kv8) return fail(e, GG_E_STATE, "the normed hidden state is not kept with an 8-bit KV cache");
   GG_CUDA(e, cudaMemcpyAsync(out, e->md.dbg_normed, 4 * (size_t)e->md.H, cudaMemcpyDeviceToHost, e->stream));
   GG_CUDA(e, cudaStreamSynchronize(e->stream));
   return GG_OK;
@@ -1009,6 +1147,20 @@ extern "C" int gg_get_kv(gg_engine* e, int seq, int layer, int pos, int which, f
   GG_TRY(ready(e, seq));
   if (!out || layer < 0 || layer >= e->cfg.num_layers || pos < 0 || pos >= e->cfg.context_length)
     return fail(e, GG_E_ARG, "bad layer/pos");
+  if (e->kv8) {
+    const gg_kv8_cache kc = kv8_cache(e, layer);
+    const int NKH = kc.kv_heads, HD = kc.head_dim, blk = seq * e->kv8_blocks + pos / KV8_BLOCK;
+    std::vector<int8_t> codes((size_t)NKH * HD);
+    std::vector<float> scale(NKH);
+    for (int h = 0; h < NKH; h++)
+      GG_CUDA(e, cudaMemcpyAsync(codes.data() + (size_t)h * HD,
+                                 static_cast<const uint8_t*>(which ? kc.v_codes : kc.k_codes) + (((size_t)blk * NKH + h) * KV8_BLOCK + pos % KV8_BLOCK) * HD,
+                                 HD, cudaMemcpyDeviceToHost, e->stream));
+    GG_CUDA(e, cudaMemcpyAsync(scale.data(), (which ? kc.v_scale : kc.k_scale) + (size_t)blk * NKH, 4 * (size_t)NKH, cudaMemcpyDeviceToHost, e->stream));
+    GG_CUDA(e, cudaStreamSynchronize(e->stream));
+    for (int i = 0; i < NKH * HD; i++) out[i] = (float)codes[i] * scale[i / HD];
+    return GG_OK;
+  }
   const uint8_t* base = which ? e->md.vcache : e->md.kcache;
   const int es = e->md.kv_es, KV = e->md.KV;
   size_t off = ((size_t)seq * e->md.kv_seq_stride + ((size_t)layer * e->md.CTX + pos) * KV) * es;
@@ -1156,6 +1308,19 @@ extern "C" int gg_seen_add(gg_engine* e, int seq, const int32_t* ids, int n) {
 
 extern "C" int gg_reset_kv(gg_engine* e, int seq) {
   GG_TRY(ready(e, seq));
+  if (e->kv8) {
+    for (int l = 0; l < e->cfg.num_layers; l++) {
+      const gg_kv8_cache kc = kv8_cache(e, l);
+      const size_t per = (size_t)e->kv8_blocks * kc.kv_heads, n = per * KV8_BLOCK * kc.head_dim;
+      GG_CUDA(e, cudaMemsetAsync(static_cast<uint8_t*>(kc.k_codes) + seq * n, 0, n, e->stream));
+      GG_CUDA(e, cudaMemsetAsync(static_cast<uint8_t*>(kc.v_codes) + seq * n, 0, n, e->stream));
+      GG_CUDA(e, cudaMemsetAsync(kc.k_scale + seq * per, 0, 4 * per, e->stream));
+      GG_CUDA(e, cudaMemsetAsync(kc.v_scale + seq * per, 0, 4 * per, e->stream));
+    }
+    e->kv8_len[seq] = 0;
+    GG_CUDA(e, cudaStreamSynchronize(e->stream));
+    return GG_OK;
+  }
   size_t n = e->md.kv_seq_stride * e->md.kv_es;
   GG_CUDA(e, cudaMemsetAsync(e->md.kcache + (size_t)seq * n, 0, n, e->stream));
   GG_CUDA(e, cudaMemsetAsync(e->md.vcache + (size_t)seq * n, 0, n, e->stream));
@@ -1313,6 +1478,7 @@ extern "C" int gg_destroy(gg_engine* e) {
   if (e->lin_x) cudaFree(e->lin_x);
   if (e->lin_tiles) cudaFree(e->lin_tiles);
   if (e->lin_y) cudaFree(e->lin_y);
+  if (e->kv8_ws) cudaFree(e->kv8_ws);
   if (e->ev0) cudaEventDestroy(e->ev0);
   if (e->ev1) cudaEventDestroy(e->ev1);
   if (e->stream) cudaStreamDestroy(e->stream);

@@ -918,6 +918,51 @@ __global__ void __launch_bounds__(PF_THREADS) pf_geglu_kernel(const float* __res
 
 // RoPE table: (cos, sin) of pos * freq_i, freq_i = 1 / theta^(2i/HD), the same f32 expressions
 // the shader evaluates per step (shaders.ts:420-467).
+// One warp per head of a row (grid.x = rows): the planes' sum in plane order, q and k divided by
+// their head's rms. Bound by the planes' bytes; the row stays in registers between sum and norm.
+__global__ void __launch_bounds__(PF_THREADS)
+    pf_qkv_norm_kernel(const float* __restrict__ part, int splits, long long plane, const float* __restrict__ q_norm,
+                       const float* __restrict__ k_norm, int NQH, int NKH, int HD, float eps, float* __restrict__ out) {
+  pdl_trigger();
+  pdl_wait();  // before touching any buffer shared with the other kernels of the chain
+  constexpr int NJ = 8;  // 32 * 8 values of a head at most
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = NQH + 2 * NKH;
+  for (int h = warp; h < heads; h += PF_THREADS / 32) {
+    const long long o = ((long long)blockIdx.x * heads + h) * HD;
+    float v[NJ], ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const int i = lane + 32 * j;
+      v[j] = i < HD ? sum_planes(part, splits, plane, o + i) : 0.f;
+      ss += v[j] * v[j];
+    }
+    const float* w = h < NQH ? q_norm : h < NQH + NKH ? k_norm : nullptr;
+    const float rms = w ? sqrtf(warp_sum(ss) / (float)HD + eps) : 1.f;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      const int i = lane + 32 * j;
+      if (i < HD) out[o + i] = w ? v[j] * w[i] / rms : v[j];
+    }
+  }
+}
+
+__global__ void pf_kv8_rows_kernel(const int32_t* __restrict__ seqs, const int32_t* __restrict__ pos, int seq, int p0, int T,
+                                   int blocks, PfKv8Rows r) {
+  pdl_trigger();
+  pdl_wait();  // before touching any buffer shared with the other kernels of the chain
+  const int n = seqs ? T : 1;  // requests
+  const long long i0 = blockIdx.x * (long long)blockDim.x + threadIdx.x, step = (long long)gridDim.x * blockDim.x;
+  for (long long i = i0; i < T; i += step) {
+    const int p = seqs ? pos[i] : p0 + (int)i;
+    r.positions[i] = p;
+    r.slots[i] = (seqs ? seqs[i] : seq) * blocks * 16 + p;
+    if (seqs) r.lens[i] = p + 1;
+  }
+  for (long long i = i0; i <= n; i += step) r.cu_rows[i] = seqs ? (int)i : (int)i * T;
+  if (!seqs && i0 == 0) r.lens[0] = p0 + T;
+  for (long long i = i0; i < (long long)n * blocks; i += step) r.table[i] = (seqs ? seqs[i / blocks] : seq) * blocks + (int)(i % blocks);
+}
+
 __global__ void pf_rope_table_kernel(float theta, int HD, int ctx, float2* out) {
   const int half = HD / 2;
   for (int idx = blockIdx.x * blockDim.x + threadIdx.x; idx < ctx * half; idx += gridDim.x * blockDim.x) {
@@ -949,6 +994,21 @@ cudaError_t pf_addnorm(const float* part, int splits, long long plane, const flo
   const int threads = ((H / 4) + 31) / 32 * 32;
   return launch_pdl(pf_addnorm_kernel, dim3(T), dim3(threads), 0, s, part, splits, plane, w_post, resid_in, resid_out,
                     w_norm, thi, tlo, H, eps);
+}
+
+cudaError_t pf_qkv_norm(const float* part, int splits, long long plane, const float* q_norm, const float* k_norm, int T,
+                        int NQH, int NKH, int HD, float eps, float* out, cudaStream_t s) {
+  if (T <= 0 || HD > 256) return cudaErrorInvalidValue;
+  return launch_pdl(pf_qkv_norm_kernel, dim3(T), dim3(PF_THREADS), 0, s, part, splits, plane, q_norm, k_norm, NQH, NKH,
+                    HD, eps, out);
+}
+
+cudaError_t pf_kv8_rows(const int32_t* seqs, const int32_t* pos, int seq, int p0, int T, int blocks, const PfKv8Rows& r,
+                        cudaStream_t s) {
+  if (T <= 0) return cudaErrorInvalidValue;
+  const long long n = seqs ? (long long)T * blocks : T > blocks ? T : blocks;
+  return launch_pdl(pf_kv8_rows_kernel, dim3((unsigned)std::min((n + 255) / 256, 148ll)), dim3(256), 0, s, seqs, pos, seq,
+                    p0, T, blocks, r);
 }
 
 cudaError_t pf_qk_rope_store(const float* part, int splits, long long plane, const float* q_norm,

@@ -33,6 +33,21 @@ cudaError_t pf_qk_rope_store(const float* part, int splits, long long plane, con
                              const float* k_norm, const float2* rope, int T, int p0, int NQH, int NKH, int HD, float eps,
                              float* q_out, void* kc, void* vc, bool kv16, uint8_t* split, int ctx, cudaStream_t s);
 
+// ---- 8-bit KV cache (GG_FLAG_KV_Q8): the rows of a step for the operators of gemma_b200.h
+
+// The q/k/v planes summed, q and k per-head rmsNorm'd, as f32 rows [T][NQH + 2 NKH][HD] (RoPE, the
+// cache write and the attention are gg_rope, gg_kv8_append and gg_kv8_attention on views of them).
+cudaError_t pf_qkv_norm(const float* part, int splits, long long plane, const float* q_norm, const float* k_norm, int T,
+                        int NQH, int NKH, int HD, float eps, float* out, cudaStream_t s);
+// Positions and cache slots of T rows, and the requests they belong to. seqs == nullptr: one request,
+// KV slot `seq`, positions p0..p0 + T - 1; else row t is KV slot seqs[t] at pos[t]. KV slot s owns the
+// blocks s * blocks .. s * blocks + blocks - 1 of 16 tokens.
+struct PfKv8Rows {
+  int32_t *positions, *slots, *cu_rows, *lens, *table;
+};
+cudaError_t pf_kv8_rows(const int32_t* seqs, const int32_t* pos, int seq, int p0, int T, int blocks, const PfKv8Rows& r,
+                        cudaStream_t s);
+
 // Causal attention of the T queries (q as written by pf_qk_rope_store) at positions
 // p0..p0+T-1 over cache rows 0..p0+t
 // (shaders.ts:229-325), output written as activation tiles of width NQH*HD. `part` is scratch

@@ -151,8 +151,8 @@ class GemmaEngine:
 
 def create_gemma_engine(model: str = "synthetic:1b", on_progress=None, context_length: int | None = None,
                         device: int = 0, random=None, kv_dtype: str = "f32", spec: bool = False) -> GemmaEngine:
-    """``createGemmaEngine`` (src/index.ts:34-38). ``kv_dtype`` ("f32" as the reference, or
-    "bf16") and ``spec`` (Gemma 3's 512-position window and local theta 1e4, off as in the
+    """``createGemmaEngine`` (src/index.ts:34-38). ``kv_dtype`` ("f32" as the reference,
+    "bf16" or "q8") and ``spec`` (Gemma 3's 512-position window and local theta 1e4, off as in the
     reference) are options the reference does not have."""
     return GemmaEngine(model=model, on_progress=on_progress, context_length=context_length, device=device,
                        random=random, kv_dtype=kv_dtype, spec=spec)
