@@ -433,6 +433,27 @@ def test_attend_prompts(code, dtype, rows, lens, window, D, H, G, B):
     check_attend(rng, rows, lens, H * G, *a, code, dtype, window=window)
 
 
+@pytest.mark.parametrize("code, dtype, D, rows, lens, window", [
+    ("int8", "f32", 128, [40, 9], [5000, 2100], 0), ("e4m3", "bf16", 64, [33, 1], [3001, 9000], 0), ("int8", "f16", 256, [34], [2500], 0),
+    ("int8", "bf16", 128, [70], [6000], 3000), ("e4m3", "f32", 256, [20, 3], [1100, 4500], 2000)])
+def test_attend_long(code, dtype, D, rows, lens, window):
+    """Keys over many tiles, several batches of block ids and, for few rows, many steps of a warp; several key ranges."""
+    rng = np.random.default_rng(D + sum(lens))
+    a = make_batch(rng, rows, lens, 16 if D == 256 else 64, 1, D, code)
+    check_attend(rng, rows, lens, 4, *a, code, dtype, window=window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attend_many_requests(dtype):
+    """More requests than one pass of a CTA's prefix sums takes, many of them without rows or keys."""
+    rng = np.random.default_rng(31)
+    n = 1300
+    rows = [int(x) for x in rng.choice([0, 1, 1, 2], n)]
+    lens = [int(x) if x > 3 else int(rows[i] and x) for i, x in enumerate(rng.integers(0, 60, n))]
+    a = make_batch(rng, rows, lens, 16, 1, 32, "int8")
+    check_attend(rng, rows, lens, 3, *a, "int8", dtype)
+
+
 def test_attend_bad_pages():
     """Block ids outside the cache hide their keys; a request with no valid block gives zeros."""
     rng = np.random.default_rng(1)

@@ -218,17 +218,11 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
   int id_even = load_id(lane), id_odd = load_id(32 + lane);  // block ids of an even and of an odd batch of 32 steps, one step per lane
   // the warp's query rows, fetched while the ids are
   constexpr int QR = RT / KV8_WARPS, QP = (HD / 4 + 31) / 32;
-  float4 qv[QR][QP];
-#pragma unroll
-  for (int j = 0; j < QR; j++) {
-    const int row = warp + j * KV8_WARPS, it = base + row;
-    const long long qi = (long long)(sq.row0 + it / a.group) * a.q_row + (long long)(h * a.group + it % a.group) * a.q_head;
-#pragma unroll
-    for (int p = 0; p < QP; p++) {
-      const int d = 4 * (lane + 32 * p);
-      qv[j][p] = row < nitems && d < a.hd ? load_elem4(a.q, a.q_type, qi + d, a.q_vec) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  }
+  uint4 qv[QR][QP];
+  load_raw4(qv, a.q, a.q_type, a.q_vec, [&](int j, int p) {
+    const int row = warp + j * KV8_WARPS, it = base + row, tok = it / a.group, d = 4 * (lane + 32 * p);
+    return row < nitems && d < a.hd ? (long long)(sq.row0 + tok) * a.q_row + (long long)(h * a.group + it - tok * a.group) * a.q_head + d : -1ll;
+  });
   constexpr int W = HD / 16;  // 16-byte words of a key
   const int k_lane = lane / W, w_lane = lane % W;  // (a warp copies 32 / W keys at a time)
   const bool w_in = w_lane * 16 < a.hd;
@@ -262,10 +256,11 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
   for (int j = 0; j < QR; j++) {
     const int row = warp + j * KV8_WARPS;
     const bool live = row < nitems;
-    float4 (&v)[QP] = qv[j];
+    float4 v[QP];
     uint32_t top = 0;
 #pragma unroll
     for (int p = 0; p < QP; p++) {
+      v[p] = widen_raw4(qv[j][p], a.q_type, a.q_vec);
       top = max(max(top, __float_as_uint(v[p].x) & 0x7fffffffu), __float_as_uint(v[p].y) & 0x7fffffffu);
       top = max(max(top, __float_as_uint(v[p].z) & 0x7fffffffu), __float_as_uint(v[p].w) & 0x7fffffffu);
     }
@@ -508,6 +503,18 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
   }
 }
 
+// Where the parts of a row stand: of many rows its key ranges, of few rows the CTAs of its unit.
+struct Kv8Parts {
+  int n;
+  long long first, step;
+};
+GG_DEV Kv8Parts kv8_parts(const Kv8Args& a, const Kv8Seq& sq, int s, int tok, int hq) {
+  if (!a.pre) return {a.splits, ((long long)(sq.row0 + tok) * a.kv_heads * a.group + hq) * a.splits, 1};
+  const int RT = a.tile_rows, item = tok * a.group + hq % a.group;
+  const Kv8Line ln = kv8_line(a, sq, RT);
+  const int n = (ln.steps + a.pre[a.seqs] - 1) / a.pre[a.seqs];
+  return {n, ((long long)a.pre[s] + ((hq / a.group) * ln.tiles + item / RT) * n) * RT + item % RT, RT};
+}
 // One CTA per (request, token, query head): the results of the key ranges joined. Bound by latency
 // (a few KB per CTA), so the ranges are spread over the threads: `lanes` threads hold four dims each
 // and MERGE_THREADS / lanes of them share the ranges; every thread has its loads in flight at once.
@@ -527,18 +534,10 @@ __global__ void __launch_bounds__(MERGE_THREADS) gg_kv8_merge_kernel(const Kv8Ar
   const Kv8Seq sq = kv8_seq(a, x);
   if (tok >= sq.n) return;
   const long long ri = sq.row0 + tok;
-  // the parts of this row: many rows, its key ranges; few rows, the CTAs of its unit
-  int nparts = a.splits;
-  long long p0 = (ri * heads + hq) * a.splits, pstep = 1;
-  if (a.pre) {
-    const int RT = a.tile_rows, item = tok * a.group + hq % a.group;
-    const Kv8Line ln = kv8_line(a, sq, RT);
-    nparts = (ln.steps + a.pre[a.seqs] - 1) / a.pre[a.seqs];
-    if (nparts == 1) return;  // finished by its CTA
-    p0 = ((long long)a.pre[x] + ((hq / a.group) * ln.tiles + item / RT) * nparts) * RT + item % RT;
-    pstep = RT;
-  }
-  const auto at = [&](int z) { return p0 + z * pstep; };
+  const Kv8Parts pt = kv8_parts(a, sq, x, tok, hq);
+  const int nparts = pt.n;
+  if (a.pre && nparts == 1) return;  // finished by its CTA
+  const auto at = [&](int z) { return pt.first + z * pt.step; };
   float r = KV8_NEG;
   for (int z = t; z < nparts; z += MERGE_THREADS) r = fmaxf(r, a.part_ml[at(z)].x);
   const int lanes = a.hd <= 64 ? 16 : a.hd <= 128 ? 32 : 64, parts = MERGE_THREADS / lanes;
@@ -579,6 +578,40 @@ __global__ void __launch_bounds__(MERGE_THREADS) gg_kv8_merge_kernel(const Kv8Ar
   const float inv = l == 0.f ? 0.f : 1.f / l;
   store_elem4(a.out, a.q_type, ri * a.o_row + (long long)hq * a.o_head + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), a.o_vec);
   if (t == 0 && a.lse) a.lse[ri * heads + hq] = l == 0.f ? -INFINITY : (r + log2f(l)) * 0.6931471805599453f;
+}
+
+// The same by one warp, for rows by the thousand with a few parts each: bound by the parts' bytes.
+__global__ void __launch_bounds__(MERGE_THREADS) gg_kv8_merge_rows_kernel(const Kv8Args a) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, heads = a.kv_heads * a.group;
+  long long x = (long long)blockIdx.x * (MERGE_THREADS / 32) + (threadIdx.x >> 5);
+  const int hq = (int)(x % heads);
+  x /= heads;
+  const int tok = (int)(x % a.merge_tokens);
+  x /= a.merge_tokens;
+  if (x >= a.seqs) return;
+  const Kv8Seq sq = kv8_seq(a, (int)x);
+  if (tok >= sq.n) return;
+  const long long ri = sq.row0 + tok, p0 = (ri * heads + hq) * a.splits;
+  float r = KV8_NEG, l = 0.f;
+  for (int z = 0; z < a.splits; z++) r = fmaxf(r, a.part_ml[p0 + z].x);
+  for (int z = 0; z < a.splits; z++) l = fmaf(ex2(a.part_ml[p0 + z].x - r), a.part_ml[p0 + z].y, l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  for (int d = 4 * lane; d < a.hd; d += 128) {
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int z = 0; z < a.splits; z++) {
+      const float f = ex2(a.part_ml[p0 + z].x - r);
+      const float4 y = *reinterpret_cast<const float4*>(a.part_o + (p0 + z) * a.hd + d);
+      v.x = fmaf(f, y.x, v.x);
+      v.y = fmaf(f, y.y, v.y);
+      v.z = fmaf(f, y.z, v.z);
+      v.w = fmaf(f, y.w, v.w);
+    }
+    store_elem4(a.out, a.q_type, ri * a.o_row + (long long)hq * a.o_head + d, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv), a.o_vec);
+  }
+  if (lane == 0 && a.lse) a.lse[ri * heads + hq] = l == 0.f ? -INFINITY : (r + log2f(l)) * 0.6931471805599453f;
 }
 
 template <int HD, int CODE, bool HILO, int NT>
@@ -641,7 +674,7 @@ static Kv8Plan kv8_plan(const gg_kv8_cache& c, const gg_kv8_attention_call& b) {
     const int tile = kv8_prompt_tile(c.head_dim);
     p.row_tiles = (int)((items + tile - 1) / tile);
     const long long units = (long long)b.seqs * c.kv_heads * p.row_tiles, n = steps(tile), most = (n + 31) / 32;
-    long long splits = (148 + units - 1) / units;
+    long long splits = 148 / units;
     if (splits > most) splits = most;
     if (splits < 1) splits = 1;
     p.split_steps = (int)((n + splits - 1) / splits);
@@ -733,6 +766,11 @@ extern "C" int gg_kv8_attention(const gg_kv8_cache* c, const gg_kv8_attention_ca
   cudaError_t r = cudaSuccess;
   const auto merge = [&](int tokens) {
     a.merge_tokens = tokens < b.max_rows ? tokens : b.max_rows;
+    const long long n = (long long)b.seqs * a.merge_tokens * b.q.heads;
+    // A CTA a row while they fit the GPU at once (148 SMs x 8). 35,776 rows of two parts took 102 us so;
+    // a warp a row takes 9.7 us for 10,176 of them, but a chain of loads as long as the parts for a few.
+    if (!a.pre && n > 148 * 8)
+      return launch_pdl(gg_kv8_merge_rows_kernel, dim3((unsigned)((n + MERGE_THREADS / 32 - 1) / (MERGE_THREADS / 32))), dim3(MERGE_THREADS), 0, s, a);
     return launch_pdl(gg_kv8_merge_kernel, dim3((unsigned)((long long)b.seqs * a.merge_tokens * b.q.heads)), dim3(MERGE_THREADS), 0, s, a);
   };
   const auto parts = [&](size_t offset, size_t n) {

@@ -15,6 +15,11 @@
 // both products twice, for the hi and the lo half of q and of the weights, into the same
 // accumulators. The running maximum r is kept an integer and raised only when a weight would pass
 // 2^KV8_SLACK, so the accumulator in TMEM is rarely rescaled (first tile, then now and then).
+//
+// The tensor cores cut the f32 sums they hold: measured, a sum loses 6e-10 of itself a key and
+// product, always downwards (1.1e-5 after 8192 keys with both products of f32 queries). For f16 and
+// bf16 outputs that stays below their own rounding up to 2^18 keys. For f32 ones O is added to an f32
+// row in memory (the row of the output itself) every PROMPT_FLUSH tiles and starts again from zero.
 #include "gg_kv8.h"
 #include "gg_tc.cuh"
 
@@ -137,6 +142,8 @@ GG_DEV float max3(float a, float b, float c) {
   return d;
 }
 
+constexpr int PROMPT_FLUSH = 64;  // tiles of 64 keys
+
 // Wait for an mbarrier phase; after two seconds (or when another warp gave up) sets *abort and
 // returns false: the CTA then drains its MMAs and leaves NaN in its rows.
 GG_DEV bool prompt_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
@@ -169,9 +176,10 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
   float4* meta = reinterpret_cast<float4*>(sm + S::OFF_META);  // per 16-key group: ks, log2 vs, 1 / vs
   float* s_mul = reinterpret_cast<float*>(sm + S::OFF_MUL);
   uint64_t* kfull = reinterpret_cast<uint64_t*>(sm + S::OFF_BAR);
-  // kfull, vfull, done: by ring stage; sfull: by the key tile's parity; pfull: [query tile][parity]
-  uint64_t *vfull = kfull + 4, *done = kfull + 8, *sfull = kfull + 12, *pfull = kfull + 14, *drain = kfull + 18, *kdone = kfull + 19;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 21);
+  // kfull, vfull, kdone: by ring stage; sfull, pfull: [query tile][parity of the key tile]; odone:
+  // [query tile][key tile mod 4], so that a parity always tells a phase from the one before
+  uint64_t *vfull = kfull + 4, *sfull = kfull + 8, *pfull = kfull + 12, *odone = kfull + 16, *kdone = kfull + 24, *drain = kfull + 26;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 27);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   constexpr int MMA_WARP = S::SOFT_WARPS + S::CONV_WARPS;
@@ -200,13 +208,12 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
       for (int i = 0; i < 4; i++) {
         mbar_init(&kfull[i], S::CONV_WARPS);
         mbar_init(&vfull[i], S::CONV_WARPS);
-        mbar_init(&done[i], 1);
+        mbar_init(&odone[i], 1);
+        mbar_init(&odone[4 + i], 1);
         mbar_init(&pfull[i], 4);
-      }
-      for (int i = 0; i < 2; i++) {
         mbar_init(&sfull[i], 1);
-        mbar_init(&kdone[i], 1);
       }
+      for (int i = 0; i < 2; i++) mbar_init(&kdone[i], 1);
       mbar_init(drain, 1);
       *abort = 0;
       mbar_fence_init();
@@ -221,39 +228,46 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
 
   // ---- query rows -> f16 tiles, each row times its own power of two
   if (nt) {
-    for (int row = warp; row < NQ * 128; row += S::THREADS / 32) {
-      const bool live = row < nitems;
-      const int it = base + row;
-      const long long qi = live ? (long long)(sq.row0 + it / a.group) * a.q_row + (long long)(h * a.group + it % a.group) * a.q_head : 0;
-      constexpr int PER = (HD / 4 + 31) / 32;
-      float4 v[PER];
-      uint32_t top = 0;
+    // (a warp takes QB rows at a time, all their loads in flight together)
+    constexpr int WARPS = S::THREADS / 32, QB = HD == 256 ? 4 : 8, PER = (HD / 4 + 31) / 32;
+    for (int row0 = warp; row0 < NQ * 128; row0 += WARPS * QB) {
+      uint4 raw[QB][PER];
+      load_raw4(raw, a.q, a.q_type, a.q_vec, [&](int j, int p) {
+        const int row = row0 + j * WARPS, it = base + row, tok = it / a.group, d = 4 * (lane + 32 * p);
+        return row < nitems && d < a.hd ? (long long)(sq.row0 + tok) * a.q_row + (long long)(h * a.group + it - tok * a.group) * a.q_head + d : -1ll;
+      });
 #pragma unroll
-      for (int p = 0; p < PER; p++) {
-        const int d = 4 * (lane + 32 * p);
-        v[p] = live && d < a.hd ? load_elem4(a.q, a.q_type, qi + d, a.q_vec) : make_float4(0.f, 0.f, 0.f, 0.f);
-        top = max(max(top, __float_as_uint(v[p].x) & 0x7fffffffu), __float_as_uint(v[p].y) & 0x7fffffffu);
-        top = max(max(top, __float_as_uint(v[p].z) & 0x7fffffffu), __float_as_uint(v[p].w) & 0x7fffffffu);
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      const int ex = min(max((int)(top >> 23) - 127, -100), 127);
-      const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
-      if (lane == 0) s_mul[row] = __uint_as_float((uint32_t)(ex - 14 + 127) << 23) * a.scale_log2;
-      unsigned char* qt = sm + (row >> 7) * S::Q_BYTES;
-      const int r = row & 127;
+      for (int j = 0; j < QB; j++) {
+        const int row = row0 + j * WARPS;
+        if (row >= NQ * 128) break;
+        float4 v[PER];
+        uint32_t top = 0;
 #pragma unroll
-      for (int p = 0; p < PER; p++) {
-        const int d = 4 * (lane + 32 * p);
-        if (d >= HD) break;
-        uint2* dst = reinterpret_cast<uint2*>(qt + (d >> 6) * (128 * 128) + sw128_offset(r, d & 63));
-        if constexpr (HILO) {
-          uint2 hi, lo;
-          split_f16(v[p].x * up, v[p].y * up, hi.x, lo.x);
-          split_f16(v[p].z * up, v[p].w * up, hi.y, lo.y);
-          *dst = hi;
-          *reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(dst) + S::Q_BYTES / 2) = lo;
-        } else {
-          *dst = make_uint2(half2_bits(v[p].x * up, v[p].y * up), half2_bits(v[p].z * up, v[p].w * up));
+        for (int p = 0; p < PER; p++) {
+          v[p] = widen_raw4(raw[j][p], a.q_type, a.q_vec);
+          top = max(max(top, __float_as_uint(v[p].x) & 0x7fffffffu), __float_as_uint(v[p].y) & 0x7fffffffu);
+          top = max(max(top, __float_as_uint(v[p].z) & 0x7fffffffu), __float_as_uint(v[p].w) & 0x7fffffffu);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        const int ex = min(max((int)(top >> 23) - 127, -100), 127);
+        const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
+        if (lane == 0) s_mul[row] = __uint_as_float((uint32_t)(ex - 14 + 127) << 23) * a.scale_log2;
+        unsigned char* qt = sm + (row >> 7) * S::Q_BYTES;
+        const int r = row & 127;
+#pragma unroll
+        for (int p = 0; p < PER; p++) {
+          const int d = 4 * (lane + 32 * p);
+          if (d >= HD) break;
+          uint2* dst = reinterpret_cast<uint2*>(qt + (d >> 6) * (128 * 128) + sw128_offset(r, d & 63));
+          if constexpr (HILO) {
+            uint2 hi, lo;
+            split_f16(v[p].x * up, v[p].y * up, hi.x, lo.x);
+            split_f16(v[p].z * up, v[p].w * up, hi.y, lo.y);
+            *dst = hi;
+            *reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(dst) + S::Q_BYTES / 2) = lo;
+          } else {
+            *dst = make_uint2(half2_bits(v[p].x * up, v[p].y * up), half2_bits(v[p].z * up, v[p].w * up));
+          }
         }
       }
     }
@@ -350,12 +364,12 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         for (int j = 0; j < 2; j++) put_group((b + 1) * 64 + lane + 32 * j, nxt[j], sc[j]);
       // A stage is free once both products of the tile that had it are done; with few stages its K
       // is waited for, and handed back, by itself once the scores are.
-      if (i >= ST && !prompt_wait_warp(S::EARLY_K ? &kdone[st] : &done[st], par ^ 1, abort)) break;
+      if (i >= ST && !prompt_wait_warp(S::EARLY_K ? &kdone[st] : &odone[4 * (NQ - 1) + (i - ST) % 4], S::EARLY_K ? par ^ 1 : ((i - ST) >> 2) & 1, abort)) break;
       put(sm + S::OFF_K + st * S::KV_BYTES, rk);
       __syncwarp();
       if (lane == 0) mbar_arrive(&kfull[st]);
       fetch(a.kc, i + 1, b, rk);
-      if (S::EARLY_K && i >= ST && !prompt_wait_warp(&done[st], par ^ 1, abort)) break;
+      if (S::EARLY_K && i >= ST && !prompt_wait_warp(&odone[4 * (NQ - 1) + (i - ST) % 4], ((i - ST) >> 2) & 1, abort)) break;
       put(sm + S::OFF_V + st * S::KV_BYTES, rv);
       __syncwarp();
       if (lane == 0) mbar_arrive(&vfull[st]);
@@ -372,19 +386,18 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     const uint64_t qd = umma_desc_sw128(smem_u32(sm)), kd = umma_desc_sw128(smem_u32(sm + S::OFF_K));
     const uint64_t vd = umma_desc_sw128_mn(smem_u32(sm + S::OFF_V), KT * 128);
     // descriptors count 16-byte units; the address field does not overflow (227 KB of shared memory)
-    const auto scores = [&](int i) {  // S buffers = Q tiles x K tile i
+    const auto scores = [&](int q, int i) {  // S buffer = Q tile q x K tile i
+      const int buf = 2 * q + (i & 1);
       const uint64_t kb = kd + (uint32_t)(i % ST) * (S::KV_BYTES / 16);
 #pragma unroll
-      for (int q = 0; q < NQ; q++)
+      for (int part = 0; part < (HILO ? 2 : 1); part++)
 #pragma unroll
-        for (int part = 0; part < (HILO ? 2 : 1); part++)
-#pragma unroll
-          for (int k = 0; k < HD / 16; k++)
-            if (k < steps)
-              umma_f16_ss(tm + (2 * q + (i & 1)) * S::TMEM_S, qd + q * (S::Q_BYTES / 16) + part * (S::Q_BYTES / 32) + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2,
-                          kb + (k >> 2) * (KT * 128 / 16) + (k & 3) * 2, idesc_s, part > 0 || k > 0, on);
-      umma_commit_on(&sfull[i & 1], on);
-      if constexpr (S::EARLY_K) umma_commit_on(&kdone[i % ST], on);
+        for (int k = 0; k < HD / 16; k++)
+          if (k < steps)
+            umma_f16_ss(tm + buf * S::TMEM_S, qd + (uint32_t)q * (S::Q_BYTES / 16) + part * (S::Q_BYTES / 32) + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2,
+                        kb + (k >> 2) * (KT * 128 / 16) + (k & 3) * 2, idesc_s, part > 0 || k > 0, on);
+      umma_commit_on(&sfull[buf], on);
+      if (S::EARLY_K && q == NQ - 1) umma_commit_on(&kdone[i % ST], on);
     };
     const auto outputs = [&](int q, int i) {  // O tile q += P x V tile i
       const uint32_t d = tm + S::TMEM_O + q * HD, p = tm + (2 * q + (i & 1)) * S::TMEM_S;
@@ -393,21 +406,29 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
       for (int k = 0; k < KT / 16; k++)
 #pragma unroll
         for (int part = 0; part < (HILO ? 2 : 1); part++)
-          umma_f16_ts(d, p + part * 32 + k * 8, vb + k * (2048 / 16), idesc_o, i > 0 || k > 0 || part > 0, on);
+          umma_f16_ts(d, p + part * 32 + k * 8, vb + k * (2048 / 16), idesc_o, (HILO ? i % PROMPT_FLUSH != 0 : i > 0) || k > 0 || part > 0, on);
+      umma_commit_on(&odone[4 * q + (i & 3)], on);
     };
-    // A tile's scores are issued before the weights of the tile before are ready, so the softmax
-    // warps hardly wait for them; they overwrite the weights of two tiles before, whose product was
-    // issued earlier (the MMAs of one thread run in order). Each commit takes the tensor pipe as
-    // long as an MMA of N = 64 (62 cycles), hence only two or three of them for a tile.
-    bool ok = prompt_wait_warp(&kfull[0], 0, abort);
-    tc_fence_after();
-    if (ok) scores(0);
-    for (int i = 0; ok && i < tiles; i++) {
-      if (ST > 1 && i + 1 < tiles) {
-        if (!(ok = prompt_wait_warp(&kfull[(i + 1) % ST], ((i + 1) / ST) & 1, abort))) break;
+    // Scores run two key tiles ahead of their weights (one with a single ring stage), so that the
+    // softmax warps hardly wait for them. They overwrite the weights of two tiles before, once the
+    // product that reads those is complete (MMAs with different accumulators are not ordered); the
+    // other query tile's product covers that wait. Each commit takes the tensor pipe as long as an
+    // MMA of N = 64 (62 cycles), hence few of them.
+    bool ok = true;
+    const auto scores_of = [&](int i) {  // all query tiles, when K is there and the buffers are free
+      if (!prompt_wait_warp(&kfull[i % ST], (i / ST) & 1, abort)) return false;
+#pragma unroll
+      for (int q = 0; q < NQ; q++) {
+        if (i > 1 && !prompt_wait_warp(&odone[4 * q + (i - 2) % 4], ((i - 2) >> 2) & 1, abort)) return false;
         tc_fence_after();
-        scores(i + 1);
+        scores(q, i);
       }
+      return true;
+    };
+    constexpr int AHEAD = ST > 1 ? 2 : 1;
+    for (int i = 0; ok && i < AHEAD && i < tiles; i++) ok = scores_of(i);
+    for (int i = 0; ok && i < tiles; i++) {
+      if (AHEAD == 1 && i + 1 < tiles && !(ok = scores_of(i + 1))) break;
 #pragma unroll
       for (int q = 0; q < NQ; q++) {
         if (!(ok = prompt_wait_warp(&pfull[2 * q + (i & 1)], (i >> 1) & 1, abort))) break;
@@ -415,13 +436,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         tc_fence_after();
         outputs(q, i);
       }
-      if (!ok) break;
-      umma_commit_on(&done[i % ST], on);
-      if (ST == 1 && i + 1 < tiles) {  // one stage: the next K tile comes after this tile's products
-        if (!(ok = prompt_wait_warp(&kfull[0], (i + 1) & 1, abort))) break;
-        tc_fence_after();
-        scores(i + 1);
-      }
+      if (AHEAD == 2 && ok && i + 2 < tiles) ok = scores_of(i + 2);
     }
     if (!ok) {  // everything issued so far has finished before TMEM is freed
       umma_commit_on(drain, on);
@@ -443,9 +458,51 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     const float mul = nt ? s_mul[row] : 0.f;
     float r = KV8_NEG, l = 0.f;
     bool ok = true;
+    const long long ri = (long long)sq.row0 + tok, pi = (ri * heads + hq) * a.splits + split;
+    // f32: the row in memory that takes O now and then, and r as it was the last time
+    float* sum = nullptr;
+    float sum_r = KV8_NEG;
+    bool summed = false;
+    const int sum_vec = a.splits > 1 || a.o_vec;
+    if constexpr (HILO) sum = a.splits > 1 ? a.part_o + pi * a.hd : static_cast<float*>(a.out) + ri * a.o_row + (long long)hq * a.o_head;
+    // O's columns c .. c + 31 and what memory has of them
+    const auto gather = [&](int c, float keep, uint32_t (&v)[32]) {
+      tmem_ld32(to + c, v);
+      tmem_ld_done();
+      if (HILO && summed && live) {
+        const int n = min(32, a.hd - c);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+          if (e < n) {
+            const float4 y = sum_vec ? *reinterpret_cast<const float4*>(sum + c + e) : make_float4(sum[c + e], sum[c + e + 1], sum[c + e + 2], sum[c + e + 3]);
+            v[e] = __float_as_uint(fmaf(y.x, keep, __uint_as_float(v[e])));
+            v[e + 1] = __float_as_uint(fmaf(y.y, keep, __uint_as_float(v[e + 1])));
+            v[e + 2] = __float_as_uint(fmaf(y.z, keep, __uint_as_float(v[e + 2])));
+            v[e + 3] = __float_as_uint(fmaf(y.w, keep, __uint_as_float(v[e + 3])));
+          }
+      }
+    };
     for (int i = 0; i < nt; i++) {
+      if (HILO && i > 0 && i % PROMPT_FLUSH == 0) {
+        if (!(ok = prompt_wait_warp(&odone[4 * q + (i - 1) % 4], ((i - 1) >> 2) & 1, abort))) break;
+        tc_fence_after();
+        const float keep = ex2(sum_r - r);
+        for (int c = 0; c < a.hd; c += 32) {
+          uint32_t v[32];
+          gather(c, keep, v);
+          if (live) {
+            const int n = min(32, a.hd - c);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (e < n)
+                store_elem4(sum, GG_T_F32, c + e, make_float4(__uint_as_float(v[e]), __uint_as_float(v[e + 1]), __uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), sum_vec);
+          }
+        }
+        sum_r = r;
+        summed = true;
+      }
       const int buf = 2 * q + (i & 1);
-      if (!(ok = prompt_wait_warp(&sfull[i & 1], (i >> 1) & 1, abort))) break;
+      if (!(ok = prompt_wait_warp(&sfull[buf], (i >> 1) & 1, abort))) break;
       tc_fence_after();
       const uint32_t ts = tl + buf * S::TMEM_S;
       const int key0 = k00 + i * KT;
@@ -487,8 +544,8 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         const float nr = raise ? ceilf(top) : r;
         const float f = ex2(r - nr);  // 0 for the first keys of a row, else a power of two
         l *= f;
-        if (i > 0) {  // O is rescaled once the previous tile's product is in it
-          if (!(ok = prompt_wait_warp(&done[(i - 1) % ST], ((i - 1) / ST) & 1, abort))) break;
+        if (HILO ? i % PROMPT_FLUSH != 0 : i > 0) {  // O is rescaled once the previous tile's product is in it
+          if (!(ok = prompt_wait_warp(&odone[4 * q + (i - 1) % 4], ((i - 1) >> 2) & 1, abort))) break;
           tc_fence_after();
           for (int c = 0; c < a.hd; c += 32) {
             tmem_ld32(to + c, v[0]);
@@ -527,18 +584,17 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
       if (lane == 0) mbar_arrive(&pfull[buf]);
     }
     if (ok && nt) {
-      ok = prompt_wait_warp(&done[(nt - 1) % ST], ((nt - 1) / ST) & 1, abort);
+      ok = prompt_wait_warp(&odone[4 * q + (nt - 1) % 4], ((nt - 1) >> 2) & 1, abort);
       tc_fence_after();
     }
-    const long long ri = (long long)sq.row0 + tok, pi = (ri * heads + hq) * a.splits + split;
     l *= 1.f / KV8_WMUL;
+    const float keep = ex2(sum_r - r);
     const float nan = __uint_as_float(0x7fffffffu);
     const float inv = !ok ? nan : a.splits > 1 ? 1.f / KV8_WMUL : l == 0.f ? 0.f : (1.f / KV8_WMUL) / l;
     for (int c = 0; c < a.hd; c += 32) {
       uint32_t v[32];
       if (nt && ok) {
-        tmem_ld32(to + c, v);
-        tmem_ld_done();
+        gather(c, keep, v);
       } else {
 #pragma unroll
         for (int e = 0; e < 32; e++) v[e] = 0;
