@@ -350,7 +350,8 @@ int gg_kv8_append(const gg_kv8_cache* cache, const gg_kv8_append_call* call, voi
 /* Attention of the query rows of a ragged batch over the cache. Rows cu_rows[i] .. cu_rows[i + 1] - 1
  * are the last tokens of request i, whose cache holds lens[i] tokens in blocks table[i][...]; the row
  * at position p = lens[i] - (rows of i) + r sees the keys at max(0, p - window + 1) .. p (window 0:
- * from 0): o = sum softmax(scale q k) v; query head h reads key head h / (q heads / kv_heads). A row
+ * from 0): o = sum softmax(scale q k) v; query head h reads key head h / (q heads / kv_heads), at
+ * most 1024 to one. A row
  * that sees no key gives zeros. lse (f32, [rows][q heads], or NULL) receives ln sum exp(scale q k),
  * -inf for such a row. out has q's type. Scores, softmax and sums are held in f32.
  *   max_rows and max_len are at least every request's number of rows and length (of longer ones,

@@ -76,7 +76,7 @@ def test_append_rows_refused(lib, kw, word):
 @pytest.mark.parametrize("kw, qkw, okw, word", [
     (dict(table_stride=7), {}, {}, "table_stride 7"), (dict(seqs=-1), {}, {}, "seqs -1"), (dict(max_len=-1), {}, {}, "max_len"),
     (dict(lens=None), {}, {}, "null array"), ({}, dict(heads=6), dict(heads=6), "6 query heads over 4"), ({}, {}, dict(type=2), "another type"),
-    ({}, dict(type=5), {}, "q.type 5"), (dict(window=-1), {}, {}, "window"), (dict(scale=math.nan), {}, {}, "scale"),
+    ({}, dict(type=5), {}, "q.type 5"), ({}, dict(heads=4 * 1025), dict(heads=4 * 1025), "1024 query heads"), (dict(window=-1), {}, {}, "window"), (dict(scale=math.nan), {}, {}, "scale"),
     (dict(scale=math.inf), {}, {}, "scale"), (dict(seqs=1 << 20, rows=1 << 20, max_rows=1 << 20), {}, {}, "tiles")])
 def test_attention_refused(lib, kw, qkw, okw, word):
     c, call = cache(), attend(rows(**qkw), rows(**okw), **kw)

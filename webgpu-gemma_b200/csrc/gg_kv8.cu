@@ -694,6 +694,7 @@ static int kv8_check(const char* fn, const gg_kv8_cache* c, const gg_kv8_attenti
   if (b->q.type < GG_T_F32 || b->q.type > GG_T_F16) return ops_fail(GG_E_ARG, "%s: q.type %d is none of GG_T_*", fn, b->q.type);
   if (b->q.heads < 1 || b->q.heads > 65535 || b->q.heads % c->kv_heads)
     return ops_fail(GG_E_ARG, "%s: %d query heads over %d key heads", fn, b->q.heads, c->kv_heads);
+  if (b->q.heads / c->kv_heads > 1024) return ops_fail(GG_E_ARG, "%s: more than 1024 query heads to a key head", fn);
   if (b->seqs < 0 || b->rows < 0 || b->max_rows < 0 || b->max_len < 0)
     return ops_fail(GG_E_ARG, "%s: seqs %d, rows %d, max_rows %d, max_len %d out of range", fn, b->seqs, b->rows, b->max_rows, b->max_len);
   if (b->window < 0) return ops_fail(GG_E_ARG, "%s: window %d", fn, b->window);

@@ -229,12 +229,17 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
   // ---- query rows -> f16 tiles, each row times its own power of two
   if (nt) {
     // (a warp takes QB rows at a time, all their loads in flight together)
+    // token and head of a row within the tile: y / group for y < 1280 by a multiplication (a division
+    // a row was most of this loop's time)
+    const int tok0 = base / a.group, rem0 = base - tok0 * a.group;
+    const uint32_t gmagic = (1u << 22) / a.group + 1;
+    const long long q0 = (long long)(sq.row0 + tok0) * a.q_row + (long long)h * a.group * a.q_head;
     constexpr int WARPS = S::THREADS / 32, QB = HD == 256 ? 4 : 8, PER = (HD / 4 + 31) / 32;
     for (int row0 = warp; row0 < NQ * 128; row0 += WARPS * QB) {
       uint4 raw[QB][PER];
       load_raw4(raw, a.q, a.q_type, a.q_vec, [&](int j, int p) {
-        const int row = row0 + j * WARPS, it = base + row, tok = it / a.group, d = 4 * (lane + 32 * p);
-        return row < nitems && d < a.hd ? (long long)(sq.row0 + tok) * a.q_row + (long long)(h * a.group + it - tok * a.group) * a.q_head + d : -1ll;
+        const int row = row0 + j * WARPS, d = 4 * (lane + 32 * p), y = rem0 + row, tok = (int)(((uint32_t)y * gmagic) >> 22);
+        return row < nitems && d < a.hd ? q0 + tok * a.q_row + (long long)(y - tok * a.group) * a.q_head + d : -1ll;
       });
 #pragma unroll
       for (int j = 0; j < QB; j++) {
