@@ -71,10 +71,15 @@ namespace gg {
 //
 // One CTA: the whole plan is a few prefix sums over the requests (blocks given back, blocks taken,
 // new rows), so it is bound by the latency of its dependent steps -- lengths, scan, stack, table,
-// rows -- and not by its bytes. A scan covers PLAN_CHUNK requests in shared memory; blocks and
-// rows are then spread one per thread and find their request by a binary search of the scan, so
+// rows -- and not by its bytes. The sums of up to PLAN_CHUNK requests stand in shared memory; blocks
+// and rows are then spread one per thread and find their request by a binary search of them, so
 // that one long prompt among many single tokens costs no more than the tokens themselves. More
-// than PLAN_INLINE_ROWS rows are filled by gg_plan_rows_kernel over all SMs.
+// than PLAN_INLINE_ROWS rows are filled by gg_plan_rows_kernel over all SMs. Up to PLAN_CHUNK requests
+// keep their lengths in registers (gg_plan_kernel, 256 threads where that many requests have one
+// each: its barriers are cheaper); more go through the chunks three times (gg_plan_many_kernel).
+// The code runs once, so instruction fetches count: with its loops unrolled by four 1000 requests
+// with 32768 rows took 16.2 us, rolled and with warp reductions 11.4; 64 requests with one row each
+// take 2.9 us (6.1 with the chunked kernel), most of it three dependent rounds of loads.
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_CHUNK = 4096;
 constexpr int PLAN_PER = PLAN_CHUNK / PLAN_THREADS;
@@ -88,6 +93,7 @@ struct PlanScan {
 // Index i with pre[i] <= k < pre[i + 1] (pre ascending, n + 1 entries, pre[0] <= k < pre[n]).
 GG_DEV int find_segment(const int* pre, int n, int k) {
   int lo = 0, hi = n;
+#pragma unroll 1
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (pre[mid] <= k) lo = mid;
@@ -96,7 +102,7 @@ GG_DEV int find_segment(const int* pre, int n, int k) {
   return lo;
 }
 
-GG_DEV int plan_blocks_of(int len, int B) { return (int)(((long long)len + B - 1) / B); }
+GG_DEV int plan_blocks_of(int len, int B) { return len > 0 ? (int)((uint32_t)(len - 1) / (uint32_t)B) + 1 : 0; }
 
 // Exclusive prefix sums of the chunk's requests i0 .. i0 + n - 1. Called with a plan that passed
 // its checks: every sum fits 32 bits.
@@ -153,7 +159,129 @@ GG_DEV void plan_scan(const gg_block_plan& p, int i0, int n, PlanScan& sc) {
   __syncthreads();
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) gg_plan_kernel(const gg_block_plan p, int inline_rows) {
+// Sum over the warp of numbers from 0 to 2^50, in two halves.
+GG_DEV long long warp_add_long(long long v) {
+  return (long long)__reduce_add_sync(0xffffffffu, (uint32_t)v & 0xffffffu) + ((long long)__reduce_add_sync(0xffffffffu, (uint32_t)(v >> 24)) << 24);
+}
+
+template <int THREADS, int PER>
+__global__ void __launch_bounds__(THREADS) gg_plan_kernel(const gg_block_plan p, int inline_rows) {
+  constexpr int WARPS = THREADS / 32;
+  extern __shared__ __align__(16) unsigned char plan_smem[];
+  PlanScan& sc = *reinterpret_cast<PlanScan*>(plan_smem);
+  __shared__ long long s_long[3][WARPS];
+  __shared__ uint32_t s_int[3][WARPS];
+  __shared__ int s_bad[WARPS];
+  pdl_trigger();
+  pdl_wait();
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5, B = p.block_tokens, n = p.seqs;
+  int a[PER], b[PER], flags = 0;
+  uint32_t v[3][PER], sum[3] = {0, 0, 0};  // (these sums wrap only where the 64-bit ones refuse the plan)
+  long long tot[3] = {0, 0, 0};
+  const int count = *p.free_count;
+#pragma unroll
+  for (int k = 0; k < PER; k++) {
+    const int i = t * PER + k;
+    a[k] = i < n ? p.old_len[i] : 0;
+    b[k] = i < n ? p.new_len[i] : 0;
+  }
+#pragma unroll
+  for (int k = 0; k < PER; k++) {
+    const int ha = plan_blocks_of(max(a[k], 0), B), hb = plan_blocks_of(max(b[k], 0), B);
+    if (a[k] < 0 || b[k] < 0 || ha > p.max_blocks) flags |= GG_PLAN_BAD_LENGTH;
+    if (hb > p.max_blocks) flags |= GG_PLAN_TOO_LONG;
+    const long long d[3] = {max(ha - hb, 0), max(hb - ha, 0), max((long long)b[k] - a[k], 0ll)};
+#pragma unroll
+    for (int q = 0; q < 3; q++) {
+      tot[q] += d[q];
+      v[q][k] = (uint32_t)d[q];
+      sum[q] += v[q][k];
+    }
+  }
+  uint32_t inc[3];
+#pragma unroll
+  for (int q = 0; q < 3; q++) {
+    inc[q] = sum[q];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, inc[q], o);
+      if (lane >= o) inc[q] += u;
+    }
+    tot[q] = warp_add_long(tot[q]);
+    if (lane == 31) {
+      s_int[q][w] = inc[q];
+      s_long[q][w] = tot[q];
+    }
+  }
+  flags = __reduce_or_sync(0xffffffffu, flags);
+  if (lane == 0) s_bad[w] = flags;
+  __syncthreads();
+  uint32_t before[3];
+  flags = __reduce_or_sync(0xffffffffu, lane < WARPS ? s_bad[lane] : 0);
+#pragma unroll
+  for (int q = 0; q < 3; q++) {
+    before[q] = __reduce_add_sync(0xffffffffu, lane < w ? s_int[q][lane] : 0u);
+    tot[q] = warp_add_long(lane < WARPS ? s_long[q][lane] : 0);
+  }
+  if (count < 0 || count > p.free_capacity || count + tot[0] > p.free_capacity) flags |= GG_PLAN_BAD_STACK;
+  else if (tot[1] > count + tot[0]) flags |= GG_PLAN_NO_BLOCKS;
+  if (tot[2] > p.rows) flags |= GG_PLAN_NO_ROWS;
+  const int given = flags ? 0 : (int)tot[0], taken = flags ? 0 : (int)tot[1], total = flags ? 0 : (int)tot[2];
+  int* const dst[3] = {sc.give, sc.take, sc.rows};
+#pragma unroll
+  for (int q = 0; q < 3; q++) {
+    uint32_t run = before[q] + inc[q] - sum[q];
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+      const int i = t * PER + k;
+      if (i < n) {
+        dst[q][i] = (int)run;
+        if (q == 2) {
+          p.cu_rows[i] = flags ? 0 : (int)run;
+          p.lens[i] = flags ? a[k] : b[k];
+        }
+      }
+      run += v[q][k];
+    }
+  }
+  if (t == 0) {
+    *p.status = flags;
+    *p.free_count_out = flags ? count : count + given - taken;
+    p.cu_rows[n] = total;
+    sc.give[n] = given;
+    sc.take[n] = taken;
+    sc.rows[n] = total;
+  }
+  __syncthreads();
+  if (given > 0) {  // pushed above the current top, which this launch only reads below it
+#pragma unroll 1
+    for (int k = t; k < given; k += THREADS) {
+      const int i = find_segment(sc.give, n, k);
+      p.free_list[count + k] = p.table[(long long)i * p.table_stride + plan_blocks_of(p.new_len[i], B) + k - sc.give[i]];
+    }
+    __syncthreads();
+  }
+  if (taken > 0) {
+#pragma unroll 1
+    for (int k = t; k < taken; k += THREADS) {
+      const int i = find_segment(sc.take, n, k);
+      p.table[(long long)i * p.table_stride + plan_blocks_of(p.old_len[i], B) + k - sc.take[i]] = p.free_list[count + given - 1 - k];
+    }
+    __syncthreads();  // the rows below read the table entries written above
+  }
+  if (inline_rows) {
+#pragma unroll 1
+    for (int r = t; r < total; r += THREADS) {
+      const int i = find_segment(sc.rows, n, r), pos = p.old_len[i] + r - sc.rows[i];
+      p.row_seq[r] = i;
+      p.positions[r] = pos;
+      p.slots[r] = p.table[(long long)i * p.table_stride + pos / B] * B + pos % B;
+    }
+    for (int r = total + t; r < p.rows; r += THREADS) p.row_seq[r] = p.positions[r] = p.slots[r] = -1;
+  }
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) gg_plan_many_kernel(const gg_block_plan p, int inline_rows) {
   extern __shared__ __align__(16) unsigned char plan_smem[];
   PlanScan& sc = *reinterpret_cast<PlanScan*>(plan_smem);
   __shared__ long long s_sum[3][PLAN_THREADS / 32];
@@ -208,7 +336,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) gg_plan_kernel(const gg_block_pl
     if (t == 0) p.cu_rows[p.seqs] = 0;
   } else {
     // blocks given back: pushed above the current top, which this launch only reads below it
-    if (given > 0 && chunks > 1) {
+    if (given > 0) {
       int base = count;
       for (int c = 0; c < chunks; c++) {
         const int i0 = c * PLAN_CHUNK, n = min(PLAN_CHUNK, p.seqs - i0);
@@ -227,14 +355,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) gg_plan_kernel(const gg_block_pl
     for (int c = 0; c < chunks; c++) {
       const int i0 = c * PLAN_CHUNK, n = min(PLAN_CHUNK, p.seqs - i0);
       plan_scan(p, i0, n, sc);
-      if (chunks == 1 && given > 0) {
-        for (int k = t; k < given; k += PLAN_THREADS) {
-          const int i = find_segment(sc.give, n, k);
-          const int b = plan_blocks_of(p.new_len[i], B) + k - sc.give[i];
-          p.free_list[count + k] = p.table[(long long)i * p.table_stride + b];
-        }
-        __syncthreads();
-      }
       for (int i = t; i < n; i += PLAN_THREADS) {
         p.lens[i0 + i] = p.new_len[i0 + i];
         p.cu_rows[i0 + i] = base_rows + sc.rows[i];
@@ -654,7 +774,12 @@ extern "C" int gg_plan_blocks(const gg_block_plan* plan, void* stream) {
   if (int rc = ops_check_stream(fn, s)) return rc;
   const int inline_rows = p.rows <= PLAN_INLINE_ROWS;
   static_assert(sizeof(PlanScan) > 48 * 1024 && sizeof(PlanScan) < 64 * 1024, "opt-in shared memory");
-  cudaError_t r = launch_big_smem(gg_plan_kernel, dim3(1), dim3(PLAN_THREADS), sizeof(PlanScan), s, p, inline_rows);
+  auto kernel = gg_plan_many_kernel;
+  int threads = PLAN_THREADS;
+  if (p.seqs <= 256) kernel = gg_plan_kernel<256, 1>, threads = 256;
+  else if (p.seqs <= PLAN_THREADS) kernel = gg_plan_kernel<PLAN_THREADS, 1>;
+  else if (p.seqs <= PLAN_CHUNK) kernel = gg_plan_kernel<PLAN_THREADS, PLAN_PER>;
+  cudaError_t r = launch_big_smem(kernel, dim3(1), dim3(threads), sizeof(PlanScan), s, p, inline_rows);
   if (r == cudaSuccess && !inline_rows) {
     const int grid = (int)(((long long)p.rows + 255) / 256);
     r = launch_pdl(gg_plan_rows_kernel, dim3(grid < 1184 ? grid : 1184), dim3(256), 0, s, p);
