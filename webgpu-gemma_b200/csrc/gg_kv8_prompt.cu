@@ -40,8 +40,8 @@ struct PromptShape {
   static constexpr int OFF_MUL = OFF_META + GROUPS * 16;
   static constexpr int OFF_BAR = OFF_MUL + NQ * 128 * 4;
   static constexpr int SMEM = OFF_BAR + 256 + 1024;  // + alignment of the operand tiles
-  static constexpr int SOFT_WARPS = 4 * NQ, CONV_WARPS = 4;
-  static constexpr int THREADS = (SOFT_WARPS + CONV_WARPS + 1) * 32;
+  static constexpr int SOFT_WARPS = 4 * NQ, CONV_WARPS = HD == 256 ? 8 : 4;
+  static constexpr int THREADS = (SOFT_WARPS + CONV_WARPS + 2) * 32;  // and two that issue MMAs
   static constexpr int TMEM_S = KT;               // columns of one S buffer: two for each query tile
   static constexpr int TMEM_O = 2 * NQ * KT;      // first column of O
   static_assert(2 * NQ * KT + NQ * HD <= 512, "TMEM columns");
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
   // kfull, vfull, kdone: by ring stage; sfull, pfull: [query tile][parity of the key tile]; odone:
   // [query tile][key tile mod 4], so that a parity always tells a phase from the one before
   uint64_t *vfull = kfull + 4, *sfull = kfull + 8, *pfull = kfull + 12, *odone = kfull + 16, *kdone = kfull + 24, *drain = kfull + 26;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 27);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 28);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   constexpr int MMA_WARP = S::SOFT_WARPS + S::CONV_WARPS;
@@ -213,8 +213,10 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         mbar_init(&pfull[i], 4);
         mbar_init(&sfull[i], 1);
       }
-      for (int i = 0; i < 2; i++) mbar_init(&kdone[i], 1);
-      mbar_init(drain, 1);
+      for (int i = 0; i < 2; i++) {
+        mbar_init(&kdone[i], NQ);
+        mbar_init(&drain[i], 1);
+      }
       *abort = 0;
       mbar_fence_init();
     }
@@ -350,6 +352,11 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
       }
       fence_proxy_async_smem();
     };
+    const auto products_done = [&](int i) {  // P V of key tile i, every query tile's
+      bool ok = true;
+      for (int q = 0; q < NQ; q++) ok = ok && prompt_wait_warp(&odone[4 * q + i % 4], (i >> 2) & 1, abort);
+      return ok;
+    };
     uint4 rk[WORDS], rv[WORDS];
     float2 sc[2] = {};
     fetch(a.kc, 0, 0, rk);
@@ -369,19 +376,22 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         for (int j = 0; j < 2; j++) put_group((b + 1) * 64 + lane + 32 * j, nxt[j], sc[j]);
       // A stage is free once both products of the tile that had it are done; with few stages its K
       // is waited for, and handed back, by itself once the scores are.
-      if (i >= ST && !prompt_wait_warp(S::EARLY_K ? &kdone[st] : &odone[4 * (NQ - 1) + (i - ST) % 4], S::EARLY_K ? par ^ 1 : ((i - ST) >> 2) & 1, abort)) break;
+      if (i >= ST && !(S::EARLY_K ? prompt_wait_warp(&kdone[st], par ^ 1, abort) : products_done(i - ST))) break;
       put(sm + S::OFF_K + st * S::KV_BYTES, rk);
       __syncwarp();
       if (lane == 0) mbar_arrive(&kfull[st]);
       fetch(a.kc, i + 1, b, rk);
-      if (S::EARLY_K && i >= ST && !prompt_wait_warp(&odone[4 * (NQ - 1) + (i - ST) % 4], ((i - ST) >> 2) & 1, abort)) break;
+      if (S::EARLY_K && i >= ST && !products_done(i - ST)) break;
       put(sm + S::OFF_V + st * S::KV_BYTES, rv);
       __syncwarp();
       if (lane == 0) mbar_arrive(&vfull[st]);
       fetch(a.vc, i + 1, b, rv);
     }
-  } else if (nt && warp == MMA_WARP) {
+  } else if (nt && warp >= MMA_WARP) {
     // ------------------------------------------------------------------ MMA issue (lane 0's MMAs)
+    // a warp for each query tile; with one query tile, a warp for each product
+    const int q = NQ == 2 ? warp - MMA_WARP : 0;
+    const bool for_s = NQ == 2 || warp == MMA_WARP, for_o = NQ == 2 || warp != MMA_WARP;
     const uint32_t on = lane == 0;
     // the same in every lane, which the compiler sees of a shuffle's result but not of a load's
     const int tiles = __shfl_sync(0xffffffffu, nt, 0);
@@ -391,7 +401,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     const uint64_t qd = umma_desc_sw128(smem_u32(sm)), kd = umma_desc_sw128(smem_u32(sm + S::OFF_K));
     const uint64_t vd = umma_desc_sw128_mn(smem_u32(sm + S::OFF_V), KT * 128);
     // descriptors count 16-byte units; the address field does not overflow (227 KB of shared memory)
-    const auto scores = [&](int q, int i) {  // S buffer = Q tile q x K tile i
+    const auto scores = [&](int i) {  // S buffer = Q tile q x K tile i
       const int buf = 2 * q + (i & 1);
       const uint64_t kb = kd + (uint32_t)(i % ST) * (S::KV_BYTES / 16);
 #pragma unroll
@@ -402,9 +412,9 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
             umma_f16_ss(tm + buf * S::TMEM_S, qd + (uint32_t)q * (S::Q_BYTES / 16) + part * (S::Q_BYTES / 32) + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2,
                         kb + (k >> 2) * (KT * 128 / 16) + (k & 3) * 2, idesc_s, part > 0 || k > 0, on);
       umma_commit_on(&sfull[buf], on);
-      if (S::EARLY_K && q == NQ - 1) umma_commit_on(&kdone[i % ST], on);
+      if (S::EARLY_K) umma_commit_on(&kdone[i % ST], on);
     };
-    const auto outputs = [&](int q, int i) {  // O tile q += P x V tile i
+    const auto outputs = [&](int i) {  // O tile q += P x V tile i
       const uint32_t d = tm + S::TMEM_O + q * HD, p = tm + (2 * q + (i & 1)) * S::TMEM_S;
       const uint64_t vb = vd + (uint32_t)(i % ST) * (S::KV_BYTES / 16);
 #pragma unroll
@@ -414,38 +424,37 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
           umma_f16_ts(d, p + part * 32 + k * 8, vb + k * (2048 / 16), idesc_o, (HILO ? i % PROMPT_FLUSH != 0 : i > 0) || k > 0 || part > 0, on);
       umma_commit_on(&odone[4 * q + (i & 3)], on);
     };
-    // Scores run two key tiles ahead of their weights (one with a single ring stage), so that the
-    // softmax warps hardly wait for them. They overwrite the weights of two tiles before, once the
-    // product that reads those is complete (MMAs with different accumulators are not ordered); the
-    // other query tile's product covers that wait. Each commit takes the tensor pipe as long as an
-    // MMA of N = 64 (62 cycles), hence few of them.
+    // Scores run two key tiles ahead of their weights, so that the softmax warps hardly wait for
+    // them. They overwrite the weights of two tiles before, once the product that reads those is
+    // complete (MMAs with different accumulators are not ordered). Each wait costs the issuing warp
+    // about 100 cycles even when it is over, and the tensor pipe runs dry meanwhile: hence two warps,
+    // whose waits the other's products cover (517 us with one, 427 with two for two prompts of 8192
+    // keys and 30 query tiles in all, 8 key heads of 128). Each commit takes the pipe as long as
+    // an MMA of N = 64 (62 cycles), hence few of them.
     bool ok = true;
-    const auto scores_of = [&](int i) {  // all query tiles, when K is there and the buffers are free
-      if (!prompt_wait_warp(&kfull[i % ST], (i / ST) & 1, abort)) return false;
-#pragma unroll
-      for (int q = 0; q < NQ; q++) {
-        if (i > 1 && !prompt_wait_warp(&odone[4 * q + (i - 2) % 4], ((i - 2) >> 2) & 1, abort)) return false;
-        tc_fence_after();
-        scores(q, i);
-      }
-      return true;
+    const auto scores_of = [&](int i) {  // when K is there and the buffer is free
+      if (!for_s || !ok || i >= tiles) return;
+      ok = prompt_wait_warp(&kfull[i % ST], (i / ST) & 1, abort);
+      if (i > 1) ok = ok && prompt_wait_warp(&odone[4 * q + (i - 2) % 4], ((i - 2) >> 2) & 1, abort);
+      if (!ok) return;
+      tc_fence_after();
+      scores(i);
     };
-    constexpr int AHEAD = ST > 1 ? 2 : 1;
-    for (int i = 0; ok && i < AHEAD && i < tiles; i++) ok = scores_of(i);
+    scores_of(0);
+    scores_of(1);
     for (int i = 0; ok && i < tiles; i++) {
-      if (AHEAD == 1 && i + 1 < tiles && !(ok = scores_of(i + 1))) break;
-#pragma unroll
-      for (int q = 0; q < NQ; q++) {
-        if (!(ok = prompt_wait_warp(&pfull[2 * q + (i & 1)], (i >> 1) & 1, abort))) break;
-        if (q == 0 && !(ok = prompt_wait_warp(&vfull[i % ST], (i / ST) & 1, abort))) break;
+      if (for_o) {  // when V and the weights are there
+        ok = prompt_wait_warp(&vfull[i % ST], (i / ST) & 1, abort) && prompt_wait_warp(&pfull[2 * q + (i & 1)], (i >> 1) & 1, abort);
+        if (!ok) break;
         tc_fence_after();
-        outputs(q, i);
+        outputs(i);
       }
-      if (AHEAD == 2 && ok && i + 2 < tiles) ok = scores_of(i + 2);
+      scores_of(i + 2);
     }
     if (!ok) {  // everything issued so far has finished before TMEM is freed
-      umma_commit_on(drain, on);
-      for (int it = 0; it < 1000000 && !mbar_try_wait(drain, 0); ++it) {
+      uint64_t* mine = &drain[warp - MMA_WARP];
+      umma_commit_on(mine, on);
+      for (int it = 0; it < 1000000 && !mbar_try_wait(mine, 0); ++it) {
       }
     }
   } else if (warp < S::SOFT_WARPS) {
