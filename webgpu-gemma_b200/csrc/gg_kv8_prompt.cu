@@ -188,9 +188,9 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
   int x = blockIdx.x;
   const int split = x % a.splits;
   x /= a.splits;
-  const int rt = a.row_tiles - 1 - x % a.row_tiles;  // the tiles with the most keys first
-  x /= a.row_tiles;
-  const int h = x % a.kv_heads, s = x / a.kv_heads;
+  const int h = x % a.kv_heads;
+  x /= a.kv_heads;
+  const int s = x % a.seqs, rt = a.row_tiles - 1 - x / a.seqs;  // every request's tiles with the most keys first
   const Kv8Seq sq = kv8_seq(a, s);
   const int items = sq.n * a.group, base = rt * (NQ * 128);
   const int nitems = max(min(NQ * 128, items - base), 0);
@@ -236,48 +236,54 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     const int tok0 = base / a.group, rem0 = base - tok0 * a.group;
     const uint32_t gmagic = (1u << 22) / a.group + 1;
     const long long q0 = (long long)(sq.row0 + tok0) * a.q_row + (long long)h * a.group * a.q_head;
-    constexpr int WARPS = S::THREADS / 32, QB = HD == 256 ? 4 : 8, PER = (HD / 4 + 31) / 32;
-    for (int row0 = warp; row0 < NQ * 128; row0 += WARPS * QB) {
-      uint4 raw[QB][PER];
-      load_raw4(raw, a.q, a.q_type, a.q_vec, [&](int j, int p) {
-        const int row = row0 + j * WARPS, d = 4 * (lane + 32 * p), y = rem0 + row, tok = (int)(((uint32_t)y * gmagic) >> 22);
-        return row < nitems && d < a.hd ? q0 + tok * a.q_row + (long long)(y - tok * a.group) * a.q_head + d : -1ll;
-      });
+    constexpr int WARPS = S::THREADS / 32, QB = 5 * NQ, PER = (HD / 4 + 31) / 32;
+    const auto fill = [&](int type, int vec) {
+      for (int row0 = warp; row0 < NQ * 128; row0 += WARPS * QB) {
+        uint4 raw[QB][PER];
+        load_raw4(raw, a.q, type, vec, [&](int j, int p) {
+          const int row = row0 + j * WARPS, d = 4 * (lane + 32 * p), y = rem0 + row, tok = (int)(((uint32_t)y * gmagic) >> 22);
+          return row < nitems && d < a.hd ? q0 + tok * a.q_row + (long long)(y - tok * a.group) * a.q_head + d : -1ll;
+        });
 #pragma unroll
-      for (int j = 0; j < QB; j++) {
-        const int row = row0 + j * WARPS;
-        if (row >= NQ * 128) break;
-        float4 v[PER];
-        uint32_t top = 0;
+        for (int j = 0; j < QB; j++) {
+          const int row = row0 + j * WARPS;  // (no branch on it: the rows' instructions interleave)
+          float4 v[PER];
+          uint32_t top = 0;
 #pragma unroll
-        for (int p = 0; p < PER; p++) {
-          v[p] = widen_raw4(raw[j][p], a.q_type, a.q_vec);
-          top = max(max(top, __float_as_uint(v[p].x) & 0x7fffffffu), __float_as_uint(v[p].y) & 0x7fffffffu);
-          top = max(max(top, __float_as_uint(v[p].z) & 0x7fffffffu), __float_as_uint(v[p].w) & 0x7fffffffu);
-        }
-        top = __reduce_max_sync(0xffffffffu, top);
-        const int ex = min(max((int)(top >> 23) - 127, -100), 127);
-        const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
-        if (lane == 0) s_mul[row] = __uint_as_float((uint32_t)(ex - 14 + 127) << 23) * a.scale_log2;
-        unsigned char* qt = sm + (row >> 7) * S::Q_BYTES;
-        const int r = row & 127;
+          for (int p = 0; p < PER; p++) {
+            v[p] = widen_raw4(raw[j][p], type, vec);
+            top = max(max(top, __float_as_uint(v[p].x) & 0x7fffffffu), __float_as_uint(v[p].y) & 0x7fffffffu);
+            top = max(max(top, __float_as_uint(v[p].z) & 0x7fffffffu), __float_as_uint(v[p].w) & 0x7fffffffu);
+          }
+          top = __reduce_max_sync(0xffffffffu, top);
+          const int ex = min(max((int)(top >> 23) - 127, -100), 127);
+          const float up = __uint_as_float((uint32_t)(14 - ex + 127) << 23);
+          if (lane == 0 && row < NQ * 128) s_mul[row] = __uint_as_float((uint32_t)(ex - 14 + 127) << 23) * a.scale_log2;
+          unsigned char* qt = sm + (row >> 7) * S::Q_BYTES;
+          const int r = row & 127;
 #pragma unroll
-        for (int p = 0; p < PER; p++) {
-          const int d = 4 * (lane + 32 * p);
-          if (d >= HD) break;
-          uint2* dst = reinterpret_cast<uint2*>(qt + (d >> 6) * (128 * 128) + sw128_offset(r, d & 63));
-          if constexpr (HILO) {
-            uint2 hi, lo;
-            split_f16(v[p].x * up, v[p].y * up, hi.x, lo.x);
-            split_f16(v[p].z * up, v[p].w * up, hi.y, lo.y);
-            *dst = hi;
-            *reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(dst) + S::Q_BYTES / 2) = lo;
-          } else {
-            *dst = make_uint2(half2_bits(v[p].x * up, v[p].y * up), half2_bits(v[p].z * up, v[p].w * up));
+          for (int p = 0; p < PER; p++) {
+            const int d = 4 * (lane + 32 * p);
+            if (d >= HD || row >= NQ * 128) continue;
+            uint2* dst = reinterpret_cast<uint2*>(qt + (d >> 6) * (128 * 128) + sw128_offset(r, d & 63));
+            if constexpr (HILO) {
+              uint2 hi, lo;
+              split_f16(v[p].x * up, v[p].y * up, hi.x, lo.x);
+              split_f16(v[p].z * up, v[p].w * up, hi.y, lo.y);
+              *dst = hi;
+              *reinterpret_cast<uint2*>(reinterpret_cast<unsigned char*>(dst) + S::Q_BYTES / 2) = lo;
+            } else {
+              *dst = make_uint2(half2_bits(v[p].x * up, v[p].y * up), half2_bits(v[p].z * up, v[p].w * up));
+            }
           }
         }
       }
-    }
+    };
+    // one loop for each type: with its branches inside a row takes half as many instructions again
+    if (HILO && a.q_vec) fill(GG_T_F32, 1);
+    else if (!HILO && a.q_vec && a.q_type == GG_T_BF16) fill(GG_T_BF16, 1);
+    else if (!HILO && a.q_vec && a.q_type == GG_T_F16) fill(GG_T_F16, 1);
+    else fill(a.q_type, 0);
     fence_proxy_async_smem();
   }
 
@@ -318,25 +324,38 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     const int k0 = (ct >> 5) * KPW + ((lane >> 2) & (KPW - 1)), w = (lane / (4 * KPW)) * 4 + (lane & 3);
     const bool mine = w * 16 < a.hd;
     constexpr int TB = 64 / GT;  // tiles of a batch of 64 groups
-    int cur[2] = {load_id(lane), load_id(lane + 32)}, nxt[2] = {-1, -1};  // this batch's ids and the next one's
-    const long long block_bytes = (long long)a.kv_heads * a.hd << a.block_shift, head_bytes = (long long)h * a.hd << a.block_shift;
+    const long long block_bytes = (long long)a.kv_heads * a.hd << a.block_shift;
     const int tok_mask = (1 << a.block_shift) - 1;
-    const auto fetch = [&](const uint8_t* codes, int tile, int batch, uint4 (&r)[WORDS]) {
+    const auto group_at = [&](int group, int id) {  // offset of a group's first key in its head's codes; -1: none
+      return id < 0 ? -1ll : id * block_bytes + (long long)((k00 + 16 * group) & tok_mask) * a.hd;
+    };
+    // the groups of this batch and the next one's: two of each to a lane
+    int nxt[2] = {load_id(lane), load_id(lane + 32)};
+    long long cur_at[2], nxt_at[2] = {group_at(lane, nxt[0]), group_at(lane + 32, nxt[1])};
+    static_assert(KS % 16 == 0 && KPW <= 8, "keys of a thread have the same place in their groups and the same swizzle");
+    const long long lane_at = ((long long)h * a.hd << a.block_shift) + (k0 & 15) * a.hd + w * 16;
+    const uint8_t *kc = a.kc + lane_at, *vc = a.vc + lane_at;
+    const int left = mine ? min(sq.len, kend) - k00 - k0 : 0;
+    long long at[WORDS];
+    const auto locate = [&](int tile, int batch) {  // this thread's words of a tile, for K and for V
       const bool now = tile / TB == batch;
-      const int id_lo = now ? cur[0] : nxt[0], id_hi = now ? cur[1] : nxt[1];
-      const uint8_t* base = codes + head_bytes + w * 16;
+      const long long lo = now ? cur_at[0] : nxt_at[0], hi = now ? cur_at[1] : nxt_at[1];
 #pragma unroll
       for (int i = 0; i < WORDS; i++) {
         const int k = k0 + KS * i, group = (tile * GT + (k >> 4)) & 63;
-        const int id = __shfl_sync(0xffffffffu, group & 32 ? id_hi : id_lo, group & 31);
-        const int key = k00 + tile * KT + k;
+        at[i] = __shfl_sync(0xffffffffu, group & 32 ? hi : lo, group & 31);
+        if (tile * KT + KS * i >= left) at[i] = -1;
+      }
+    };
+    const auto fetch = [&](const uint8_t* codes, uint4 (&r)[WORDS]) {
+#pragma unroll
+      for (int i = 0; i < WORDS; i++) {
         r[i] = make_uint4(0, 0, 0, 0);
-        if (mine && id >= 0 && key < sq.len) r[i] = __ldg(reinterpret_cast<const uint4*>(base + id * block_bytes + (key & tok_mask) * a.hd));
+        if (at[i] >= 0) r[i] = __ldg(reinterpret_cast<const uint4*>(codes + at[i]));
       }
     };
     const uint32_t row0 = (w >> 2) * (KT * 128) + (k0 >> 3) * 1024 + (k0 & 7) * 128;
     const uint32_t at0 = row0 + ((((w & 3) * 2) ^ (k0 & 7)) << 4), at1 = row0 + ((((w & 3) * 2 + 1) ^ (k0 & 7)) << 4);
-    static_assert(KS % 8 == 0 && KPW <= 8, "key rows of a thread share their swizzle");
     const auto put = [&](unsigned char* tile, const uint4 (&r)[WORDS]) {
       if (mine) {
 #pragma unroll
@@ -359,15 +378,19 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     };
     uint4 rk[WORDS], rv[WORDS];
     float2 sc[2] = {};
-    fetch(a.kc, 0, 0, rk);
-    fetch(a.vc, 0, 0, rv);
+    cur_at[0] = nxt_at[0], cur_at[1] = nxt_at[1];
+    locate(0, 0);
+    fetch(kc, rk);
+    fetch(vc, rv);
     for (int i = 0; i < nt; i++) {
       const int st = i % ST, par = (i / ST) & 1, b = i / TB, q = i % TB;
       // the next batch of groups: ids, then (one warp) scales, then shared memory, a quarter batch apart
       if (q == 0) {
         for (int j = 0; j < 2; j++) {
-          if (b) cur[j] = nxt[j];
-          nxt[j] = load_id((b + 1) * 64 + lane + 32 * j);
+          const int group = (b + 1) * 64 + lane + 32 * j;
+          cur_at[j] = nxt_at[j];
+          nxt[j] = load_id(group);
+          nxt_at[j] = group_at(group, nxt[j]);
         }
       }
       if (ct < 32 && q == TB / 4)
@@ -380,12 +403,13 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
       put(sm + S::OFF_K + st * S::KV_BYTES, rk);
       __syncwarp();
       if (lane == 0) mbar_arrive(&kfull[st]);
-      fetch(a.kc, i + 1, b, rk);
+      locate(i + 1, b);
+      fetch(kc, rk);
       if (S::EARLY_K && i >= ST && !products_done(i - ST)) break;
       put(sm + S::OFF_V + st * S::KV_BYTES, rv);
       __syncwarp();
       if (lane == 0) mbar_arrive(&vfull[st]);
-      fetch(a.vc, i + 1, b, rv);
+      fetch(vc, rv);
     }
   } else if (nt && warp >= MMA_WARP) {
     // ------------------------------------------------------------------ MMA issue (lane 0's MMAs)
@@ -527,11 +551,12 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
       // x = t - r + 7 in place of the scores: weights are 2^x = 2^7 w
       const auto exponents = [&](float from) {
         tmem_ld32(ts, v[0]);
-        tmem_ld32(ts + 32, v[1]);
         tmem_ld_done();
+        tmem_ld32(ts + 32, v[1]);
         float tops[8];
 #pragma unroll
         for (int g = 0; g < 4; g++) {
+          if (g == 2) tmem_ld_done();
           const float4 m = mt[g];
           const float f = m.x * mul, c = m.y - from;
           const uint64_t f2 = pack2(f, f), c2 = pack2(c, c);
@@ -551,7 +576,30 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         for (int e = 0; e < 64; e += 2) tops[(e >> 1) & 7] = max3(tops[(e >> 1) & 7], __uint_as_float(v[e >> 5][e & 31]), __uint_as_float(v[e >> 5][(e & 31) + 1]));
         top = max3(max3(tops[0], tops[1], tops[2]), max3(tops[3], tops[4], tops[5]), fmaxf(tops[6], tops[7]));
       };
+      uint32_t ph[16], pl[16];
+      // 32 keys: 16 columns of weights (HILO: and 16 of what they leave); returns their part of l
+      const auto weights = [&](int g2) {
+        float add = 0.f;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+          uint64_t sum = 0;  // (0, 0)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float w0 = ex2(__uint_as_float(v[g2][g * 16 + 2 * e])), w1 = ex2(__uint_as_float(v[g2][g * 16 + 2 * e + 1]));
+            add2(sum, w0, w1);
+            if constexpr (HILO) split_f16(w0, w1, ph[g * 8 + e], pl[g * 8 + e]);
+            else ph[g * 8 + e] = half2_bits(w0, w1);
+          }
+          add = fmaf(sum2(sum), mt[2 * g2 + g].z, add);
+        }
+        return add;
+      };
+      const auto store = [&](int g2) {
+        tmem_st16(ts + g2 * 16, ph);
+        if constexpr (HILO) tmem_st16(ts + 32 + g2 * 16, pl);
+      };
       exponents(r - 7.f);
+      float dl = weights(0);  // ahead of the vote, whose latency it covers (430 -> 415 us)
       if (__any_sync(0xffffffffu, top > 7.f + KV8_SLACK)) {
         const bool raise = top > 7.f + KV8_SLACK;
         exponents(0.f);
@@ -572,26 +620,12 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         tmem_st_done();
         r = nr;
         exponents(r - 7.f);
+        dl = weights(0);
       }
-#pragma unroll
-      for (int g2 = 0; g2 < 2; g2++) {  // 32 keys: 16 columns of weights (HILO: and 16 of what they leave)
-        uint32_t ph[16], pl[16];
-#pragma unroll
-        for (int g = 0; g < 2; g++) {
-          const float iv = mt[2 * g2 + g].z;
-          uint64_t sum = 0;  // (0, 0)
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const float w0 = ex2(__uint_as_float(v[g2][g * 16 + 2 * e])), w1 = ex2(__uint_as_float(v[g2][g * 16 + 2 * e + 1]));
-            add2(sum, w0, w1);
-            if constexpr (HILO) split_f16(w0, w1, ph[g * 8 + e], pl[g * 8 + e]);
-            else ph[g * 8 + e] = half2_bits(w0, w1);
-          }
-          l = fmaf(sum2(sum), iv, l);
-        }
-        tmem_st16(ts + g2 * 16, ph);
-        if constexpr (HILO) tmem_st16(ts + 32 + g2 * 16, pl);
-      }
+      l += dl;
+      store(0);
+      l += weights(1);
+      store(1);
       tmem_st_done();
       tc_fence_before();
       __syncwarp();
