@@ -316,9 +316,10 @@ typedef struct {
 int gg_plan_blocks(const gg_block_plan* plan, void* stream);
 
 /* A paged KV cache in 8 bits: codes [num_blocks][kv_heads][block_tokens][head_dim], one f32 scale
- * for each (block, head) of K and of V, [num_blocks][kv_heads]; a value is code * scale. Codes are
- * int8 (-127..127) or e4m3 (finite). block_tokens is 16, 32, 64 or 128, head_dim a multiple of 16
- * up to 256, num_blocks * block_tokens below 2^31, all four arrays 16-byte aligned. */
+ * for each (block, head) of K and of V, [num_blocks][kv_heads]; a value is code * scale. Scales are
+ * positive (or NaN: see the append). Codes are int8 (-127..127) or e4m3 (finite). block_tokens is
+ * 16, 32, 64 or 128, head_dim a multiple of 16 up to 256, num_blocks * block_tokens below 2^31, all
+ * four arrays 16-byte aligned. */
 #define GG_KV8_INT8 0
 #define GG_KV8_E4M3 1
 typedef struct {
@@ -351,8 +352,7 @@ int gg_kv8_append(const gg_kv8_cache* cache, const gg_kv8_append_call* call, voi
  * are the last tokens of request i, whose cache holds lens[i] tokens in blocks table[i][...]; the row
  * at position p = lens[i] - (rows of i) + r sees the keys at max(0, p - window + 1) .. p (window 0:
  * from 0): o = sum softmax(scale q k) v; query head h reads key head h / (q heads / kv_heads), at
- * most 1024 to one. A row
- * that sees no key gives zeros. lse (f32, [rows][q heads], or NULL) receives ln sum exp(scale q k),
+ * most 1024 to one. A row that sees no key gives zeros. lse (f32, [rows][q heads], or NULL) receives ln sum exp(scale q k),
  * -inf for such a row. out has q's type. Scores, softmax and sums are held in f32.
  *   max_rows and max_len are at least every request's number of rows and length (of longer ones,
  *   rows from max_rows on are not computed and keys from max_len on not read); a table entry outside

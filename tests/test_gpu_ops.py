@@ -477,6 +477,26 @@ def test_attend_limits_cut():
         check_attend(rng, rows, lens, 4, *a, "int8", dtype, max_rows=9, max_len=0)
 
 
+@pytest.mark.parametrize("group, last", [(2, [2 ** 31 - 1]), (16, [])])
+def test_attend_bad_cu_rows(group, last):
+    """cu_rows that do not ascend, below zero and beyond the batch: no access outside of it, and the
+    requests whose own two entries are right (rows 5 to 7 and 0 to 2) have their results."""
+    rng = np.random.default_rng(group)
+    lens = [40, 20, 30, 25, 9][:4 + len(last)]
+    c, raws, scales, table = make_batch(rng, None, lens, 16, 1, 64, "int8")
+    cu = [5, 8, -2 ** 31, 0, 3] + last
+    guarded = torch.full((30, group, 64), 7.0, device="cuda")
+    out, q = guarded[10:20], torch.randn(10, group, 64, device="cuda")
+    c.attend(q, dev(cu), dev(lens), dev(table), max_rows=2 if last else 80, max_len=40, out=out)
+    n = 2 if last else 3
+    for first, i in ((5, 0), (0, 3)):
+        want = c.attend(q[first:first + 3], dev([0, 3]), dev(lens[i:i + 1]), dev(table[i:i + 1]), max_rows=n, max_len=40)
+        assert torch.equal(out[first:first + n], want[:n])
+    assert bool((out[8:] == 7.0).all()) and bool((guarded[:10] == 7.0).all()) and bool((guarded[20:] == 7.0).all())
+    if last:  # its rows are more than its tokens: they see nothing
+        assert bool((out[3:5] == 0.0).all())
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("rows, lens", [([1, 1], [700, 300]), ([40], [300])])
 def test_attend_scales_far_apart(dtype, rows, lens):

@@ -12,7 +12,8 @@
 // power of two that puts its largest value in [2^14, 2^15). f32 queries are split into f16 hi + lo
 // (22 bits) and so are their weights: the lo rows fill the half of the 16-row MMA tile that few
 // query rows leave empty, and the two halves are added in registers. f16 and bf16 queries are exact
-// in one f16; their weights are rounded to f16 (2^-12 relative, below the output's own 2^-9 / 2^-12).
+// in one f16; their weights are rounded to f16 (2^-11 relative at most, and not all the same way; the
+// output's own rounding is 2^-8 or 2^-11).
 #include "gg_kv8.h"
 
 
@@ -26,7 +27,10 @@ namespace gg {
 // fill the GPU once whatever the lengths of the requests are (only the device knows them: every CTA
 // sums up the requests and finds its part). Bound by the cache's bytes. Each of the four warps
 // streams its own steps through a private cp.async ring (no barriers between warps); the warps'
-// results meet in shared memory at the end, the parts of a unit in gg_kv8_merge_kernel.
+// results meet in shared memory at the end, the parts of a unit in gg_kv8_merge_kernel. Four requests
+// of up to 131072 keys, 8 key heads of 128, bf16: 157 us, 6.0 TB/s of codes and scales; 64 requests of
+// up to 8192 keys of one head of 256, f32: 38 us, 3.5 TB/s, of which the start, the first loads and
+// the merge take about 15; one request of 641 keys: 10 us, all of it latency.
 //
 // Both products are transposed, so that the few query rows are the narrow side (N = 8) of an
 // m16n8k16 MMA and the accumulators hold nothing else: S^T = K Q^T (16 keys x 8 rows), then
@@ -790,7 +794,10 @@ extern "C" int gg_kv8_attention(const gg_kv8_cache* c, const gg_kv8_attention_ca
   r = c->head_dim <= 64 ? launch_rows_hd<64>(a, c->code, p.nt, s)
       : c->head_dim <= 128 ? launch_rows_hd<128>(a, c->code, p.nt, s)
                            : launch_rows_hd<256>(a, c->code, p.nt, s);
-  if (r == cudaSuccess && p.few_parts) r = merge((KV8_FEW + a.group - 1) / a.group);
+  if (r == cudaSuccess && p.few_parts) {  // no request has more than max_rows tokens
+    const int most = (KV8_FEW + a.group - 1) / a.group;
+    r = merge(b.max_rows < most ? b.max_rows : most);
+  }
   // requests with many
   if (r == cudaSuccess && p.row_tiles) {
     a.items_lo = KV8_FEW;

