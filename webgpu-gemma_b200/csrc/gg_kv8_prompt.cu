@@ -23,7 +23,7 @@
 // 406 us, 798 TFLOP/s. A step of 64 keys takes about 2250 cycles: the MMAs 1850 (61 cycles for N = 64,
 // 75 for N = 128, both as slow from TMEM as from shared memory), the softmax about as long and the
 // conversion of the codes almost so (without widening the step falls by an eighth, and without the
-// exponentials by a twelfth). Before and after its steps a CTA takes 11 us: query rows, output
+// exponentials by a twelfth; with queries of zeros by a seventh, at 975 W the operands count). Before and after its steps a CTA takes 11 us: query rows, output
 // rows, and the next CTA's start.
 //
 // The tensor cores cut the f32 sums they hold: measured, a sum loses 6e-10 of itself a key and
@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     };
     // the groups of this batch and the next one's: two of each to a lane
     int nxt[2] = {load_id(lane), load_id(lane + 32)};
-    long long cur_at[2], nxt_at[2] = {group_at(lane, nxt[0]), group_at(lane + 32, nxt[1])};
+    long long nxt_at[2] = {group_at(lane, nxt[0]), group_at(lane + 32, nxt[1])}, cur_at[2] = {nxt_at[0], nxt_at[1]};
     static_assert(KS % 16 == 0 && KPW <= 8, "keys of a thread have the same place in their groups and the same swizzle");
     const long long lane_at = ((long long)h * a.hd << a.block_shift) + (k0 & 15) * a.hd + w * 16;
     const uint8_t *kc = a.kc + lane_at, *vc = a.vc + lane_at;
@@ -387,7 +387,6 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     };
     uint4 rk[WORDS], rv[WORDS];
     float2 sc[2] = {};
-    cur_at[0] = nxt_at[0], cur_at[1] = nxt_at[1];
     locate(0, 0);
     fetch(kc, rk);
     fetch(vc, rv);
