@@ -454,6 +454,15 @@ def test_attend_many_requests(dtype):
     check_attend(rng, rows, lens, 3, *a, "int8", dtype)
 
 
+@pytest.mark.parametrize("G, rows, lens", [(33, [1, 0, 2], [40, 0, 300]), (1000, [2, 1], [70, 9]), (1024, [1, 1], [1, 200])])
+@pytest.mark.parametrize("code, dtype, D", [("int8", "f32", 64), ("e4m3", "bf16", 256), ("int8", "f16", 128)])
+def test_attend_wide_groups(code, dtype, D, G, rows, lens):
+    """More query heads to a key head than a tile has rows: tokens begin and end inside tiles."""
+    rng = np.random.default_rng(G + D)
+    a = make_batch(rng, rows, lens, 16, 1, D, code)
+    check_attend(rng, rows, lens, G, *a, code, dtype)
+
+
 def test_attend_bad_pages():
     """Block ids outside the cache hide their keys; a request with no valid block gives zeros."""
     rng = np.random.default_rng(1)
@@ -686,3 +695,24 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in got[i])  # and the result does not depend on the order of its parts
+
+
+@pytest.mark.parametrize("D, dtype", [(64, "bf16"), (128, "f32")])
+def test_two_streams_of_prompts_at_once(D, dtype):
+    """Two calls with many rows at the same time: their CTAs take turns on the SMs' tensor memory."""
+    rng = np.random.default_rng(D)
+    rows, lens = [300, 90], [900, 400]
+    c, raws, scales, table = make_batch(rng, rows, lens, 16, 2, D, "int8")
+    cu, ln, tb = dev([0, 300, 390]), dev(lens), dev(table)
+    qs = [torch.randn(390, 8, D, device="cuda").to(DT[dtype]) for _ in range(2)]
+    want = [c.attend(q, cu, ln, tb, max_rows=300, max_len=900) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(c.attend(qs[i], cu, ln, tb, max_rows=300, max_len=900))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, want[i]) for o in got[i])
