@@ -20,10 +20,10 @@
 // then now and then).
 //
 // Measured with 2005 and 1804 rows over 7058 and 5134 keys, 32 query heads over 8 of 128, int8, bf16:
-// 406 us, 798 TFLOP/s. A step of 64 keys takes about 2250 cycles: the MMAs 1850 (61 cycles for N = 64,
+// 405 us, 800 TFLOP/s. A step of 64 keys takes about 2250 cycles: the MMAs 1850 (61 cycles for N = 64,
 // 75 for N = 128, both as slow from TMEM as from shared memory), the softmax about as long and the
 // conversion of the codes almost so (without widening the step falls by an eighth, and without the
-// exponentials by a twelfth; with queries of zeros by a seventh, at 975 W the operands count). Before and after its steps a CTA takes 11 us: query rows, output
+// exponentials by a twelfth; with queries of zeros by a seventh, at 975 W the operands count). Before and after its steps a CTA takes 10 us: query rows, output
 // rows, and the next CTA's start.
 //
 // The tensor cores cut the f32 sums they hold: measured, a sum loses 6e-10 of itself a key and
@@ -646,6 +646,13 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     const float keep = ex2(sum_r - r);
     const float nan = __uint_as_float(0x7fffffffu);
     const float inv = !ok ? nan : a.splits > 1 ? 1.f / KV8_WMUL : l == 0.f ? 0.f : (1.f / KV8_WMUL) / l;
+    // A warp's rows pass through the shared memory of its query rows, which no product reads any more, so
+    // that they leave as whole rows and not 16 bytes of each at a time (2.9 us a
+    // CTA instead of 3.6). Words are swizzled by row.
+    constexpr int ES = HILO ? 4 : 2, WORDS_OUT = HD * ES / 16;
+    unsigned char* turned = sm + q * S::Q_BYTES + (warp & 3) * (S::Q_BYTES / 4);
+    const auto word_at = [&](int r, int w) { return reinterpret_cast<uint4*>(turned + r * (HD * ES) + ((w ^ (r & 7)) << 4)); };
+    const long long oi = ri * a.o_row + (long long)hq * a.o_head;
     for (int c = 0; c < a.hd; c += 32) {
       uint32_t v[32];
       if (nt && ok) {
@@ -664,30 +671,38 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
           for (int e = 0; e < 32; e += 4)
             if (e < n) *reinterpret_cast<uint4*>(dst + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
         } else {
-          const long long oi = ri * a.o_row + (long long)hq * a.o_head + c;
           if (!a.o_vec) {
 #pragma unroll
             for (int e = 0; e < 32; e++)
-              if (e < n) store_elem(a.out, a.q_type, oi + e, __uint_as_float(v[e]));
-          } else if (a.q_type == GG_T_F32) {
+              if (e < n) store_elem(a.out, a.q_type, oi + c + e, __uint_as_float(v[e]));
+          } else if constexpr (HILO) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (e < n) *reinterpret_cast<uint4*>(static_cast<float*>(a.out) + oi + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            for (int e = 0; e < 32; e += 4) *word_at(lane, (c + e) / 4) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
           } else {
             const bool bf = a.q_type == GG_T_BF16;
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              if (e < n) {
-                uint32_t w[4];
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t w[4];
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                  const float y0 = __uint_as_float(v[e + 2 * j]), y1 = __uint_as_float(v[e + 2 * j + 1]);
-                  w[j] = bf ? pack_bf16x2(__float2bfloat16_rn(y0), __float2bfloat16_rn(y1)) : half2_bits(y0, y1);
-                }
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + oi + e) = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int j = 0; j < 4; j++) {
+                const float y0 = __uint_as_float(v[e + 2 * j]), y1 = __uint_as_float(v[e + 2 * j + 1]);
+                w[j] = bf ? pack_bf16x2(__float2bfloat16_rn(y0), __float2bfloat16_rn(y1)) : half2_bits(y0, y1);
               }
+              *word_at(lane, (c + e) / 8) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
           }
         }
+      }
+    }
+    if (a.splits == 1 && a.o_vec) {
+      __syncwarp();
+      const uint32_t rows_live = __ballot_sync(0xffffffffu, live);
+      const int words = a.hd * ES / 16;
+#pragma unroll 4
+      for (int k = 0; k < WORDS_OUT; k++) {
+        const int x = k * 32 + lane, from = x / WORDS_OUT, w = x % WORDS_OUT;
+        const long long at = __shfl_sync(0xffffffffu, oi, from);
+        if ((rows_live >> from & 1) && w < words) reinterpret_cast<uint4*>(static_cast<unsigned char*>(a.out) + at * ES)[w] = *word_at(from, w);
       }
     }
     if (live) {
