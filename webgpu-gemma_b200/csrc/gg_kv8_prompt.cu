@@ -23,8 +23,8 @@
 // 405 us, 800 TFLOP/s. A step of 64 keys takes about 2250 cycles: the MMAs 1850 (61 cycles for N = 64,
 // 75 for N = 128, both as slow from TMEM as from shared memory), the softmax about as long and the
 // conversion of the codes almost so (without widening the step falls by an eighth, and without the
-// exponentials by a twelfth; with queries of zeros by a seventh, at 975 W the operands count). Before and after its steps a CTA takes 10 us: query rows, output
-// rows, and the next CTA's start.
+// exponentials by a twelfth; with queries of zeros by a seventh, at 975 W the operands count). Before
+// and after its steps a CTA takes 10 us: query rows, output rows, and the next CTA's start.
 //
 // The tensor cores cut the f32 sums they hold: measured, a sum loses 6e-10 of itself a key and
 // product, always downwards (1.1e-5 after 8192 keys with both products of f32 queries). For f16 and

