@@ -176,7 +176,9 @@ GG_DEV void store_elem4(void* p, int type, long long i, const float4& v, int vec
   }
 }
 
-// The rows of request s: first row, number of rows (within the batch and max_rows), length.
+// The rows of request s: first row, number of rows (within the batch and max_rows), and the keys they
+// may see: up to the last row's own, whatever of the request lies behind it. The launch is sized from max_rows,
+// max_len and the window (kv8_plan), so no request may have more keys than they allow.
 struct Kv8Seq {
   int row0, n, len;
   long long first_pos;  // position of row row0
@@ -190,7 +192,7 @@ GG_DEV Kv8Seq kv8_seq(const Kv8Args& a, int s) {
   q.n = min(q.n, a.max_rows);
   const long long items = (long long)q.n * a.group;
   if (items <= a.items_lo || items > a.items_hi) q.n = 0;  // another launch's request
-  q.len = min(len, a.max_len);
+  q.len = (int)max(min((long long)min(len, a.max_len), q.first_pos + q.n), 0ll);
   return q;
 }
 
