@@ -641,7 +641,8 @@ static int kv8_row_tiles(long long items, int head_dim) { return items <= 8 ? 1 
 
 // How a call is cut. Requests with few rows (rows * group up to KV8_FEW) take the kernel above, the
 // others the one of gg_kv8_prompt.cu; a call that may hold both launches both, and each skips the
-// other's requests.
+// other's requests. Of calls that kv8_check lets through: seqs * max_rows * heads
+// is below 2^31, so row_tiles fits an int.
 constexpr int KV8_FEW = 32, KV8_WHOLE = 128 << 10;
 
 struct Kv8Plan {
@@ -702,8 +703,9 @@ static int kv8_check(const char* fn, const gg_kv8_cache* c, const gg_kv8_attenti
   if (b->seqs < 0 || b->rows < 0 || b->max_rows < 0 || b->max_len < 0)
     return ops_fail(GG_E_ARG, "%s: seqs %d, rows %d, max_rows %d, max_len %d out of range", fn, b->seqs, b->rows, b->max_rows, b->max_len);
   if (b->window < 0) return ops_fail(GG_E_ARG, "%s: window %d", fn, b->window);
-  const Kv8Plan p = kv8_plan(*c, *b);
-  if (p.few_ctas < 0 || (double)b->seqs * c->kv_heads * p.row_tiles * p.splits >= 2147483647.0 || (double)b->seqs * b->max_rows * b->q.heads >= 2147483647.0)
+  const bool rows_fit = (double)b->seqs * b->max_rows * b->q.heads < 2147483647.0;
+  const Kv8Plan p = rows_fit ? kv8_plan(*c, *b) : Kv8Plan();
+  if (!rows_fit || p.few_ctas < 0 || (double)b->seqs * c->kv_heads * p.row_tiles * p.splits >= 2147483647.0)
     return ops_fail(GG_E_ARG, "%s: the batch needs more than 2^31 tiles", fn);
   return GG_OK;
 }
