@@ -317,7 +317,7 @@ int gg_plan_blocks(const gg_block_plan* plan, void* stream);
 
 /* A paged KV cache in 8 bits: codes [num_blocks][kv_heads][block_tokens][head_dim], one f32 scale
  * for each (block, head) of K and of V, [num_blocks][kv_heads]; a value is code * scale. Scales are
- * positive (or NaN: see the append). Codes are int8 (-127..127) or e4m3 (finite). block_tokens is
+ * positive, 2^127 at most (or NaN: see the append); they need not be powers of two. Codes are int8 (-127..127) or e4m3 (finite). block_tokens is
  * 16, 32, 64 or 128, head_dim a multiple of 16 up to 256, num_blocks * block_tokens below 2^31, all
  * four arrays 16-byte aligned. */
 #define GG_KV8_INT8 0
@@ -337,9 +337,9 @@ typedef struct {
  * same slot the last one counts. For each (block, head): the scale is the smallest power of two
  * 2^e, e >= -60, whose largest code reaches every new value (127 2^e, 448 2^e). If the first new
  * slot is not the block's first one, the slots below it hold earlier tokens: the scale is at
- * least the block's old one, and where it grows their codes are re-rounded to it. Slots above the
+ * least the block's old one, and where it differs from that their codes are re-rounded to it. Slots above the
  * new ones keep their codes. Division by a power of two is exact, so every code is off by at most
- * half a step of the final scale per growth. A NaN or infinity makes the scale of its
+ * half a step of the final scale per change. A NaN or infinity makes the scale of its
  * (block, head) NaN until the block is started anew. */
 typedef struct {
   gg_rows k, v;

@@ -1,10 +1,13 @@
 """The device-memory operators at the limits of their calls: sizes that cut a batch short, lengths
 beyond one tile or range, scales and slots at the edge of what a cache may hold. References and tolerances are
 those of test_gpu_ops.py."""
+import math
+
 import numpy as np
 import pytest
 
-from test_gpu_ops import check_attend, make_batch
+import ops_reference as ref
+from test_gpu_ops import check_attend, dev, f64, make_batch, new_cache, raw
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -22,3 +25,73 @@ def test_attend_window_of_cut_requests(code, dtype, D, H, G, window, max_rows):
     a = make_batch(rng, rows, lens, 16, H, D, code)
     check_attend(rng, rows, lens, H * G, *a, code, dtype, window=window, max_rows=max_rows)
     assert a[0].workspace_bytes(torch.empty(1541, H * G, D, device="cuda"), 3, max_rows, 2600, window) > 0  # (the units are cut)
+
+
+# ------------------------------------------------------------------------- scales of any size in a started block
+
+def append_reference(raws, scales, x, slots, code):
+    """ref.append for started blocks whose old scale is any positive number: one run, all in 64 bits."""
+    B, top = raws.shape[2], ref.TOP[code]
+    blk, first = slots[0] // B, min(s % B for s in slots)
+    for h in range(raws.shape[1]):
+        amax, old = np.abs(x[:, h]).max(), scales[blk, h]
+        need = max(amax / top, 2.0 ** -60, old if first > 0 else 0.0)
+        e = math.floor(math.log2(need))
+        e += 2.0 ** e < need
+        if e > 127:  # no f32 holds it
+            scales[blk, h], raws[blk, h, [s % B for s in slots]] = math.nan, 0
+            continue
+        if first > 0 and old != 2.0 ** e:
+            raws[blk, h, :first] = ref.encode(ref.decode(raws[blk, h, :first], code) * (old / 2.0 ** e), code)
+        scales[blk, h] = 2.0 ** e
+        for r, s in enumerate(slots):
+            raws[blk, h, s % B] = ref.encode(x[r, h] * 2.0 ** -e, code)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("size", [0.001, 1.0, 300.0])
+def test_append_to_scales_of_any_size(code, size):
+    """An old scale that is no power of two, or below or above the range that the append itself writes: the
+    new one is the next power of two that holds it and the new values, and earlier tokens keep their values
+    (to half a step). The scales have few bits, so that code times scale is exact in f32."""
+    olds = [1.5, 1.0, 0.75, 1.25, 3.0, 0.0234375, 2.0 ** -60, 1.5 * 2.0 ** -60, 2.0 ** -61, 2.0 ** -100, 2.0 ** -149, 3 * 2.0 ** -149,
+            2.0 ** 122, 1.5 * 2.0 ** 122, 2.0 ** 125, 2.0 ** 127, 1.5 * 2.0 ** 126, 1.25 * 2.0 ** 127]
+    H, D, B = len(olds), 32, 16
+    rng = np.random.default_rng(5)
+    c, raws, scales = new_cache(3, H, B, D, code, 6)
+    for s, t in zip(scales, (c.k_scale, c.v_scale)):
+        s[:] = olds
+        t.copy_(dev(s, torch.float32))
+        assert np.array_equal(f64(t), s)
+    for start in (0, 5):
+        k, v = ((rng.standard_normal((2, H, D)) * size).astype(np.float32) for _ in range(2))
+        for i, x in enumerate((k, v)):
+            append_reference(raws[i], scales[i], x.astype(np.float64), [B + start, B + start + 1], code)
+        c.append(dev(k, torch.float32), dev(v, torch.float32), dev([B + start, B + start + 1]))
+        for got, want in ((c.k_scale, scales[0]), (c.v_scale, scales[1])):
+            assert np.array_equal(f64(got), want, equal_nan=True), start
+        for got, want in ((c.k_codes, raws[0]), (c.v_codes, raws[1])):
+            assert np.array_equal(raw(got), want), start
+        for s, t in zip(scales, (c.k_scale, c.v_scale)):  # the second pass starts from these scales again
+            s[:] = olds
+            t.copy_(dev(s, torch.float32))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_append_keeps_earlier_values(code):
+    """Old scales of 24 bits: the value of every earlier token is off by half a step of the new scale at most
+    (and by the f32 product's 2^-24 of itself)."""
+    H, D, B = 64, 32, 16
+    rng = np.random.default_rng(8)
+    c, raws, scales = new_cache(2, H, B, D, code, 2)
+    for t in (c.k_scale, c.v_scale):
+        t.copy_(torch.rand(2, H, device="cuda") * 2 + 0.01)
+    before = [ref.decode(r[1], code) * f64(t)[1][:, None, None] for r, t in zip(raws, (c.k_scale, c.v_scale))]
+    x = dev(rng.standard_normal((1, H, D)), torch.float32)
+    c.append(x, x, dev([B + 9]))
+    for b, codes, t, r in zip(before, (c.k_codes, c.v_codes), (c.k_scale, c.v_scale), raws):
+        s = f64(t)[1][:, None, None]
+        after = ref.decode(raw(codes)[1], code) * s
+        step = s if code == "int8" else s * 2.0 ** (np.floor(np.log2(np.maximum(np.abs(b / s), 2.0 ** -6))) - 3)
+        assert np.all(np.abs(after - b)[:, :9] <= (step / 2 + np.abs(b) * 2.0 ** -24)[:, :9])
+        assert np.array_equal(raw(codes)[1][:, 10:], r[1][:, 10:])  # slots behind keep their codes

@@ -549,8 +549,8 @@ GG_DEV int kv8_exponent(uint32_t bits) {
   const int e = CODE == GG_KV8_INT8 ? x - 6 + (m > 0x7e0000u) : x - 8 + (m > 0x600000u);
   return max(e, KV8_MIN_EXP);  // zero and subnormal values (x = -127) end here too
 }
-// 2^e for -126 <= e <= 127
-GG_DEV float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// 2^e for -127 <= e <= 127
+GG_DEV float pow2i(int e) { return __uint_as_float(e < -126 ? 0x00400000u : (uint32_t)(e + 127) << 23); }
 
 // Eight values already divided by the scale -> eight codes.
 template <int CODE>
@@ -706,11 +706,13 @@ __global__ void __launch_bounds__(APPEND_THREADS) gg_append_kernel(const AppendA
     float shrink = 1.f;  // what the codes of earlier tokens are multiplied by
     if (first > 0) {
       const uint32_t ob = __float_as_uint(before);
-      if ((ob & 0x7f800000u) == 0x7f800000u) finite = false;  // the block was poisoned before
-      else if (finite) {
-        const int old = min(max((int)(ob >> 23 & 0xffu) - 127, KV8_MIN_EXP), 122);
-        if (e > old) shrink = pow2i(max(old - e, -126));
-        else e = old;
+      // the smallest exponent that holds the old scale, which need not be a power of two; 128 where no
+      // f32 does (or the block was poisoned before)
+      const int old = (int)(ob >> 23) - 127 + ((ob & 0x7fffffu) != 0);
+      if (old > 127) finite = false;
+      if (finite) {
+        e = max(e, old);
+        shrink = before * pow2i(-e);  // exact, or 0 where every code becomes 0
       }
     }
     if (t == 0) *scale = finite ? pow2i(e) : __uint_as_float(0x7fffffffu);
