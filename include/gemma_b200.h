@@ -332,9 +332,10 @@ typedef struct {
 } gg_kv8_cache;
 
 /* Quantises k and v [rows][kv_heads][head_dim] into the cache at slots[row] (device int32; a slot
- * outside 0 .. num_blocks * block_tokens - 1 skips the row). The rows of one block stand next to
- * each other, as gg_plan_blocks lists them, and a block belongs to one request; of rows with the
- * same slot the last one counts. For each (block, head): the scale is the smallest power of two
+ * outside 0 .. num_blocks * block_tokens - 1 skips the row). The rows of one block stand together, as
+ * gg_plan_blocks lists them, with skipped rows between them at most (neighbours fewer than 128 rows
+ * apart, as the tokens of a block are), and a block belongs to one request; of rows with the same
+ * slot the last one counts. For each (block, head): the scale is the smallest power of two
  * 2^e, e >= -60, whose largest code reaches every new value (127 2^e, 448 2^e). If the first new
  * slot is not the block's first one, the slots below it hold earlier tokens: the scale is at
  * least the block's old one, and where it differs from that their codes are re-rounded to it. Slots above the

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import ops_reference as ref
-from test_gpu_ops import check_attend, dev, f64, make_batch, new_cache, raw
+from test_gpu_ops import DT, check_attend, dev, f64, make_batch, new_cache, raw
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -95,3 +95,53 @@ def test_append_keeps_earlier_values(code):
         step = s if code == "int8" else s * 2.0 ** (np.floor(np.log2(np.maximum(np.abs(b / s), 2.0 ** -6))) - 3)
         assert np.all(np.abs(after - b)[:, :9] <= (step / 2 + np.abs(b) * 2.0 ** -24)[:, :9])
         assert np.array_equal(raw(codes)[1][:, 10:], r[1][:, 10:])  # slots behind keep their codes
+
+
+# ------------------------------------------------------------------------- skipped rows inside a block's run
+
+def append_together(raws, scales, x, slots, code):
+    """ref.append where skipped rows may stand between the rows of a block: the batch without them."""
+    live = [r for r, s in enumerate(slots) if 0 <= s < raws.shape[0] * raws.shape[2]]
+    ref.append(raws, scales, x[live], [slots[r] for r in live], code)
+
+
+def gaps(rng, n, start, share, longest):
+    """Slots start .. of consecutive tokens, some masked, now and then a longer stretch without a slot; rows
+    with a slot stand fewer than 128 apart."""
+    slots, since = [], 0
+    for s in range(start, start + n):
+        live = since > 60 or rng.random() >= share
+        slots.append(s if live else int(rng.choice([-1, -9, 2 ** 31 - 1])))
+        since = 0 if live else since + 1
+        if rng.random() < 0.05:
+            more = int(rng.integers(1, longest))
+            slots += [-1] * min(more, 125 - since)
+            since += min(more, 125 - since)
+    return slots
+
+
+@pytest.mark.parametrize("code, dtype", [("int8", "f32"), ("e4m3", "bf16"), ("int8", "f16")])
+@pytest.mark.parametrize("H, D, B, nb", [(1, 256, 16, 60), (3, 80, 32, 40), (2, 64, 128, 20)])
+def test_append_skipped_rows(code, dtype, H, D, B, nb):
+    """Rows masked by -1 between rows of a block: one scale for all of them, whichever row of a CTA's tile or
+    of a 32-row step they stand at. Then rows as far apart as the call allows."""
+    rng = np.random.default_rng(B)
+    c, raws, scales = new_cache(nb, H, B, D, code, B)
+    batches = [[B + 5, -1, B + 6], [-1, B + 7, -1, -1, B + 9, -1], [-1] * 200 + [2 * B, -1, 2 * B + 2] + [-1] * 300,
+               [3 * B] + [-1] * 126 + [3 * B + 1] + [-1] * 126 + [3 * B + 2], [3 * B + 3, -1, -1, 4 * B, -1, 4 * B + 1, 5 * B],
+               [6 * B + 3, -1, 6 * B + 3, -1, 6 * B + 1]]
+    batches += [gaps(rng, nb * B - 3, 3, share, 130) for share in (0.1, 0.5, 0.9)]
+    for slots in batches:
+        last = None  # neighbours with a slot stand fewer than 128 rows apart, or are of different blocks
+        for r, s in enumerate(slots):
+            if 0 <= s < nb * B:
+                assert last is None or r - last[0] < 128 or last[1] // B != s // B
+                last = r, s
+        k, v = ((dev(rng.standard_normal((len(slots), H, D)) * 2.0 ** rng.uniform(-3, 3, (len(slots), H, 1)), torch.float32)).to(DT[dtype]) for _ in range(2))
+        for i, x in enumerate((k, v)):
+            append_together(raws[i], scales[i], f64(x), slots, code)
+        c.append(k, v, dev(slots))
+        for got, want in ((c.k_scale, scales[0]), (c.v_scale, scales[1])):
+            assert np.array_equal(f64(got), want), slots[:20]
+        for got, want in ((c.k_codes, raws[0]), (c.v_codes, raws[1])):
+            assert np.array_equal(raw(got), want), slots[:20]

@@ -538,6 +538,7 @@ cudaError_t launch_rope(const RopeArgs& a, bool vec, cudaStream_t s) {
 // bf16 to e4m3: 10.9 us, 3.5 TB/s (39 us with a search for each row's run and maxima one value at a
 // time); 64 rows of one head of 256, f32 to int8: 2.6 us, all latency.
 constexpr int APPEND_THREADS = 128;
+constexpr int APPEND_GAP = 128;  // rows of a block stand fewer than this apart, as the tokens of the largest block do
 constexpr int KV8_MIN_EXP = -60;
 
 // Smallest e >= KV8_MIN_EXP with |x| <= Q 2^e; bits = the pattern of a finite |x|.
@@ -647,11 +648,30 @@ __global__ void __launch_bounds__(APPEND_THREADS) gg_append_kernel(const AppendA
   const int r0 = blockIdx.x * a.rows_per_cta;
   const int s_here = lane < a.rows_per_cta ? slot_of(r0 + lane) : -1, s_prev = slot_of(r0 + lane - 1);
   uint32_t leaders = __ballot_sync(0xffffffffu, s_here >= 0 && (s_prev < 0 || (s_prev >> a.block_shift) != (s_here >> a.block_shift)));
+  // The nearest row with a slot among the APPEND_GAP - 1 from r on (step 1) or back from r (step -1): its
+  // distance from r, or -1, and its slot.
+  const auto nearest = [&](int r, int step, int& slot) {
+    int s[APPEND_GAP / 32];
+#pragma unroll
+    for (int c = 0; c < APPEND_GAP / 32; c++) s[c] = 32 * c + lane < APPEND_GAP - 1 ? slot_of(r + step * (32 * c + lane)) : -1;
+    int at = -1;
+#pragma unroll
+    for (int c = APPEND_GAP / 32 - 1; c >= 0; c--) {
+      const uint32_t in = __ballot_sync(0xffffffffu, s[c] >= 0);
+      if (!in) continue;
+      at = 32 * c + __ffs(in) - 1;
+      slot = __shfl_sync(0xffffffffu, s[c], at & 31);
+    }
+    return at;
+  };
   for (; leaders; leaders &= leaders - 1) {
     const int r = r0 + __ffs(leaders) - 1;
     const int s0 = __shfl_sync(0xffffffffu, s_here, r - r0);
     const int blk = s0 >> a.block_shift;
-    // the run: rows r .. r + m - 1 of this block; each warp finds it alone
+    // behind skipped rows: the continuation of an earlier row's run?
+    int other = -1;
+    if (r > 0 && __shfl_sync(0xffffffffu, s_prev, r - r0) < 0 && nearest(r - 1, -1, other) >= 0 && other >> a.block_shift == blk) continue;
+    // the run: rows r .. r + m - 1, of this block or skipped; each warp finds it alone
     int m = 0, first = B;
     bool ascending = true;
     for (;;) {
@@ -661,17 +681,26 @@ __global__ void __launch_bounds__(APPEND_THREADS) gg_append_kernel(const AppendA
       const int n = out ? __ffs(out) - 1 : 32;
       first = min(first, (int)__reduce_min_sync(0xffffffffu, lane < n ? (uint32_t)(s & (B - 1)) : (uint32_t)B));
       ascending &= __all_sync(0xffffffffu, lane >= n || s == s0 + m + lane);
+      const int seen = m + 32;
       m += n;
-      if (n < 32) break;
+      if (n == 32) continue;
+      // ended by a row of another block or the last row; behind skipped rows the block may go on
+      if (r + m >= a.rows || __shfl_sync(0xffffffffu, s, n) >= 0) break;
+      if (r + seen >= a.rows && !(__ballot_sync(0xffffffffu, s >= 0) >> n)) break;
+      const int ahead = nearest(r + m, 1, other);
+      if (ahead < 0 || other >> a.block_shift != blk) break;
+      m += ahead;
+      ascending = false;
     }
     const auto row_of = [&](int i) { return i < 2048 ? (int)((i * gmagic) >> 16) : i / groups; };
     const auto fetch = [&](int i, Raw8<T, VEC>& v) {
       const int j = row_of(i);
       v.load(x + (long long)(r + j) * xrow + (i - j * groups) * 8);
     };
-    // of rows with the same slot only the last counts (rows in ascending order have no such)
+    // skipped, or not the last of the rows with its slot (a run in ascending order has no such rows)
     const auto replaced = [&](int j) {
-      const int s = a.slots[r + j];
+      const int s = slot_of(r + j);
+      if (s < 0) return true;
       for (int k = j + 1; k < m; k++)
         if (a.slots[r + k] == s) return true;
       return false;
