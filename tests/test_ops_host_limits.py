@@ -1,4 +1,5 @@
 """Sizes at the edge of what the operators take, on the host: refusals and workspaces, without a GPU."""
+import ctypes
 import subprocess
 import sys
 
@@ -6,7 +7,7 @@ import pytest
 
 from conftest import ROOT
 from gemma_b200 import native
-from test_ops_host import lib  # noqa: F401 (a fixture)
+from test_ops_host import attend, cache, lib, rows  # noqa: F401 (lib is a fixture)
 
 HUGE = """
 import ctypes, sys
@@ -32,8 +33,24 @@ def test_attention_of_too_many_rows_refused(lib, kv, heads):  # noqa: F811
     lines = r.stdout.splitlines()
     assert len(lines) == 12
     for ln in lines:
-        rows, rc, rc2, *msg = ln.split(" ", 3)
-        if int(rows) >= 2 ** 31 - 1:
+        total, rc, rc2, *msg = ln.split(" ", 3)
+        if int(total) >= 2 ** 31 - 1:
             assert (int(rc), int(rc2)) == (native.GG_E_ARG, native.GG_E_ARG) and "tiles" in msg[0]
-        elif int(rows) == 0:
+        elif int(total) == 0:
             assert (int(rc), int(rc2)) == (0, 0)
+
+
+@pytest.mark.parametrize("type_", [0, 1])
+@pytest.mark.parametrize("kv, group, dim", [(1, 4, 256), (8, 4, 128), (2, 1, 64)])
+def test_attention_workspace_grows_with_the_length(lib, type_, kv, group, dim):  # noqa: F811
+    """A workspace for the longest context is enough for every shorter one (what holds one for many calls
+    sizes it once)."""
+    c, need = cache(kv_heads=kv, head_dim=dim, num_blocks=1 << 16), ctypes.c_size_t()
+    for seqs, max_rows, window in ((1, 1, 0), (1, 500, 0), (3, 70, 0), (1, 40, 700), (64, 1, 0), (2, 9, 5000)):
+        last = 0
+        for max_len in list(range(0, 40000, 16)) + list(range(40000, 140000, 1000)):
+            call = attend(rows(heads=kv * group, type=type_), seqs=seqs, rows=seqs * max_rows, max_rows=max_rows, max_len=max_len, window=window)
+            assert lib.gg_kv8_attention_workspace(ctypes.byref(c), ctypes.byref(call), ctypes.byref(need)) == 0
+            assert need.value >= last, (seqs, max_rows, window, max_len)
+            last = need.value
+        assert last > 0

@@ -179,7 +179,7 @@ struct gg_engine {
   std::vector<const double*> kv8_freqs;   // RoPE frequencies of each layer
   PfKv8Rows kv8_rows{};
   float *kv8_qkv = nullptr, *kv8_att = nullptr;
-  void* kv8_ws = nullptr;
+  uint8_t* kv8_ws = nullptr;
   size_t kv8_ws_bytes = 0;
 };
 
@@ -248,7 +248,32 @@ static gg_kv8_cache kv8_cache(const gg_engine* e, int l) {
   return {e->k8 + l * codes, e->v8 + l * codes, e->k8s + l * scales, e->v8s + l * scales, c.max_seqs * e->kv8_blocks, KV8_BLOCK,
           c.num_kv_heads, c.head_dim, GG_KV8_INT8};
 }
-static int grow(gg_engine* e, void** p, size_t* cap, size_t need);
+// Workspace of every attention call to come: prompt chunks of 1 to GG_PF_CHUNK rows, steps of 1 to `reqs`
+// requests, each at the full context (no shorter one needs more).
+static int kv8_alloc_workspace(gg_engine* e, int reqs) {
+  const GGModelDev& m = e->md;
+  std::vector<int> windows;
+  for (int l = 0; l < m.L; l++) {
+    const int w = m.layers[l].window;
+    if (std::find(windows.begin(), windows.end(), w) != windows.end()) continue;
+    windows.push_back(w);
+    const gg_kv8_cache c = kv8_cache(e, l);
+    gg_kv8_attention_call att = {};
+    att.q = {nullptr, 0, 0, m.NQH, GG_T_F32};
+    att.max_len = m.CTX;
+    att.window = w;
+    for (int i = 1; i <= GG_PF_CHUNK + reqs; i++) {
+      const bool chunk = i <= GG_PF_CHUNK;
+      att.seqs = chunk ? 1 : i - GG_PF_CHUNK;
+      att.max_rows = chunk ? i : 1;
+      att.rows = att.seqs * att.max_rows;
+      size_t need = 0;
+      GG_OPS(e, gg_kv8_attention_workspace(&c, &att, &need));
+      e->kv8_ws_bytes = std::max(e->kv8_ws_bytes, need);
+    }
+  }
+  return dalloc(e, &e->kv8_ws, e->kv8_ws_bytes);
+}
 // One layer's attention over the 8-bit cache: the q/k/v planes in pf_y to activation tiles. The rows'
 // positions, slots and requests are in kv8_rows (pf_kv8_rows, once per step).
 static int kv8_attention(gg_engine* e, int l, int splits, long long plane, int reqs, int rows, int max_rows, int max_len,
@@ -266,13 +291,8 @@ static int kv8_attention(gg_engine* e, int l, int splits, long long plane, int r
   const gg_kv8_append_call put = {k, v, e->kv8_rows.slots, rows};
   GG_OPS(e, gg_kv8_append(&c, &put, s));
   const gg_rows out = {e->kv8_att, m.Q, m.HD, m.NQH, GG_T_F32};
-  gg_kv8_attention_call att = {q, out, nullptr, e->kv8_rows.cu_rows, e->kv8_rows.lens, e->kv8_rows.table, e->kv8_blocks, nullptr, 0,
-                               m.attn_scale, reqs, rows, max_rows, max_len, w.window};
-  size_t need = 0;
-  GG_OPS(e, gg_kv8_attention_workspace(&c, &att, &need));
-  GG_TRY(grow(e, &e->kv8_ws, &e->kv8_ws_bytes, need));
-  att.workspace = e->kv8_ws;
-  att.workspace_bytes = e->kv8_ws_bytes;
+  const gg_kv8_attention_call att = {q, out, nullptr, e->kv8_rows.cu_rows, e->kv8_rows.lens, e->kv8_rows.table, e->kv8_blocks, e->kv8_ws,
+                                     e->kv8_ws_bytes, m.attn_scale, reqs, rows, max_rows, max_len, w.window};
   GG_OPS(e, gg_kv8_attention(&c, &att, s));
   GG_CUDA(e, gg_xtiles_from_f32(e->kv8_att, rows, m.Q, thi, tlo, s));
   return GG_OK;
@@ -654,6 +674,7 @@ extern "C" int gg_finalize(gg_engine* e) {
     GG_TRY(dalloc(e, &e->kv8_rows.table, 4 * (size_t)reqs * e->kv8_blocks));
     GG_TRY(dalloc(e, &e->kv8_qkv, 4 * (size_t)rows * (m.Q + 2 * m.KV)));
     GG_TRY(dalloc(e, &e->kv8_att, 4 * (size_t)rows * m.Q));
+    GG_TRY(kv8_alloc_workspace(e, reqs));
     std::vector<std::pair<float, double*>> tabs;
     for (int l = 0; l < c.num_layers; l++) {
       double* f = nullptr;
@@ -1478,7 +1499,6 @@ extern "C" int gg_destroy(gg_engine* e) {
   if (e->lin_x) cudaFree(e->lin_x);
   if (e->lin_tiles) cudaFree(e->lin_tiles);
   if (e->lin_y) cudaFree(e->lin_y);
-  if (e->kv8_ws) cudaFree(e->kv8_ws);
   if (e->ev0) cudaEventDestroy(e->ev0);
   if (e->ev1) cudaEventDestroy(e->ev1);
   if (e->stream) cudaStreamDestroy(e->stream);

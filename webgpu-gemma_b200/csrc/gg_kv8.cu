@@ -686,7 +686,8 @@ static Kv8Plan kv8_plan(const gg_kv8_cache& c, const gg_kv8_attention_call& b) {
     if (p.split_steps < 1) p.split_steps = 1;
     p.splits = (int)((n + p.split_steps - 1) / p.split_steps);
     if (p.splits < 1) p.splits = 1;
-    if (p.splits > 1) p.many_parts = (size_t)b.rows * b.q.heads * p.splits;
+    // room for the ranges before they are evened out: a longer max_len never needs less workspace
+    if (splits > 1) p.many_parts = (size_t)b.rows * b.q.heads * splits;
   }
   // partial outputs, then their (r, l) pairs; few rows: then the line's prefix sums
   p.few_bytes = p.few_parts ? (p.few_parts * (c.head_dim * 4 + 8) + ((size_t)b.seqs + 1) * 4 + 15) / 16 * 16 : 0;
