@@ -44,7 +44,8 @@ typedef struct gg_engine gg_engine;
  * runs through the batched path (gg_prefill in chunks, gg_step and gg_decode as gg_decode_batch of one
  * sequence), which needs the tensor-core shapes and head_dim <= 256; any grouping of query heads
  * works. A slot's positions are written in order: a call may start at or below the slot's length, not
- * beyond it. gg_get_hidden is not available. Not together with GG_FLAG_KV_BF16 or
+ * beyond it. After a call that failed on the device the slot holds the tokens before that call's first
+ * position. gg_get_hidden is not available. Not together with GG_FLAG_KV_BF16 or
  * GG_FLAG_SERIAL_PREFILL. */
 #define GG_FLAG_KV_Q8 4
 
@@ -179,6 +180,10 @@ int gg_set_gemm_kernel(int kind);
  * timed out") after about timeout_ns; the engine stays usable afterwards. No counterpart in
  * the reference (its WebGPU device-lost handler, engine.ts:134-137, has no bounded waits). */
 int gg_selftest_wait(gg_engine* eng, uint64_t timeout_ns);
+
+/* Self-test of callers' recovery, on the host alone: the next call that waits for the device does its work
+ * and then reports GG_E_DEVICE, as after a wait that ran out. */
+int gg_selftest_fail(gg_engine* eng);
 
 /* Bounded-wait limit of the device spins, in nanoseconds (default 1e9). */
 int gg_set_timeout(gg_engine* eng, uint64_t ns);

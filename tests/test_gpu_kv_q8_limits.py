@@ -2,7 +2,8 @@
 import numpy as np
 import pytest
 
-from test_gpu_kv_q8 import _q8
+from conftest import rel_l2
+from test_gpu_kv_q8 import LOGIT_TOL, Reference, _q8
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -26,4 +27,41 @@ def test_no_allocation_after_the_first_call():
         torch.cuda.synchronize()
         free.append(torch.cuda.mem_get_info()[0])
     assert free == free[:1] * 5
+    eng.close()
+
+
+def test_a_failed_call_drops_the_tokens_it_replaced():
+    """A prefill, a step or a batch that starts below the slot's length and fails has replaced some of the
+    later tokens: the slot then ends where that call started, and goes on from there."""
+    from gemma_b200 import synth
+    from gemma_b200.native import GemmaB200Error, engine_from_tensors
+    cfg, tens = _q8("tiny", 7)
+    prompt = [int(t) for t in synth.make_prompt(7, 60, cfg.vocab_size)]
+    eng, want = engine_from_tensors(cfg, tens, max_seqs=2), Reference(cfg, tens)
+    eng.prefill(prompt, 0)
+    want.tokens(prompt, 0)
+    eng.selftest_fail()
+    with pytest.raises(GemmaB200Error, match="timed out"):
+        eng.prefill(prompt[:9], 41)
+    with pytest.raises(GemmaB200Error, match="beyond the 41 tokens"):
+        eng.step(5, 50)
+    eng.prefill(prompt[:9], 41)
+    lg = want.tokens(prompt[:9], 41)
+    eng.sample_last(0)
+    assert rel_l2(eng.logits(), lg) < LOGIT_TOL
+    eng.prefill(prompt, 0, seq=1)
+    eng.selftest_fail()
+    with pytest.raises(GemmaB200Error, match="timed out"):
+        eng.decode_batch([1, 0], [3, 4], [30, 50], 2, [(0.0, 0.9, 1.0)] * 2, np.zeros((2, 2)))
+    for seq, n in ((0, 50), (1, 30)):
+        with pytest.raises(GemmaB200Error, match=f"beyond the {n} tokens of slot {seq}"):
+            eng.step(5, n + 1, seq=seq)
+    eng.selftest_fail()
+    with pytest.raises(GemmaB200Error, match="timed out"):
+        eng.step(5, 47)
+    with pytest.raises(GemmaB200Error, match="beyond the 47 tokens"):
+        eng.step(5, 48)
+    want.tokens([5], 47)  # (it may have raised its block's scale)
+    eng.step(11, 47)
+    assert rel_l2(eng.logits(), want.tokens([11], 47)) < LOGIT_TOL
     eng.close()

@@ -136,6 +136,7 @@ struct gg_engine {
   int last_hidden_seq = -1;
   int trace_on = 0;
   uint64_t timeout_ns = 1000000000ull;
+  bool fail_next = false;  // gg_selftest_fail
   float last_ms = 0.f;
   std::string err;
   // tensor-core GEMM: tensor maps per weight matrix ([layer][0 qkv, 1 o, 2 gu, 3 down]), LM head
@@ -175,7 +176,7 @@ struct gg_engine {
   int kv8_blocks = 0;
   uint8_t *k8 = nullptr, *v8 = nullptr;   // codes [layer][slot][block][head][token][dim]
   float *k8s = nullptr, *v8s = nullptr;   // scales [layer][slot][block][head]
-  std::vector<int> kv8_len;               // tokens in each slot
+  std::vector<int> kv8_len;               // tokens in each slot that are known to be whole
   std::vector<const double*> kv8_freqs;   // RoPE frequencies of each layer
   PfKv8Rows kv8_rows{};
   float *kv8_qkv = nullptr, *kv8_att = nullptr;
@@ -776,6 +777,8 @@ static int finish_synced(gg_engine* e, int32_t* out_token) {
     cudaGetLastError();  // no pending error left for a later call to pick up
   }
   uint32_t err = e->h_st->error;
+  if (e->fail_next) err |= GG_ERR_WAIT_FLAG;
+  e->fail_next = false;
   if (err) {
     cudaMemsetAsync(&e->d_st->error, 0, 4, e->stream);
     cudaStreamSynchronize(e->stream);
@@ -996,6 +999,8 @@ extern "C" int gg_decode_batch(gg_engine* e, int n, const int32_t* seqs, const i
   GG_CUDA(e, cudaMemcpyAsync(e->bd_sp, sp, sizeof(GGSampleDev) * (size_t)n, cudaMemcpyHostToDevice, s));
   GG_CUDA(e, cudaMemcpyAsync(e->bd_unif, uniforms, sizeof(double) * io, cudaMemcpyHostToDevice, s));
   GG_CUDA(e, cudaEventRecord(e->ev0, s));
+  // from here on the slots' later tokens are being replaced: after a failure only the earlier ones count
+  for (int i = 0; e->kv8 && i < n; i++) e->kv8_len[seqs[i]] = pos[i];
   for (int k = 0; k < steps; k++) GG_TRY(batch_step(e, n, max_pos + k, e->bd_unif + (size_t)k * n, e->bd_out + (size_t)k * n));
   GG_CUDA(e, cudaEventRecord(e->ev1, s));
   GG_CUDA(e, cudaMemcpyAsync(e->bd_out_h, e->bd_out, sizeof(int32_t) * io, cudaMemcpyDeviceToHost, s));
@@ -1043,6 +1048,7 @@ extern "C" int gg_prefill(gg_engine* e, int seq, const int32_t* ids, int n, int 
   GG_CUDA(e, cudaGetLastError());
   if (e->gemm_ok && !(e->cfg.flags & GG_FLAG_SERIAL_PREFILL)) {
     GG_CUDA(e, cudaEventRecord(e->ev0, e->stream));
+    if (e->kv8) e->kv8_len[seq] = start_pos;  // (as in gg_decode_batch)
     GG_TRY(prefill_batched(e, seq, n, start_pos));
     GG_CUDA(e, cudaEventRecord(e->ev1, e->stream));
     GG_TRY(finish(e, nullptr));
@@ -1391,6 +1397,12 @@ extern "C" int gg_selftest_wait(gg_engine* e, uint64_t timeout_ns) {
   cudaFree(word);
   if (r != cudaSuccess) return fail(e, GG_E_CUDA, "wait probe: %s", cudaGetErrorString(r));
   return finish(e, nullptr);  // reads and clears the error word, GG_E_DEVICE if it is set
+}
+
+extern "C" int gg_selftest_fail(gg_engine* e) {
+  GG_TRY(ready(e, 0));
+  e->fail_next = true;
+  return GG_OK;
 }
 
 // Sum of `splits` consecutive planes of n floats, in plane order.

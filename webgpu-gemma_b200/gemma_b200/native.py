@@ -48,6 +48,7 @@ SIGNATURES = {
     "gg_linear": (_I, [_P, _I, _I, _P, _I, _P]),
     "gg_decode_batch": (_I, [_P, _I, _P, _P, _P, _I, _P, _P, _P]),
     "gg_selftest_wait": (_I, [_P, ctypes.c_uint64]),
+    "gg_selftest_fail": (_I, [_P]),
     "gg_set_gemm_kernel": (_I, [_I]),
     "gg_sample_logits_noalloc": (_I, [_P, _I, _P, _P, _D, _P, _P]),
     "gg_rope": (_I, [_P, _P]),
@@ -307,6 +308,10 @@ class NativeEngine:
     def selftest_wait(self, timeout_ns: int) -> int:
         """Runs the bounded-wait self-test; returns the status code (GG_E_DEVICE expected)."""
         return self.lib.gg_selftest_wait(self.h, int(timeout_ns))
+
+    def selftest_fail(self):
+        """The next call that waits for the device reports GG_E_DEVICE after doing its work."""
+        self._check(self.lib.gg_selftest_fail(self.h))
 
     def last_error(self) -> str:
         return self.lib.gg_last_error(self.h).decode()
