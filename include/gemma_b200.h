@@ -176,8 +176,9 @@ int gg_linear(gg_engine* eng, int which, int layer, const float* x, int batch, f
 int gg_set_gemm_kernel(int kind);
 
 /* Failure-detection self-test: a one-CTA kernel waits on a device flag that nothing sets,
- * with the same bounded wait the step kernel uses. Returns GG_E_DEVICE ("activation wait
- * timed out") after about timeout_ns; the engine stays usable afterwards. No counterpart in
+ * with the same bounded wait the step kernel uses (with GG_FLAG_KV_Q8 another one then waits as the
+ * prompt attention does). Returns GG_E_DEVICE ("activation wait timed out", "ring wait timed out")
+ * after about timeout_ns each; the engine stays usable afterwards. No counterpart in
  * the reference (its WebGPU device-lost handler, engine.ts:134-137, has no bounded waits). */
 int gg_selftest_wait(gg_engine* eng, uint64_t timeout_ns);
 
@@ -363,7 +364,8 @@ int gg_kv8_append(const gg_kv8_cache* cache, const gg_kv8_append_call* call, voi
  *   max_rows and max_len are at least every request's number of rows and length (of longer ones,
  *   rows from max_rows on are not computed and keys from max_len on not read); a table entry outside
  *   0 .. num_blocks - 1 hides its keys; rows outside cu_rows[0] .. cu_rows[seqs] - 1 are left as
- *   they were. workspace: gg_kv8_attention_workspace bytes, 16-byte aligned, for this call alone
+ *   they were. Waits within the call are bounded: rows whose CTA makes no progress for two seconds are
+ *   NaN (the engine reports GG_E_DEVICE, after gg_set_timeout). workspace: gg_kv8_attention_workspace bytes, 16-byte aligned, for this call alone
  *   until it has run (calls that may run at the same time need one each). */
 typedef struct {
   gg_rows q, out;

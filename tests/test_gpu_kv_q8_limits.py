@@ -65,3 +65,18 @@ def test_a_failed_call_drops_the_tokens_it_replaced():
     eng.step(11, 47)
     assert rel_l2(eng.logits(), want.tokens([11], 47)) < LOGIT_TOL
     eng.close()
+
+
+def test_attention_wait_that_runs_out_is_reported():
+    """The prompt attention's own wait ends after its limit and sets the engine's error word; the engine goes on."""
+    from gemma_b200 import synth
+    from gemma_b200.native import GG_E_DEVICE, engine_from_tensors
+    cfg, tens = _q8("tiny", 7)
+    eng, want = engine_from_tensors(cfg, tens), Reference(cfg, tens)
+    assert eng.selftest_wait(20_000_000) == GG_E_DEVICE
+    assert "activation wait timed out" in eng.last_error() and "ring wait timed out" in eng.last_error()
+    prompt = [int(t) for t in synth.make_prompt(7, 50, cfg.vocab_size)]
+    eng.prefill(prompt, 0)
+    eng.sample_last(0)
+    assert rel_l2(eng.logits(), want.tokens(prompt, 0)) < LOGIT_TOL
+    eng.close()

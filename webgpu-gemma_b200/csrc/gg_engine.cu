@@ -19,6 +19,7 @@
 #include "gg_device.cuh"
 #include "gg_model.h"
 #include "gg_gemm.h"
+#include "gg_kv8.h"
 #include "gg_launch.h"
 #include "gg_prefill.h"
 
@@ -294,7 +295,7 @@ static int kv8_attention(gg_engine* e, int l, int splits, long long plane, int r
   const gg_rows out = {e->kv8_att, m.Q, m.HD, m.NQH, GG_T_F32};
   const gg_kv8_attention_call att = {q, out, nullptr, e->kv8_rows.cu_rows, e->kv8_rows.lens, e->kv8_rows.table, e->kv8_blocks, e->kv8_ws,
                                      e->kv8_ws_bytes, m.attn_scale, reqs, rows, max_rows, max_len, w.window};
-  GG_OPS(e, gg_kv8_attention(&c, &att, s));
+  GG_OPS(e, kv8_attention_bounded(&c, &att, s, &e->d_st->error, e->timeout_ns));
   GG_CUDA(e, gg_xtiles_from_f32(e->kv8_att, rows, m.Q, thi, tlo, s));
   return GG_OK;
 }
@@ -1391,8 +1392,9 @@ extern "C" int gg_selftest_wait(gg_engine* e, uint64_t timeout_ns) {
   cudaMemsetAsync(word, 0, 64, e->stream);
   cudaEventRecord(e->ev0, e->stream);  // finish() reads the ev0 -> ev1 time
   gg_wait_probe_kernel<<<1, 32, 0, e->stream>>>(word, &e->d_st->error, timeout_ns);
-  cudaEventRecord(e->ev1, e->stream);
   cudaError_t r = cudaGetLastError();
+  if (r == cudaSuccess && e->kv8) r = gg::kv8_wait_probe(&e->d_st->error, timeout_ns, e->stream);
+  cudaEventRecord(e->ev1, e->stream);
   if (r == cudaSuccess) r = cudaStreamSynchronize(e->stream);
   cudaFree(word);
   if (r != cudaSuccess) return fail(e, GG_E_CUDA, "wait probe: %s", cudaGetErrorString(r));

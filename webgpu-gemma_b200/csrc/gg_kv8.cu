@@ -723,6 +723,10 @@ extern "C" int gg_kv8_attention_workspace(const gg_kv8_cache* c, const gg_kv8_at
 }
 
 extern "C" int gg_kv8_attention(const gg_kv8_cache* c, const gg_kv8_attention_call* call, void* stream) {
+  return kv8_attention_bounded(c, call, static_cast<cudaStream_t>(stream), nullptr, KV8_TIMEOUT_NS);
+}
+
+int kv8_attention_bounded(const gg_kv8_cache* c, const gg_kv8_attention_call* call, cudaStream_t s, uint32_t* err, uint64_t timeout_ns) {
   using namespace gg;
   const char* fn = "gg_kv8_attention";
   if (!c || !call) return ops_fail(GG_E_ARG, "%s: null argument", fn);
@@ -735,7 +739,6 @@ extern "C" int gg_kv8_attention(const gg_kv8_cache* c, const gg_kv8_attention_ca
   if (b.table_stride < ((long long)b.max_len + c->block_tokens - 1) / c->block_tokens)
     return ops_fail(GG_E_ARG, "%s: table_stride %lld holds fewer than max_len %d tokens", fn, (long long)b.table_stride, b.max_len);
   if (!(b.scale >= -1e30 && b.scale <= 1e30)) return ops_fail(GG_E_ARG, "%s: scale is not a number", fn);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (int rc = ops_check_stream(fn, s)) return rc;
   if (b.seqs == 0 || b.rows == 0 || b.max_rows == 0) return GG_OK;
   const Kv8Plan p = kv8_plan(*c, b);
@@ -771,6 +774,8 @@ extern "C" int gg_kv8_attention(const gg_kv8_cache* c, const gg_kv8_attention_ca
   a.q_type = b.q.type;
   a.q_vec = ops_aligned16(b.q);
   a.o_vec = ops_aligned16(b.out);
+  a.err = err;
+  a.timeout_ns = timeout_ns;
   cudaError_t r = cudaSuccess;
   const auto merge = [&](int tokens) {
     a.merge_tokens = tokens < b.max_rows ? tokens : b.max_rows;

@@ -32,6 +32,8 @@ struct Kv8Args {
   int merge_tokens;                    // tokens of a request that the merge looks at
   int items_lo, items_hi;  // this launch takes requests with items_lo < rows * group <= items_hi
   int q_vec, o_vec;  // every head of q / out starts on a 16-byte boundary
+  uint32_t* err;     // takes GG_ERR_WAIT_MBAR when a wait of the many-rows kernel runs out; or NULL
+  unsigned long long timeout_ns;
 };
 
 GG_DEV float ex2(float x) {
@@ -200,5 +202,7 @@ GG_DEV Kv8Seq kv8_seq(const Kv8Args& a, int s) {
 // Many rows (gg_kv8_prompt.cu): query rows of a tile, and the launch.
 int kv8_prompt_tile(int head_dim);
 cudaError_t kv8_launch_prompt(const Kv8Args& a, int code, cudaStream_t s);
+// Its wait for a barrier that nobody arrives at, for the self-test.
+cudaError_t kv8_wait_probe(uint32_t* err, unsigned long long timeout_ns, cudaStream_t s);
 
 }  // namespace gg

@@ -154,9 +154,9 @@ GG_DEV float max3(float a, float b, float c) {
 
 constexpr int PROMPT_FLUSH = 64;  // tiles of 64 keys
 
-// Wait for an mbarrier phase; after two seconds (or when another warp gave up) sets *abort and
+// Wait for an mbarrier phase; after timeout_ns (or when another warp gave up) sets *abort and *err and
 // returns false: the CTA then drains its MMAs and leaves NaN in its rows.
-GG_DEV bool prompt_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+GG_DEV bool prompt_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t* err, unsigned long long timeout_ns) {
 #pragma unroll 1
   for (int it = 0; it < 64; ++it)
     if (mbar_try_wait(bar, parity)) return true;
@@ -165,16 +165,29 @@ GG_DEV bool prompt_wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
   for (;;) {
     if (mbar_try_wait(bar, parity)) return true;
     if (*abort) return false;
-    if (global_timer_ns() - t0 > 2000000000ull) {
+    if (global_timer_ns() - t0 > timeout_ns) {
       *abort = 1;
+      if (err) atomicOr(err, GG_ERR_WAIT_MBAR);
       return false;
     }
   }
 }
 
 // The same for a whole warp: all lanes agree on the outcome.
-GG_DEV bool prompt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort) {
-  return __all_sync(0xffffffffu, prompt_wait(bar, parity, abort));
+GG_DEV bool prompt_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t* err, unsigned long long timeout_ns) {
+  return __all_sync(0xffffffffu, prompt_wait(bar, parity, abort, err, timeout_ns));
+}
+
+__global__ void gg_kv8_wait_probe_kernel(uint32_t* err, unsigned long long timeout_ns) {
+  __shared__ uint64_t bar;
+  __shared__ int abort;
+  if (threadIdx.x == 0) {
+    mbar_init(&bar, 1);
+    mbar_fence_init();
+    abort = 0;
+  }
+  __syncthreads();
+  (void)prompt_wait_warp(&bar, 0, &abort, err, timeout_ns);
 }
 
 template <int HD, int CODE, bool HILO>
@@ -192,6 +205,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kfull + 28);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const auto wait = [&](uint64_t* bar, uint32_t parity) { return prompt_wait_warp(bar, parity, abort, a.err, a.timeout_ns); };
   constexpr int MMA_WARP = S::SOFT_WARPS + S::CONV_WARPS;
 
   pdl_wait();
@@ -382,7 +396,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     };
     const auto products_done = [&](int i) {  // P V of key tile i, every query tile's
       bool ok = true;
-      for (int q = 0; q < NQ; q++) ok = ok && prompt_wait_warp(&odone[4 * q + i % 4], (i >> 2) & 1, abort);
+      for (int q = 0; q < NQ; q++) ok = ok && wait(&odone[4 * q + i % 4], (i >> 2) & 1);
       return ok;
     };
     uint4 rk[WORDS], rv[WORDS];
@@ -407,7 +421,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         for (int j = 0; j < 2; j++) put_group((b + 1) * 64 + lane + 32 * j, nxt[j], sc[j]);
       // A stage is free once both products of the tile that had it are done; with few stages its K
       // is waited for, and handed back, by itself once the scores are.
-      if (i >= ST && !(S::EARLY_K ? prompt_wait_warp(&kdone[st], par ^ 1, abort) : products_done(i - ST))) break;
+      if (i >= ST && !(S::EARLY_K ? wait(&kdone[st], par ^ 1) : products_done(i - ST))) break;
       put(sm + S::OFF_K + st * S::KV_BYTES, rk);
       __syncwarp();
       if (lane == 0) mbar_arrive(&kfull[st]);
@@ -465,8 +479,8 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     bool ok = true;
     const auto scores_of = [&](int i) {  // when K is there and the buffer is free
       if (!for_s || !ok || i >= tiles) return;
-      ok = prompt_wait_warp(&kfull[i % ST], (i / ST) & 1, abort);
-      if (i > 1) ok = ok && prompt_wait_warp(&odone[4 * q + (i - 2) % 4], ((i - 2) >> 2) & 1, abort);
+      ok = wait(&kfull[i % ST], (i / ST) & 1);
+      if (i > 1) ok = ok && wait(&odone[4 * q + (i - 2) % 4], ((i - 2) >> 2) & 1);
       if (!ok) return;
       tc_fence_after();
       scores(i);
@@ -475,7 +489,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     scores_of(1);
     for (int i = 0; ok && i < tiles; i++) {
       if (for_o) {  // when V and the weights are there
-        ok = prompt_wait_warp(&vfull[i % ST], (i / ST) & 1, abort) && prompt_wait_warp(&pfull[2 * q + (i & 1)], (i >> 1) & 1, abort);
+        ok = wait(&vfull[i % ST], (i / ST) & 1) && wait(&pfull[2 * q + (i & 1)], (i >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
         outputs(i);
@@ -529,7 +543,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
     };
     for (int i = 0; i < nt; i++) {
       if (HILO && i > 0 && i % PROMPT_FLUSH == 0) {
-        if (!(ok = prompt_wait_warp(&odone[4 * q + (i - 1) % 4], ((i - 1) >> 2) & 1, abort))) break;
+        if (!(ok = wait(&odone[4 * q + (i - 1) % 4], ((i - 1) >> 2) & 1))) break;
         tc_fence_after();
         const float keep = ex2(sum_r - r);
         for (int c = 0; c < a.hd; c += 32) {
@@ -547,7 +561,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         summed = true;
       }
       const int buf = 2 * q + (i & 1);
-      if (!(ok = prompt_wait_warp(&sfull[buf], (i >> 1) & 1, abort))) break;
+      if (!(ok = wait(&sfull[buf], (i >> 1) & 1))) break;
       tc_fence_after();
       const uint32_t ts = tl + buf * S::TMEM_S;
       const int key0 = k00 + i * KT;
@@ -614,7 +628,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
         const float f = ex2(r - nr);  // 0 for the first keys of a row, else a power of two
         l *= f;
         if (HILO ? i % PROMPT_FLUSH != 0 : i > 0) {  // O is rescaled once the previous tile's product is in it
-          if (!(ok = prompt_wait_warp(&odone[4 * q + (i - 1) % 4], ((i - 1) >> 2) & 1, abort))) break;
+          if (!(ok = wait(&odone[4 * q + (i - 1) % 4], ((i - 1) >> 2) & 1))) break;
           tc_fence_after();
           for (int c = 0; c < a.hd; c += 32) {
             tmem_ld32(to + c, v[0]);
@@ -639,7 +653,7 @@ __global__ void __launch_bounds__(PromptShape<HD, HILO>::THREADS, 1) gg_kv8_prom
       if (lane == 0) mbar_arrive(&pfull[buf]);
     }
     if (ok && nt) {
-      ok = prompt_wait_warp(&odone[4 * q + (nt - 1) % 4], ((nt - 1) >> 2) & 1, abort);
+      ok = wait(&odone[4 * q + (nt - 1) % 4], ((nt - 1) >> 2) & 1);
       tc_fence_after();
     }
     l *= 1.f / KV8_WMUL;
@@ -729,6 +743,11 @@ static cudaError_t launch_prompt_hd(const Kv8Args& a, int code, cudaStream_t s) 
   const bool hilo = a.q_type == GG_T_F32;
   if (code == GG_KV8_INT8) return hilo ? launch_prompt<HD, GG_KV8_INT8, true>(a, s) : launch_prompt<HD, GG_KV8_INT8, false>(a, s);
   return hilo ? launch_prompt<HD, GG_KV8_E4M3, true>(a, s) : launch_prompt<HD, GG_KV8_E4M3, false>(a, s);
+}
+
+cudaError_t kv8_wait_probe(uint32_t* err, unsigned long long timeout_ns, cudaStream_t s) {
+  gg_kv8_wait_probe_kernel<<<1, 32, 0, s>>>(err, timeout_ns);
+  return cudaGetLastError();
 }
 
 int kv8_prompt_tile(int head_dim) { return head_dim <= 128 ? 256 : 128; }

@@ -19,6 +19,10 @@ int ops_check_stream(const char* fn, cudaStream_t s);
 // GG_OK if the view is usable for `rows` rows of head_dim values.
 int ops_check_rows(const char* fn, const char* name, const gg_rows* v, int rows, int head_dim);
 int ops_check_cache(const char* fn, const gg_kv8_cache* c);
+// gg_kv8_attention whose waits are bounded by timeout_ns; one that runs out sets GG_ERR_WAIT_MBAR in *err
+// (device memory, or NULL) and leaves NaN in the rows concerned.
+int kv8_attention_bounded(const gg_kv8_cache* c, const gg_kv8_attention_call* call, cudaStream_t s, uint32_t* err, uint64_t timeout_ns);
+constexpr uint64_t KV8_TIMEOUT_NS = 2000000000ull;  // of gg_kv8_attention
 
 inline int ops_type_bytes(int type) { return type == GG_T_F32 ? 4 : 2; }
 // Every head of the view starts on a 16-byte boundary.
