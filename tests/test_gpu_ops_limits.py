@@ -145,3 +145,30 @@ def test_append_skipped_rows(code, dtype, H, D, B, nb):
             assert np.array_equal(f64(got), want), slots[:20]
         for got, want in ((c.k_codes, raws[0]), (c.v_codes, raws[1])):
             assert np.array_equal(raw(got), want), slots[:20]
+
+
+# ------------------------------------------------------------------------- every kernel in one process
+
+def test_attend_raises_no_limit_twice():
+    """All kernels of the attention (a process may use them all) raise their shared-memory limit on their first
+    launch, and no later call does so again."""
+    from torch.profiler import ProfilerActivity, profile
+    rng = np.random.default_rng(3)
+    lens, cu = [300], dev([0, 40])
+    caches = [make_batch(rng, None, lens, 16, 1, D, code) for D in (64, 128, 256) for code in ("int8", "e4m3")]
+    qs = {(heads, D, dtype): torch.randn(40, heads, D, device="cuda").to(DT[dtype]) for heads in (8, 16, 32) for D in (64, 128, 256) for dtype in ("f32", "bf16")}
+
+    def every():
+        for c, _, _, table in caches:
+            for dtype in ("f32", "bf16"):
+                for heads, max_rows in ((8, 1), (16, 1), (32, 1), (8, 40)):
+                    c.attend(qs[heads, c.head_dim, dtype], cu, dev(lens), dev(table), max_rows=max_rows, max_len=300)
+        torch.cuda.synchronize()
+
+    every()
+    with profile(activities=[ProfilerActivity.CPU, ProfilerActivity.CUDA]) as p:
+        every()
+    names = [e.name for e in p.events()]
+    assert len({n for n in names if "gg_kv8_rows_kernel" in n or "gg_kv8_prompt_kernel" in n}) == 44
+    assert sum(n.startswith("cudaLaunchKernel") for n in names) >= 48
+    assert not [n for n in names if n.startswith("cudaFuncSetAttribute")]

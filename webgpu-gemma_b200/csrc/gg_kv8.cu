@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(MERGE_THREADS) gg_kv8_merge_rows_kernel(const 
 
 template <int HD, int CODE, bool HILO, int NT>
 cudaError_t launch_rows(const Kv8Args& a, cudaStream_t s) {
-  return launch_big_smem(gg_kv8_rows_kernel<HD, CODE, HILO, NT>, dim3((unsigned)a.few_ctas), dim3(KV8_WARPS * 32), RowsShape<HD, HILO, NT>::SMEM, s, a);
+  return launch_big_smem<gg_kv8_rows_kernel<HD, CODE, HILO, NT>>(dim3((unsigned)a.few_ctas), dim3(KV8_WARPS * 32), RowsShape<HD, HILO, NT>::SMEM, s, a);
 }
 template <int HD, int CODE, bool HILO>
 cudaError_t launch_rows_nt(const Kv8Args& a, int nt, cudaStream_t s) {

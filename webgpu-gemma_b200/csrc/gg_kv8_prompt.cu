@@ -736,7 +736,7 @@ template <int HD, int CODE, bool HILO>
 static cudaError_t launch_prompt(const Kv8Args& a, cudaStream_t s) {
   typedef PromptShape<HD, HILO> S;
   const long long grid = (long long)a.seqs * a.kv_heads * a.row_tiles * a.splits;
-  return launch_big_smem(gg_kv8_prompt_kernel<HD, CODE, HILO>, dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s, a);
+  return launch_big_smem<gg_kv8_prompt_kernel<HD, CODE, HILO>>(dim3((unsigned)grid), dim3(S::THREADS), S::SMEM, s, a);
 }
 template <int HD>
 static cudaError_t launch_prompt_hd(const Kv8Args& a, int code, cudaStream_t s) {

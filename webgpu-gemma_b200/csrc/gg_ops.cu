@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <type_traits>
 
 #include "gg_launch.h"
 #include "gg_ops.h"
@@ -383,6 +384,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) gg_plan_many_kernel(const gg_blo
   if (inline_rows)
     for (int r = total + t; r < p.rows; r += PLAN_THREADS) p.row_seq[r] = p.positions[r] = p.slots[r] = -1;
 }
+
+template <void (*Kernel)(const gg_block_plan, int)>
+using PlanKernel = std::integral_constant<void (*)(const gg_block_plan, int), Kernel>;
 
 // The row arrays of a large plan, one row per thread (after gg_plan_kernel).
 constexpr int PLAN_ROWS_SMEM = 8192;  // requests whose cu_rows fit this kernel's shared memory
@@ -810,12 +814,13 @@ extern "C" int gg_plan_blocks(const gg_block_plan* plan, void* stream) {
   if (int rc = ops_check_stream(fn, s)) return rc;
   const int inline_rows = p.rows <= PLAN_INLINE_ROWS;
   static_assert(sizeof(PlanScan) > 48 * 1024 && sizeof(PlanScan) < 64 * 1024, "opt-in shared memory");
-  auto kernel = gg_plan_many_kernel;
-  int threads = PLAN_THREADS;
-  if (p.seqs <= 256) kernel = gg_plan_kernel<256, 1>, threads = 256;
-  else if (p.seqs <= PLAN_THREADS) kernel = gg_plan_kernel<PLAN_THREADS, 1>;
-  else if (p.seqs <= PLAN_CHUNK) kernel = gg_plan_kernel<PLAN_THREADS, PLAN_PER>;
-  cudaError_t r = launch_big_smem(kernel, dim3(1), dim3(threads), sizeof(PlanScan), s, p, inline_rows);
+  const auto launch = [&](auto kernel, int threads) {
+    return launch_big_smem<kernel.value>(dim3(1), dim3(threads), sizeof(PlanScan), s, p, inline_rows);
+  };
+  cudaError_t r = p.seqs <= 256            ? launch(PlanKernel<gg_plan_kernel<256, 1>>(), 256)
+                  : p.seqs <= PLAN_THREADS ? launch(PlanKernel<gg_plan_kernel<PLAN_THREADS, 1>>(), PLAN_THREADS)
+                  : p.seqs <= PLAN_CHUNK   ? launch(PlanKernel<gg_plan_kernel<PLAN_THREADS, PLAN_PER>>(), PLAN_THREADS)
+                                           : launch(PlanKernel<gg_plan_many_kernel>(), PLAN_THREADS);
   if (r == cudaSuccess && !inline_rows) {
     const int grid = (int)(((long long)p.rows + 255) / 256);
     r = launch_pdl(gg_plan_rows_kernel, dim3(grid < 1184 ? grid : 1184), dim3(256), 0, s, p);

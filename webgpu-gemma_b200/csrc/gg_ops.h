@@ -34,28 +34,24 @@ inline bool ops_aligned16(const gg_rows& v) {
 namespace gg {
 
 // launch_pdl of a kernel that needs more dynamic shared memory than the default limit. The limit is
-// raised on the kernel's first launch on a device, and again when a launch is refused: a context made after cudaDeviceReset has forgotten it.
-template <typename... KArgs, typename... Args>
-inline cudaError_t launch_big_smem(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, Args... args) {
-  static std::atomic<void*> known[64][32];  // kernels of this signature whose limit is raised, per device
+// raised on the kernel's first launch on a device, and again when a launch is refused: a context made
+// after cudaDeviceReset has forgotten it.
+template <auto Kernel, typename... Args>
+inline cudaError_t launch_big_smem(dim3 grid, dim3 block, size_t smem, cudaStream_t s, const Args&... args) {
+  static std::atomic<uint64_t> raised;  // devices, by bit
   int dev = 0;
   cudaError_t r = cudaGetDevice(&dev);
   if (r != cudaSuccess) return r;
-  std::atomic<void*>* seen = known[dev & 63];
-  bool raised = false;
-  for (int i = 0; i < 32 && dev < 64; i++) raised |= seen[i].load(std::memory_order_acquire) == reinterpret_cast<void*>(kernel);
-  if (raised) {
-    r = launch_pdl(kernel, grid, block, smem, s, args...);
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (raised.load(std::memory_order_acquire) & bit) {
+    r = launch_pdl(Kernel, grid, block, smem, s, args...);
     if (r != cudaErrorInvalidValue) return r;
     cudaGetLastError();
   }
-  r = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  r = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (r != cudaSuccess) return r;
-  for (int i = 0; i < 32 && !raised && dev < 64; i++) {
-    void* none = nullptr;
-    if (seen[i].compare_exchange_strong(none, reinterpret_cast<void*>(kernel), std::memory_order_acq_rel)) break;
-  }
-  return launch_pdl(kernel, grid, block, smem, s, args...);
+  raised.fetch_or(bit, std::memory_order_acq_rel);
+  return launch_pdl(Kernel, grid, block, smem, s, args...);
 }
 
 GG_DEV float to_f32(float v) { return v; }
