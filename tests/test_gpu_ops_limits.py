@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import ops_reference as ref
-from test_gpu_ops import DT, check_attend, dev, f64, make_batch, new_cache, raw
+from test_gpu_ops import DT, HALF_EPS, check_attend, dev, f64, make_batch, new_cache, raw
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -172,3 +172,58 @@ def test_attend_raises_no_limit_twice():
     assert len({n for n in names if "gg_kv8_rows_kernel" in n or "gg_kv8_prompt_kernel" in n}) == 44
     assert sum(n.startswith("cudaLaunchKernel") for n in names) >= 48
     assert not [n for n in names if n.startswith("cudaFuncSetAttribute")]
+
+
+# ------------------------------------------------------------------------- long sums
+
+@pytest.mark.parametrize("D, H, n", [(64, 8, 40), (128, 4, 80), (256, 1, 300)])
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_attend_sums_over_many_keys_of_a_warp(code, D, H, n):
+    """Single f32 tokens of so many requests that none is cut: a warp sums 16384 keys. All values are positive and
+    all weights alike, so a sum that is always rounded one way would be off by 1e-4. The requests share
+    their pages. Tolerance as in check_attend."""
+    from gemma_b200 import ops
+    B, L, G = 128, 65536, 4
+    g = torch.Generator(device="cuda").manual_seed(D)
+    c = ops.KV8Cache.empty(L // B, B, H, D, code)
+    for t, lo in ((c.k_codes, -127), (c.v_codes, 64)):
+        t.copy_(torch.randint(lo, 128, t.shape, device="cuda", generator=g).float().to(t.dtype))
+    c.k_scale.fill_(2.0 ** -20)
+    table = torch.arange(L // B, dtype=torch.int32, device="cuda").repeat(n, 1)
+    q = torch.randn(n, H * G, D, device="cuda", generator=g)
+    out, lse = c.attend(q, torch.arange(n + 1, dtype=torch.int32, device="cuda"), torch.full((n,), L, dtype=torch.int32, device="cuda"), table,
+                        max_rows=1, max_len=L, return_lse=True)
+    for i, h in ((0, 0), (n - 1, H - 1)):
+        k, v = (t[:, h].float().double().reshape(-1, D) for t in (c.k_codes, c.v_codes))
+        z = q[i, h * G:(h + 1) * G].double() @ (k * 2.0 ** -20).T * D ** -0.5
+        want = torch.softmax(z, -1) @ v  # the values are positive: also the sum of p |v|
+        ds = (q[i, h * G:(h + 1) * G].double().abs() @ (k.abs() * 2.0 ** -20).T * D ** -0.5).amax(-1, keepdim=True) * (2.0 ** -21 + 2.0 ** -19) + 2.0 ** -22
+        tol = (2 * (2 * ds + 2.0 ** -18) + 2.0 ** -24) * want
+        got = out[i, h * G:(h + 1) * G].double()
+        assert bool(((got - want).abs() <= tol).all()), ((got - want) / want).abs().max().item()
+        assert bool(((lse[i, h * G:(h + 1) * G].double() - torch.logsumexp(z, -1)).abs() <= ds[:, 0] + 2.0 ** -20 + 2.0 ** -22 * 12).all())
+
+
+@pytest.mark.parametrize("rows, n, L", [(1, 300, 1 << 22), (128, 75, 1 << 22)])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_attend_sums_over_millions_of_keys(dtype, rows, n, L):
+    """16-bit rows over contexts beyond 2^18 keys, more (request, head) units than the GPU holds: no sum may lose
+    more than its rounding. Tolerance as in check_attend; all values are positive, the requests share their pages."""
+    from gemma_b200 import ops
+    B, D, G = 128, 16, 4 if rows == 1 else 2
+    g = torch.Generator(device="cuda").manual_seed(L)
+    c = ops.KV8Cache.empty(L // B, B, 1, D, "int8")
+    for t, lo in ((c.k_codes, -127), (c.v_codes, 64)):
+        t.copy_(torch.randint(lo, 128, t.shape, device="cuda", generator=g, dtype=torch.int32))
+    c.k_scale.fill_(2.0 ** -20)
+    table = torch.arange(L // B, dtype=torch.int32, device="cuda").repeat(n, 1)
+    q = torch.randn(n * rows, G, D, device="cuda", generator=g).to(DT[dtype])
+    out = c.attend(q, torch.arange(n + 1, dtype=torch.int32, device="cuda") * rows, torch.full((n,), L, dtype=torch.int32, device="cuda"), table,
+                   max_rows=rows, max_len=L)
+    k, v = (t.double().reshape(-1, D) for t in (c.k_codes, c.v_codes))
+    for i in (rows - 1, n * rows - 1):  # rows that see all keys
+        z = q[i].double() @ (k * 2.0 ** -20).T * D ** -0.5
+        want = torch.softmax(z, -1) @ v
+        ds = (q[i].double().abs() @ (k.abs() * 2.0 ** -20).T * D ** -0.5).amax(-1, keepdim=True) * (2.0 ** -21 + 2.0 ** -19) + 2.0 ** -22
+        tol = (2 * (2 * ds + 2.0 ** -18) + 2 * 2.0 ** -11 + HALF_EPS[dtype]) * want
+        assert bool(((out[i].double() - want).abs() <= tol).all()), ((out[i].double() - want) / want).abs().max().item()

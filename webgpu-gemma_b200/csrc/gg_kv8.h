@@ -10,6 +10,9 @@ namespace gg {
 
 constexpr float KV8_SLACK = 8.f;    // w_j <= 2^8
 constexpr float KV8_WMUL = 128.f;    // weights enter the MMA as w_j 2^7 <= 2^15
+// The tensor cores cut the f32 sums they hold (they do not round them). f16 and bf16 outputs leave O there,
+// so no sum of theirs takes more than 2^18 keys, in steps of 16 (losses: gg_kv8.cu, gg_kv8_prompt.cu).
+constexpr int KV8_LONGEST = 1 << 14;
 constexpr float KV8_NEG = -1e30f;   // stands for -inf in running maxima (no inf - inf)
 
 struct Kv8Args {
@@ -45,6 +48,16 @@ GG_DEV void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+GG_DEV void mma_f16_from_zero(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
+}
+GG_DEV void add_f32x2(float& a, float& b, float c, float d) {  // a += c, b += d, each rounded to nearest
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "+f"(a), "+f"(b)
+      : "f"(c), "f"(d));
 }
 GG_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {  // bytes 0: fills zeros, reads nothing
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");

@@ -28,8 +28,8 @@
 //
 // The tensor cores cut the f32 sums they hold: measured, a sum loses 6e-10 of itself a key and
 // product, always downwards (1.1e-5 after 8192 keys with both products of f32 queries). For f16 and
-// bf16 outputs that stays below their own rounding up to 2^18 keys. For f32 ones O is added to an f32
-// row in memory (the row of the output itself) every PROMPT_FLUSH tiles and starts again from zero.
+// bf16 outputs that stays below their own rounding up to 2^18 keys, the most that a range has
+// (KV8_LONGEST). For f32 ones O is added to an f32 row in memory (the row of the output itself) every PROMPT_FLUSH tiles and starts again from zero.
 #include "gg_kv8.h"
 #include "gg_tc.cuh"
 
