@@ -227,3 +227,25 @@ def test_attend_sums_over_millions_of_keys(dtype, rows, n, L):
         ds = (q[i].double().abs() @ (k.abs() * 2.0 ** -20).T * D ** -0.5).amax(-1, keepdim=True) * (2.0 ** -21 + 2.0 ** -19) + 2.0 ** -22
         tol = (2 * (2 * ds + 2.0 ** -18) + 2 * 2.0 ** -11 + HALF_EPS[dtype]) * want
         assert bool(((out[i].double() - want).abs() <= tol).all()), ((out[i].double() - want) / want).abs().max().item()
+
+
+# ------------------------------------------------------------------------- what autograd would follow
+
+def test_rope_refuses_tangents_and_learned_frequencies():
+    """Neither a dual tensor nor frequencies that require a gradient lose it silently."""
+    from gemma_b200 import ops
+    from torch.autograd import forward_ad
+    x, pos = torch.randn(4, 2, 32, device="cuda"), torch.arange(4, dtype=torch.int32, device="cuda")
+    f, _ = ops.rope_frequencies(32, 1e4)
+    want = ops.rope(x, None, pos, f)[0]
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for q, k, fr in ((dual, None, f), (x, dual, f), (x, None, forward_ad.make_dual(f, f))):
+            with pytest.raises(ValueError, match="tangent"):
+                ops.rope(q, k, pos, fr)
+        assert torch.equal(ops.rope(x, None, pos, f)[0], want)
+    learned = f.clone().requires_grad_()
+    with pytest.raises(ValueError, match="freqs requires a gradient"):
+        ops.rope(x, None, pos, learned)
+    with torch.no_grad():
+        assert torch.equal(ops.rope(x, None, pos, learned)[0], want)

@@ -54,3 +54,20 @@ def test_attention_workspace_grows_with_the_length(lib, type_, kv, group, dim): 
             assert need.value >= last, (seqs, max_rows, window, max_len)
             last = need.value
         assert last > 0
+
+
+def test_gradients_of_either_mode_are_refused():
+    """A tensor that requires a gradient, and a dual tensor, whose requires_grad is False."""
+    torch = pytest.importorskip("torch")
+    from torch.autograd import forward_ad
+    from gemma_b200 import ops
+    x = torch.zeros(2, 1, 32)
+    assert ops._rows("q", x, -1)[3] == 1  # (-1: where a CPU tensor is; the wrappers never come here with one)
+    with pytest.raises(ValueError, match="gradient"):
+        ops._rows("q", x.clone().requires_grad_(), -1)
+    with torch.no_grad():
+        ops._rows("q", x.clone().requires_grad_(), -1)
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="tangent"):
+            ops._rows("q", forward_ad.make_dual(x, torch.ones_like(x)), -1)
+        ops._rows("q", x, -1)

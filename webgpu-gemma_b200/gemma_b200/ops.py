@@ -11,7 +11,8 @@ Each is one or two kernels of libgemma_b200.so on the current stream of the tens
 (declarations, formulas and limits: include/gemma_b200.h). Nothing is synchronised or copied to the host and every call may
 be captured into a CUDA graph. Shapes, types and devices are checked here (ValueError); lengths,
 slots and block ids live on the device and are bounds-checked by the kernels. No operator records
-gradients: tensors that require one are refused while grad mode is on. The gradient of ``rope`` is
+gradients: tensors that require one are refused while grad mode is on, and so are dual tensors of
+forward-mode differentiation. The gradient of ``rope`` is
 ``rope(..., inverse=True)`` of the outputs' gradients.
 """
 from __future__ import annotations
@@ -22,6 +23,7 @@ from functools import lru_cache
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import native
 from .native import GG_OK, GemmaB200Error, GGKv8AttentionCall, GGKv8Cache, GGRows
@@ -80,6 +82,14 @@ def _elsewhere(name: str, t: torch.Tensor, index: int):
     raise ValueError(f"{name} is on {t.device}, the other tensors on cuda:{index}")
 
 
+def _no_gradient(name: str, t: torch.Tensor):
+    """Refuses what autograd would follow: in reverse mode, or as a dual tensor in forward mode."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which this operator does not record")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} carries a tangent, which this operator does not propagate")
+
+
 def _rows(name: str, t: torch.Tensor, index: int) -> tuple:
     """gg_rows of a [rows][heads][head_dim] tensor of any strides with contiguous heads."""
     stride = t.stride()
@@ -90,8 +100,8 @@ def _rows(name: str, t: torch.Tensor, index: int) -> tuple:
         raise ValueError(f"{name} must be float32, bfloat16 or float16, not {t.dtype}")
     if t.get_device() != index:
         _elsewhere(name, t, index)
-    if t.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"{name} requires a gradient, which this operator does not record")
+    if t.requires_grad or forward_ad._current_level >= 0:
+        _no_gradient(name, t)
     shape = t.shape
     if stride[2] != 1 and shape[2] > 1:
         raise ValueError(f"the values of a head of {name} must be contiguous (stride {stride[2]})")
@@ -191,6 +201,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs
         raise ValueError("freqs must be a contiguous float64 vector (rope_frequencies)")
     if freqs.get_device() != dev:
         _elsewhere("freqs", freqs, dev)
+    if freqs.requires_grad or forward_ad._current_level >= 0:
+        _no_gradient("freqs", freqs)
     vq = _rows("q", q, dev)
     n, _, dim = q.shape
     vk = wk = _NO_ROWS
