@@ -277,8 +277,9 @@ int gg_rope(const gg_rope_call* call, void* stream);
  *                   t = (trained w_i / 2 pi - low) / (high - low)
  *   GG_ROPE_YARN    t w_i + (1 - t) w_i / factor, t = 1 up to the pair that turns `high` times in
  *                   the trained positions, 0 from the pair that turns `low` times, linear in i
- *                   between (the border pairs rounded outwards); *mscale = 0.1 ln(factor) + 1
- * *mscale is 1 for the others. low < high; trained, low, high are ignored by the first two. */
+ *                   between (the border pairs rounded outwards); *mscale = 0.1 ln(factor) + 1 for a
+ *                   factor above 1 (a context that is stretched)
+ * *mscale is 1 otherwise. low < high; trained, low, high are ignored by the first two. */
 #define GG_ROPE_NONE 0
 #define GG_ROPE_LINEAR 1
 #define GG_ROPE_BANDS 2

@@ -1,5 +1,6 @@
 """Sizes at the edge of what the operators take, on the host: refusals and workspaces, without a GPU."""
 import ctypes
+import math
 import subprocess
 import sys
 
@@ -7,7 +8,7 @@ import pytest
 
 from conftest import ROOT
 from gemma_b200 import native
-from test_ops_host import attend, cache, lib, rows  # noqa: F401 (lib is a fixture)
+from test_ops_host import attend, cache, freqs, lib, rows  # noqa: F401 (lib is a fixture)
 
 HUGE = """
 import ctypes, sys
@@ -71,3 +72,11 @@ def test_gradients_of_either_mode_are_refused():
         with pytest.raises(ValueError, match="tangent"):
             ops._rows("q", forward_ad.make_dual(x, torch.ones_like(x)), -1)
         ops._rows("q", x, -1)
+
+
+@pytest.mark.parametrize("factor", [0.25, 0.5, 1.0, 1.0000001, 4.0])
+def test_yarn_never_shrinks_the_rotation(lib, factor):  # noqa: F811
+    """cos and sin are lengthened where a context is stretched, and left alone where it is not."""
+    rc, f, m = freqs(lib, native.GG_ROPE_YARN, 64, factor=factor, trained=32768.0, low=1.0, high=32.0)
+    assert rc == 0 and m == (pytest.approx(0.1 * math.log(factor) + 1, rel=1e-15) if factor > 1 else 1.0)
+    assert f[0] == pytest.approx(1.0, rel=1e-15) and f[-1] == pytest.approx(1e6 ** (-62 / 64) / factor, rel=1e-13)

@@ -894,7 +894,7 @@ extern "C" int gg_rope_freqs(int scaling, int rot_dim, double theta, double fact
     last = std::fmin(std::ceil(pair(low)), rot_dim - 1.0);
     if (last - first < 0.001) last = first + 0.001;
   }
-  *mscale = scaling == GG_ROPE_YARN ? 0.1 * std::log(factor) + 1.0 : 1.0;
+  *mscale = scaling == GG_ROPE_YARN && factor > 1.0 ? 0.1 * std::log(factor) + 1.0 : 1.0;
   for (int i = 0; i < n; i++) {
     const double w = std::pow(theta, -2.0 * i / rot_dim);
     double keep = 1.0;  // share of the unscaled frequency
