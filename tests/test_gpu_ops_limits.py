@@ -249,3 +249,18 @@ def test_rope_refuses_tangents_and_learned_frequencies():
         ops.rope(x, None, pos, learned)
     with torch.no_grad():
         assert torch.equal(ops.rope(x, None, pos, learned)[0], want)
+
+
+# ------------------------------------------------------------------------- large keys, small queries
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows, lens", [([1, 1], [90, 700]), ([40], [300])])
+def test_attend_large_keys_small_queries(dtype, rows, lens):
+    """Scores of ordinary size from keys of 2^120, queries of 2^-100 and a scale of 2^-16: no step between them
+    overflows."""
+    rng = np.random.default_rng(2)
+    c, raws, scales, table = make_batch(rng, rows, lens, 16, 1, 64, "int8")
+    scales[0][:] = 2.0 ** 113
+    c.k_scale.fill_(2.0 ** 113)
+    q = (torch.randn(sum(rows), 4, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) * 2.0 ** -40).to(DT[dtype])
+    check_attend(rng, rows, lens, 4, c, raws, scales, table, "int8", dtype, q=q * 2.0 ** -60, scale=2.0 ** -16)

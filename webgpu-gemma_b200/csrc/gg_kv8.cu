@@ -374,26 +374,27 @@ __global__ void __launch_bounds__(KV8_WARPS * 32, RowsShape<HD, HILO, NT>::CTAS)
       float w[4];
 #pragma unroll
       for (int e = 0; e < 2; e++) {
+        const float f = ks * mul[u][e];  // (before it meets the sum: large keys may go with small queries)
         float sc[2], top = KV8_NEG;
         bool seen[2];
 #pragma unroll
         for (int k = 0; k < 2; k++) {
           const int key = key0 + g + 8 * k;
           seen[k] = key <= hi_key[u][e] && key >= lo_key[u][e] && iv != 0.f;
-          sc[k] = seen[k] ? fmaf((c[u][0][2 * k + e] + c[u][1][2 * k + e]) * ks, mul[u][e], lv) : KV8_NEG;
+          sc[k] = seen[k] ? fmaf(c[u][0][2 * k + e] + c[u][1][2 * k + e], f, lv) : KV8_NEG;
           top = fmaxf(top, sc[k]);
         }
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         if (__any_sync(0xffffffffu, top > rmax[u][e] + KV8_SLACK)) {
           const float nr = top > rmax[u][e] + KV8_SLACK ? top : rmax[u][e];
-          const float f = ex2(rmax[u][e] - nr);  // rmax = KV8_NEG: 2^-huge = 0
+          const float down = ex2(rmax[u][e] - nr);  // rmax = KV8_NEG: 2^-huge = 0
           rmax[u][e] = nr;
-          lsum[u][e] *= f;
+          lsum[u][e] *= down;
 #pragma unroll
           for (int d = 0; d < OT; d++) {
-            o[u][d][e] *= f;
-            o[u][d][2 + e] *= f;
+            o[u][d][e] *= down;
+            o[u][d][2 + e] *= down;
           }
         }
 #pragma unroll
