@@ -294,7 +294,8 @@ int gg_rope_freqs(int scaling, int rot_dim, double theta, double factor, double 
  *   free_list[0 .. *free_count); then growing requests take theirs from its top, in request and
  *   block order. Tokens old_len[i] .. new_len[i] - 1 become rows cu_rows[i] .. cu_rows[i + 1] - 1.
  *   Outputs: cu_rows [seqs + 1], lens [seqs] (= new_len), row_seq / positions / slots [rows]
- *   (slot = block * block_tokens + position % block_tokens; all three -1 behind the last row),
+ *   (slot = block * block_tokens + position % block_tokens, or -1 if that is not from 0 to 2^31 - 1; all three
+ *   -1 behind the last row),
  *   *free_count_out (may be free_count itself) and *status, a sum of GG_PLAN_* bits.
  * All or nothing: with a status other than 0 the table, the list and the count stay as they were,
  * lens = old_len, cu_rows is all 0 and every row is padding, so later operators do nothing. */

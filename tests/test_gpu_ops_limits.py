@@ -264,3 +264,31 @@ def test_attend_large_keys_small_queries(dtype, rows, lens):
     c.k_scale.fill_(2.0 ** 113)
     q = (torch.randn(sum(rows), 4, 64, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)) * 2.0 ** -40).to(DT[dtype])
     check_attend(rng, rows, lens, 4, c, raws, scales, table, "int8", dtype, q=q * 2.0 ** -60, scale=2.0 ** -16)
+
+
+# ------------------------------------------------------------------------- block ids that no cache has
+
+@pytest.mark.parametrize("n, chunk", [(3, 20), (700, 5), (5000, 2), (64, 100)])
+def test_plan_of_impossible_block_ids(n, chunk):
+    """Ids below 0, and so large that their slots pass 31 bits, from the table or from the free list: the rows
+    there have no slot. (Wrapped around, they would be another request's.)"""
+    from gemma_b200 import ops
+    B = 16
+    rng = np.random.default_rng(n)
+    old = rng.integers(0, 40, n)
+    new = old + chunk
+    blocks = -(-int(new.max()) // B)
+    held = -(-old // B)
+    bad = np.array([-1, -2 ** 27, 2 ** 27, 2 ** 27 + 3, 2 ** 28 + 1, 2 ** 31 - 1, -2 ** 31])
+    ids = np.where(rng.random(n * (blocks + 1)) < 0.3, rng.choice(bad, n * (blocks + 1)), rng.integers(0, 2 ** 27, n * (blocks + 1)))
+    table = np.where(np.arange(blocks)[None] < held[:, None], ids[:n * blocks].reshape(n, blocks), -1)
+    free = rng.permutation(ids)
+    rows = n * chunk + 3
+    t, fl = dev(table), dev(free)
+    p = ops.plan_blocks(dev(old), dev(new), t, fl, dev([len(free)]), B, rows)
+    assert int(p.status) == 0
+    t = t.cpu().numpy().astype(np.int64)
+    slots = [t[i, x // B] * B + x % B for i in range(n) for x in range(old[i], new[i])]
+    want = [int(s) if 0 <= s < 2 ** 31 else -1 for s in slots] + [-1] * 3
+    assert want.count(-1) > 3  # some rows stand in such a block
+    assert p.slots.cpu().tolist() == want

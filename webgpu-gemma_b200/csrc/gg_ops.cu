@@ -103,6 +103,12 @@ GG_DEV int find_segment(const int* pre, int n, int k) {
   return lo;
 }
 
+// Slot of position pos in a block; -1 for an id that no cache has (below 0, or with slots beyond 31 bits).
+GG_DEV int plan_slot(int id, int pos, int B) {
+  const long long s = (long long)id * B + pos % B;
+  return s >= 0 && s <= 0x7fffffff ? (int)s : -1;
+}
+
 GG_DEV int plan_blocks_of(int len, int B) { return len > 0 ? (int)((uint32_t)(len - 1) / (uint32_t)B) + 1 : 0; }
 
 // Exclusive prefix sums of the chunk's requests i0 .. i0 + n - 1. Called with a plan that passed
@@ -276,7 +282,7 @@ __global__ void __launch_bounds__(THREADS) gg_plan_kernel(const gg_block_plan p,
       const int i = find_segment(sc.rows, n, r), pos = p.old_len[i] + r - sc.rows[i];
       p.row_seq[r] = i;
       p.positions[r] = pos;
-      p.slots[r] = p.table[(long long)i * p.table_stride + pos / B] * B + pos % B;
+      p.slots[r] = plan_slot(p.table[(long long)i * p.table_stride + pos / B], pos, B);
     }
     for (int r = total + t; r < p.rows; r += THREADS) p.row_seq[r] = p.positions[r] = p.slots[r] = -1;
   }
@@ -372,7 +378,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) gg_plan_many_kernel(const gg_blo
           const int pos = p.old_len[i0 + i] + r - sc.rows[i];
           p.row_seq[base_rows + r] = i0 + i;
           p.positions[base_rows + r] = pos;
-          p.slots[base_rows + r] = p.table[(long long)(i0 + i) * p.table_stride + pos / B] * B + pos % B;
+          p.slots[base_rows + r] = plan_slot(p.table[(long long)(i0 + i) * p.table_stride + pos / B], pos, B);
         }
       base_take += sc.take[n];
       base_rows += sc.rows[n];
@@ -407,7 +413,7 @@ __global__ void __launch_bounds__(256) gg_plan_rows_kernel(const gg_block_plan p
     if (r < total) {
       seq = find_segment(pre, p.seqs, r);
       pos = p.old_len[seq] + r - pre[seq];
-      slot = p.table[(long long)seq * p.table_stride + pos / B] * B + pos % B;
+      slot = plan_slot(p.table[(long long)seq * p.table_stride + pos / B], pos, B);
     }
     p.row_seq[r] = seq;
     p.positions[r] = pos;
