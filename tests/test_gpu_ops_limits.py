@@ -292,3 +292,18 @@ def test_plan_of_impossible_block_ids(n, chunk):
     want = [int(s) if 0 <= s < 2 ** 31 else -1 for s in slots] + [-1] * 3
     assert want.count(-1) > 3  # some rows stand in such a block
     assert p.slots.cpu().tolist() == want
+
+
+def test_sizes_beyond_32_bits_refused():
+    """As ValueError, before anything of that size is allocated or looked up."""
+    from gemma_b200 import ops
+    c = ops.KV8Cache.empty(4, 16, 1, 32)
+    q, one, t = torch.zeros(1, 4, 32, device="cuda"), dev([1]), dev([[0, 1]])
+    for kw in (dict(max_rows=(1 << 32) + 1, max_len=16), dict(max_rows=1, max_len=16, window=1 << 31), dict(max_rows=1, max_len=-(1 << 40))):
+        with pytest.raises(ValueError, match="32 bits"):
+            c.attend(q, dev([0, 1]), one, t, **kw)
+    with pytest.raises(ValueError, match="32 bits"):
+        c.workspace_bytes(q, 1 << 40, 1, 16)
+    for rows, block in ((1 << 31, 16), (4, 1 << 33)):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.plan_blocks(one, one, t, dev([0]), dev([1]), block, rows)

@@ -80,3 +80,15 @@ def test_yarn_never_shrinks_the_rotation(lib, factor):  # noqa: F811
     rc, f, m = freqs(lib, native.GG_ROPE_YARN, 64, factor=factor, trained=32768.0, low=1.0, high=32.0)
     assert rc == 0 and m == (pytest.approx(0.1 * math.log(factor) + 1, rel=1e-15) if factor > 1 else 1.0)
     assert f[0] == pytest.approx(1.0, rel=1e-15) and f[-1] == pytest.approx(1e6 ** (-62 / 64) / factor, rel=1e-13)
+
+
+@pytest.mark.parametrize("at, name", [(7, "requests"), (8, "rows"), (9, "max_rows"), (10, "max_len"), (11, "window")])
+@pytest.mark.parametrize("value", [1 << 31, (1 << 32) + 1, -(1 << 31) - 1, 1 << 70])
+def test_sizes_beyond_32_bits_refused(lib, at, name, value):  # noqa: F811
+    """Not cut to their low bits on the way into the library."""
+    ops = pytest.importorskip("gemma_b200.ops")
+    sizes = [8, 16, 1, 64, native.GG_KV8_INT8, 4, native.GG_T_F32, 1, 1, 1, 100, 0]
+    assert ops._attend_bytes(*sizes) >= 0
+    sizes[at] = value
+    with pytest.raises(ValueError, match=f"{name} {value} does not fit"):
+        ops._attend_bytes(*sizes)

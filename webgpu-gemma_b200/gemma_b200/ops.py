@@ -90,6 +90,12 @@ def _no_gradient(name: str, t: torch.Tensor):
         raise ValueError(f"{name} carries a tangent, which this operator does not propagate")
 
 
+def _int32(name: str, value: int):
+    """Sizes travel as 32 bits: neither struct nor ctypes may see one that does not fit."""
+    if not -(1 << 31) <= value < 1 << 31:
+        raise ValueError(f"{name} {value} does not fit 32 bits")
+
+
 def _rows(name: str, t: torch.Tensor, index: int) -> tuple:
     """gg_rows of a [rows][heads][head_dim] tensor of any strides with contiguous heads."""
     stride = t.stride()
@@ -155,6 +161,8 @@ def plan_blocks(old_len: torch.Tensor, new_len: torch.Tensor, table: torch.Tenso
     A plan that does not fit changes nothing and says so in ``status``."""
     dev = _gpu_index("old_len", old_len)
     n = old_len.shape[0] if old_len.dim() else 0
+    _int32("rows", rows)
+    _int32("block_tokens", block_tokens)
     if out is None:
         if rows < 0:
             raise ValueError(f"rows must not be negative, not {rows}")
@@ -233,6 +241,8 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, freqs
 @lru_cache(maxsize=1024)
 def _attend_bytes(num_blocks, block_tokens, kv_heads, head_dim, code, heads, type_, seqs, rows, max_rows, max_len, window) -> int:
     """Workspace of a call of these sizes (a pure function of them)."""
+    for name, value in (("requests", seqs), ("rows", rows), ("max_rows", max_rows), ("max_len", max_len), ("window", window)):
+        _int32(name, value)
     c = GGKv8Cache(16, 16, 16, 16, num_blocks, block_tokens, kv_heads, head_dim, code)
     call = GGKv8AttentionCall(q=GGRows(heads=heads, type=type_), seqs=seqs, rows=rows, max_rows=max_rows, max_len=max_len, window=window)
     need = ctypes.c_size_t()
