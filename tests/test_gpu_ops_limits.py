@@ -307,3 +307,111 @@ def test_sizes_beyond_32_bits_refused():
     for rows, block in ((1 << 31, 16), (4, 1 << 33)):
         with pytest.raises(ValueError, match="32 bits"):
             ops.plan_blocks(one, one, t, dev([0]), dev([1]), block, rows)
+
+
+# ------------------------------------------------------------------------- many keys to a CTA
+
+LONG = [511, 512, 513, 1023, 1025, 4095, 4096, 4097, 8191, 8193, 16383, 16385]
+
+
+def long_cache(D, H, B, code, g):
+    """A cache with room for LONG[-1] tokens of one request, random codes and scales, blocks in random order."""
+    from gemma_b200 import ops
+    nb = -(-LONG[-1] // B) + 2
+    c = ops.KV8Cache.empty(nb, B, H, D, code)
+    for t in (c.k_codes, c.v_codes):
+        t.copy_(torch.randint(-127, 128, t.shape, device="cuda", generator=g).float().to(t.dtype))
+    c.k_scale.copy_(2.0 ** torch.randint(-7, -4, c.k_scale.shape, device="cuda", generator=g))
+    c.v_scale.copy_(2.0 ** torch.randint(-9, -3, c.v_scale.shape, device="cuda", generator=g))
+    return c, torch.randperm(nb, device="cuda", generator=g)[:-(-LONG[-1] // B)].int()
+
+
+def check_long(c, row, lens, rows, q, out, lse, window, dtype):
+    """The first and the last row of every request, in the first and the last key head, against softmax in 64
+    bits; tolerances as in check_attend. All requests share the pages of `row`."""
+    B, D, H = c.block_tokens, c.head_dim, c.kv_heads
+    G, w = q.shape[1] // H, 0.0 if dtype == "f32" else 2 * 2.0 ** -11
+    for h in {0, H - 1}:
+        codes = [t.view(torch.int8)[row.long(), h].view(t.dtype).float().double() for t in (c.k_codes, c.v_codes)]
+        ks, vs = (t[row.long(), h].double().repeat_interleave(B) for t in (c.k_scale, c.v_scale))
+        k, v = codes[0].reshape(-1, D) * ks[:, None], codes[1].reshape(-1, D) * vs[:, None]
+        for i, n in enumerate(lens):
+            for r in {0, rows - 1}:
+                p = n - rows + r
+                lo = max(0, p - window + 1) if window else 0
+                x = q[i * rows + r, h * G:(h + 1) * G].double()
+                kk, vv = k[lo:p + 1], v[lo:p + 1]
+                z = x @ kk.T * D ** -0.5
+                pr = torch.softmax(z, -1)
+                want, pv = pr @ vv, pr @ vv.abs()
+                least = (pr * vs[lo:p + 1]).amax(-1, keepdim=True) * (vv.abs() / vs[lo:p + 1, None]).sum(0)
+                ds = (x.abs() @ kk.abs().T).amax(-1, keepdim=True) * D ** -0.5 * (2.0 ** -21 + 2.0 ** -19) + 2.0 ** -22
+                tol = (2 * (2 * ds + 2.0 ** -18) + w) * pv + HALF_EPS[dtype] * want.abs() + (2.0 ** -25 if dtype == "f16" else 0) + 2.0 ** -32 * least
+                got = out[i * rows + r, h * G:(h + 1) * G].double()
+                assert bool(((got - want).abs() <= tol).all()), (h, i, r, ((got - want).abs() / tol).max().item())
+                ref_lse = torch.logsumexp(z, -1)
+                err = (lse[i * rows + r, h * G:(h + 1) * G].double() - ref_lse).abs()
+                assert bool((err <= ds[:, 0] + 2.0 ** -20 + 2.0 ** -22 * ref_lse.abs()).all()), (h, i, r)
+
+
+def attend_long(c, row, lens, rows, q, window, odd):
+    n = len(lens)
+    table = row.repeat(n, 1)
+    room = torch.full((n * rows * (q.shape[1] * c.head_dim + 3) + 1,), 7.0, device="cuda", dtype=q.dtype)
+    width = q.shape[1] * c.head_dim + (3 if odd else 0)
+    out = torch.as_strided(room, q.shape, (width, c.head_dim, 1), 1 if odd else 0)
+    _, lse = c.attend(q, torch.arange(n + 1, dtype=torch.int32, device="cuda") * rows, dev(lens), table, max_rows=rows, max_len=max(lens),
+                      window=window, out=out, return_lse=True)
+    return out, lse
+
+
+def ranges(c, q, n, rows, window):
+    """Key ranges that a call with many rows is cut into: what its workspace holds beyond that of few rows."""
+    few = c.workspace_bytes(q, n, 32 // (q.shape[1] // c.kv_heads), LONG[-1], window)
+    more = c.workspace_bytes(q, n, rows, LONG[-1], window) - few
+    each = q.shape[0] * q.shape[1] * (4 * c.head_dim + 8)
+    assert more % each == 0
+    return max(1, more // each)
+
+
+@pytest.mark.parametrize("code, dtype", [("int8", "f32"), ("e4m3", "f32"), ("int8", "bf16"), ("e4m3", "f16")])
+@pytest.mark.parametrize("D, H, B", [(64, 8, 32), (128, 8, 64), (256, 4, 16), (80, 8, 128)])
+@pytest.mark.parametrize("window, odd", [(0, False), (0, True), (5000, False)])
+def test_attend_prompts_over_many_tiles(code, dtype, D, H, B, window, odd):
+    """So many tiles of query rows that no key range is cut: a CTA walks up to 257 tiles of 64 keys, through several
+    batches of block ids, around its ring of scales, and adds f32 rows to memory every 4096 keys (at any
+    alignment of the output)."""
+    g = torch.Generator(device="cuda").manual_seed(D + B)
+    c, row = long_cache(D, H, B, code, g)
+    rows = 40
+    q = torch.randn(len(LONG) * rows, 4 * H, D, device="cuda", generator=g).to(DT[dtype])
+    assert ranges(c, q, len(LONG), rows, window) == 1
+    out, lse = attend_long(c, row, LONG, rows, q, window, odd)
+    check_long(c, row, LONG, rows, q, out, lse, window, dtype)
+
+
+@pytest.mark.parametrize("code, dtype", [("int8", "f32"), ("e4m3", "bf16")])
+@pytest.mark.parametrize("D, H, B", [(64, 8, 32), (128, 8, 64), (256, 4, 16)])
+def test_attend_prompts_in_long_ranges(code, dtype, D, H, B):
+    """Ranges of more than 4096 keys: f32 rows are added up in the workspace, then joined."""
+    g = torch.Generator(device="cuda").manual_seed(D)
+    c, row = long_cache(D, H, B, code, g)
+    rows, lens = 40, [16385, 9000, 16384, 5000, 12289]
+    q = torch.randn(len(lens) * rows, 4 * H, D, device="cuda", generator=g).to(DT[dtype])
+    assert 2 <= ranges(c, q, len(lens), rows, 0) <= 3  # of 1025 steps of 16 keys
+    out, lse = attend_long(c, row, lens, rows, q, 0, False)
+    check_long(c, row, lens, rows, q, out, lse, 0, dtype)
+
+
+@pytest.mark.parametrize("code, dtype", [("int8", "f32"), ("e4m3", "f32"), ("int8", "bf16"), ("e4m3", "f16")])
+@pytest.mark.parametrize("D, H, B, n, rows", [(64, 8, 32, 48, 1), (128, 8, 64, 36, 2), (256, 4, 16, 72, 2), (80, 8, 128, 36, 7)])
+@pytest.mark.parametrize("window", [0, 5000])
+def test_attend_steps_over_many_batches(code, dtype, D, H, B, n, rows, window):
+    """So many requests that none is cut far: a warp walks hundreds of steps, through several batches of block ids
+    and scales."""
+    g = torch.Generator(device="cuda").manual_seed(D + n)
+    c, row = long_cache(D, H, B, code, g)
+    lens = (LONG * 6)[:n]
+    q = torch.randn(n * rows, 4 * H, D, device="cuda", generator=g).to(DT[dtype])
+    out, lse = attend_long(c, row, lens, rows, q, window, rows == 2)
+    check_long(c, row, lens, rows, q, out, lse, window, dtype)
