@@ -287,7 +287,7 @@ int gg_rope(const gg_rope_call* call, void* stream);
 int gg_rope_freqs(int scaling, int rot_dim, double theta, double factor, double trained, double low, double high,
                   double* freqs, double* mscale);
 
-/* One scheduler step over `seqs` requests whose cached length goes from old_len[i] to new_len[i]:
+/* One scheduler step over `seqs` (1 or more) requests whose cached length goes from old_len[i] to new_len[i]:
  * the block table, the stack of free blocks and, for every new token, its request, position and
  * cache slot, all on the device. Request i holds blocks table[i][0 .. ceil(len / block_tokens)).
  *   shrinking requests give their blocks back first (request order, then block order), pushed on
@@ -362,7 +362,11 @@ int gg_kv8_append(const gg_kv8_cache* cache, const gg_kv8_append_call* call, voi
  * at position p = lens[i] - (rows of i) + r sees the keys at max(0, p - window + 1) .. p (window 0:
  * from 0): o = sum softmax(scale q k) v; query head h reads key head h / (q heads / kv_heads), at
  * most 1024 to one. A row that sees no key gives zeros. lse (f32, [rows][q heads], or NULL) receives ln sum exp(scale q k),
- * -inf for such a row. out has q's type. Scores, softmax and sums are held in f32.
+ * -inf for such a row. out has q's type. Scores, softmax statistics and sums are held in f32, with these
+ * roundings of what enters the products: f32 queries and weights as two f16 (2^-22 of a value), weights of f16
+ * and bf16 calls as one f16 (2^-11); a weight below 2^-31 of the row's largest may count as 0. f32 requests
+ * with more than 32 pairs of row and head of a key head lose up to 5e-6 of a sum. Value scales that one row
+ * sees lie within 2^100 of one another.
  *   max_rows and max_len are at least every request's number of rows and length (of longer ones,
  *   rows from max_rows on are not computed and keys from max_len on not read); a table entry outside
  *   0 .. num_blocks - 1 hides its keys; rows outside cu_rows[0] .. cu_rows[seqs] - 1 are left as

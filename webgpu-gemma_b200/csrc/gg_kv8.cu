@@ -28,9 +28,10 @@ namespace gg {
 // sums up the requests and finds its part). Bound by the cache's bytes. Each of the four warps
 // streams its own steps through a private cp.async ring (no barriers between warps); the warps'
 // results meet in shared memory at the end, the parts of a unit in gg_kv8_merge_kernel. Four requests
-// of up to 131072 keys, 8 key heads of 128, bf16: 157 us, 6.0 TB/s of codes and scales; 64 requests of
-// up to 8192 keys of one head of 256, f32: 38 us, 3.5 TB/s, of which the start, the first loads and
-// the merge take about 15; one request of 641 keys: 10 us, all of it latency.
+// of up to 131072 keys, 8 key heads of 128, bf16: 156 us, 6.0 TB/s of codes and scales; 64 requests of
+// up to 8192 keys of one head of 256, f32: 39 us, 3.4 TB/s, of which the start, the first loads and
+// the merge take about 15 and the SMs that hold three parts where others hold two some of the rest; one
+// request of 641 keys: 10 us, all of it latency.
 //
 // Both products are transposed, so that the few query rows are the narrow side (N = 8) of an
 // m16n8k16 MMA and the accumulators hold nothing else: S^T = K Q^T (16 keys x 8 rows), then
@@ -39,7 +40,7 @@ namespace gg {
 //
 // An MMA cuts the sum it adds to: measured, 0.9 2^-24 of it an MMA, always towards zero (f32 rows lost
 // 1.1e-4 over 65536 uncut keys, 2.2e-4 over 131072). For f32 rows each step's two MMAs therefore start from
-// zero, and their result is added to O with rounding (64 requests, f32, heads of 256: 39.7 us, 38.6 without). For
+// zero, and their result is added to O with rounding (64 requests, f32, heads of 256: 39.3 us, 38.3 without). For
 // f16 and bf16 rows, 4096 steps of a warp lose 2.2e-4, less than their own rounding, and a part has no
 // more (KV8_LONGEST).
 //
@@ -689,7 +690,11 @@ static Kv8Plan kv8_plan(const gg_kv8_cache& c, const gg_kv8_attention_call& b) {
   const double most = cut ? line / KV8_WARPS : 0;
   p.few_ctas = (int)((most < p.resident ? most : p.resident) + units + line / KV8_LONGEST) + 1;  // parts are at most that many
   p.few_parts = cut ? (size_t)p.few_ctas * rt : 0;
-  if (items > KV8_FEW) {  // one CTA an SM; ranges of at least 512 keys where there are fewer tiles than SMs
+  // One CTA an SM; ranges of at least 512 keys where there are fewer tiles than SMs. Against 256 and 128, merge
+  // included: 512 f32 rows of 4 heads over 1 of 256 at position 0 38.9 / 35.7 / 31.2 us, at 1536 45.1 / 40.2 / 44.2;
+  // bf16, 32 heads over 8 of 128, 64 rows at 4000 34.2 / 35.1 / 37.1, 256 at 0 20.8 / 20.8 / 27.7, 16 at 2000
+  // 27.4 / 24.1 / 23.1. (512 suits the bf16 prompts; f32 ones would gain from shorter ranges.)
+  if (items > KV8_FEW) {
     const int tile = kv8_prompt_tile(c.head_dim);
     p.row_tiles = (int)((items + tile - 1) / tile);
     const long long units = (long long)b.seqs * c.kv_heads * p.row_tiles, n = steps(tile), most = (n + 31) / 32;

@@ -79,8 +79,8 @@ namespace gg {
 // keep their lengths in registers (gg_plan_kernel, 256 threads where that many requests have one
 // each: its barriers are cheaper); more go through the chunks three times (gg_plan_many_kernel).
 // The code runs once, so instruction fetches count: with its loops unrolled by four 1000 requests
-// with 32768 rows took 16.2 us, rolled and with warp reductions 11.4; 64 requests with one row each
-// take 2.9 us (6.1 with the chunked kernel), most of it three dependent rounds of loads.
+// with 32768 rows took 16.2 us, rolled and with warp reductions 10.8; 64 requests with one row each
+// take 2.8 us (6.1 with the chunked kernel), most of it three dependent rounds of loads.
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_CHUNK = 4096;
 constexpr int PLAN_PER = PLAN_CHUNK / PLAN_THREADS;
@@ -427,9 +427,9 @@ __global__ void __launch_bounds__(256) gg_plan_rows_kernel(const gg_block_plan p
 // takes a few rows: it forms their (c, s) once in shared memory -- the angle p w in f64 turns,
 // reduced to [-1/2, 1/2] before the f32 sincospi, because p w of a far position has no correct
 // digits left in f32 -- and applies them to every head of q and k. 8192 rows of 40 heads of 128 in
-// bf16: 30.9 us, 5.4 TB/s; 64 rows of 5 heads of 256 in f32: 2.1 us, one round of loads after a launch.
-// 2047 rows of 32 heads of 96, interleaved f16: 8.2 us, 3.1 TB/s -- too few bytes to fill the memory's
-// latency behind the sincospi.
+// bf16: 31.0 us, 5.4 TB/s; 64 rows of 5 heads of 256 in f32: 2.0 us, one round of loads after a launch.
+// 2047 rows of 32 heads of 96, interleaved f16: 8.5 us, 3.0 TB/s -- the loads of q and k stand behind the
+// barrier that ends the sincospi.
 constexpr int ROPE_THREADS = 256;
 constexpr int ROPE_CS = 1024;  // (c, s) pairs in shared memory
 
@@ -545,8 +545,9 @@ cudaError_t launch_rope(const RopeArgs& a, bool vec, cudaStream_t s) {
 // the first row of a block's run takes the whole run, so the block's scale needs no atomics and
 // no second launch: one pass for the largest value, one that rounds (the rows stay in registers, as
 // they were read; what long runs have above that comes from L1/L2 again). 6300 rows of 8 heads of 128,
-// bf16 to e4m3: 10.9 us, 3.5 TB/s (39 us with a search for each row's run and maxima one value at a
-// time); 64 rows of one head of 256, f32 to int8: 2.6 us, all latency.
+// bf16 to e4m3: 11.5 us, 3.4 TB/s (39 us with a search for each row's run and maxima one value at a
+// time; 10.8 where skipped rows end a run, but then a block could have two); 64 rows of one head of 256,
+// f32 to int8: 2.7 us, all latency.
 constexpr int APPEND_THREADS = 128;
 constexpr int APPEND_GAP = 128;  // rows of a block stand fewer than this apart, as the tokens of the largest block do
 constexpr int KV8_MIN_EXP = -60;

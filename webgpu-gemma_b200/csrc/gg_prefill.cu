@@ -916,8 +916,6 @@ __global__ void __launch_bounds__(PF_THREADS) pf_geglu_kernel(const float* __res
   }
 }
 
-// RoPE table: (cos, sin) of pos * freq_i, freq_i = 1 / theta^(2i/HD), the same f32 expressions
-// the shader evaluates per step (shaders.ts:420-467).
 // One warp per head of a row (grid.x = rows): the planes' sum in plane order, q and k divided by
 // their head's rms. Bound by the planes' bytes; the row stays in registers between sum and norm.
 __global__ void __launch_bounds__(PF_THREADS)
@@ -963,6 +961,8 @@ __global__ void pf_kv8_rows_kernel(const int32_t* __restrict__ seqs, const int32
   for (long long i = i0; i < (long long)n * blocks; i += step) r.table[i] = (seqs ? seqs[i / blocks] : seq) * blocks + (int)(i % blocks);
 }
 
+// RoPE table: (cos, sin) of pos * freq_i, freq_i = 1 / theta^(2i/HD), the same f32 expressions
+// the shader evaluates per step (shaders.ts:420-467).
 __global__ void pf_rope_table_kernel(float theta, int HD, int ctx, float2* out) {
   const int half = HD / 2;
   for (int idx = blockIdx.x * blockDim.x + threadIdx.x; idx < ctx * half; idx += gridDim.x * blockDim.x) {
