@@ -365,7 +365,7 @@ int gg_kv8_append(const gg_kv8_cache* cache, const gg_kv8_append_call* call, voi
  * -inf for such a row. out has q's type. Scores, softmax statistics and sums are held in f32, with these
  * roundings of what enters the products: f32 queries and weights as two f16 (2^-22 of a value), weights of f16
  * and bf16 calls as one f16 (2^-11); a weight below 2^-31 of the row's largest may count as 0. f32 requests
- * with more than 32 pairs of row and head of a key head lose up to 5e-6 of a sum. Value scales that one row
+ * with more than 32 pairs of row and head of a key head lose up to 7e-6 of a sum. Value scales that one row
  * sees lie within 2^100 of one another.
  *   max_rows and max_len are at least every request's number of rows and length (of longer ones,
  *   rows from max_rows on are not computed and keys from max_len on not read); a table entry outside

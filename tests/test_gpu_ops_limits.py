@@ -204,6 +204,27 @@ def test_attend_sums_over_many_keys_of_a_warp(code, D, H, n):
         assert bool(((lse[i, h * G:(h + 1) * G].double() - torch.logsumexp(z, -1)).abs() <= ds[:, 0] + 2.0 ** -20 + 2.0 ** -22 * 12).all())
 
 
+@pytest.mark.parametrize("D, H", [(64, 8), (128, 8), (256, 4)])
+@pytest.mark.parametrize("L", [4095, 4097, 16385])
+def test_attend_sums_of_f32_prompts(D, H, L):
+    """Many f32 rows, positive values and weights alike, between and behind the points where O goes to memory: off
+    by no more than the bound the header gives (7e-6) and the output's rounding."""
+    from gemma_b200 import ops
+    B, n, rows = 64, 12, 40
+    g = torch.Generator(device="cuda").manual_seed(D + L)
+    c = ops.KV8Cache.empty(-(-L // B), B, H, D, "int8")
+    for t, lo in ((c.k_codes, -127), (c.v_codes, 64)):
+        t.copy_(torch.randint(lo, 128, t.shape, device="cuda", generator=g, dtype=torch.int32))
+    c.k_scale.fill_(2.0 ** -20)
+    table = torch.arange(c.num_blocks, dtype=torch.int32, device="cuda").repeat(n, 1)
+    q = torch.randn(n * rows, 4 * H, D, device="cuda", generator=g)
+    out = c.attend(q, torch.arange(n + 1, dtype=torch.int32, device="cuda") * rows, dev([L] * n), table, max_rows=rows, max_len=L)
+    for h in (0, H - 1):
+        k, v = (t[:, h].double().reshape(-1, D)[:L] for t in (c.k_codes, c.v_codes))
+        want = torch.softmax(q[rows - 1, 4 * h:4 * h + 4].double() @ (k * 2.0 ** -20).T * D ** -0.5, -1) @ v
+        assert bool(((out[rows - 1, 4 * h:4 * h + 4].double() - want).abs() <= (7e-6 + 2.0 ** -24) * want).all())
+
+
 @pytest.mark.parametrize("rows, n, L", [(1, 300, 1 << 22), (128, 75, 1 << 22)])
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 def test_attend_sums_over_millions_of_keys(dtype, rows, n, L):
