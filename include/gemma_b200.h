@@ -325,7 +325,8 @@ int gg_plan_blocks(const gg_block_plan* plan, void* stream);
 
 /* A paged KV cache in 8 bits: codes [num_blocks][kv_heads][block_tokens][head_dim], one f32 scale
  * for each (block, head) of K and of V, [num_blocks][kv_heads]; a value is code * scale. Scales are
- * positive, 2^127 at most (or NaN: see the append); they need not be powers of two. Codes are int8 (-127..127) or e4m3 (finite). block_tokens is
+ * positive, 2^127 at most (or NaN: see the append); they need not be powers of two. Codes are int8
+ * (-127..127) or e4m3 (finite). block_tokens is
  * 16, 32, 64 or 128, head_dim a multiple of 16 up to 256, num_blocks * block_tokens below 2^31, all
  * four arrays 16-byte aligned. */
 #define GG_KV8_INT8 0
@@ -371,8 +372,9 @@ int gg_kv8_append(const gg_kv8_cache* cache, const gg_kv8_append_call* call, voi
  *   rows from max_rows on are not computed and keys from max_len on not read); a table entry outside
  *   0 .. num_blocks - 1 hides its keys; rows outside cu_rows[0] .. cu_rows[seqs] - 1 are left as
  *   they were. Waits within the call are bounded: rows whose CTA makes no progress for two seconds are
- *   NaN (the engine reports GG_E_DEVICE, after gg_set_timeout). workspace: gg_kv8_attention_workspace bytes, 16-byte aligned, for this call alone
- *   until it has run (calls that may run at the same time need one each). */
+ *   NaN (the engine reports GG_E_DEVICE, after gg_set_timeout's limit). workspace:
+ *   gg_kv8_attention_workspace bytes, 16-byte aligned, for this call alone until it has run (calls
+ *   that may run at the same time need one each). */
 typedef struct {
   gg_rows q, out;
   float* lse;
